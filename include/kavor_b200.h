@@ -188,6 +188,66 @@ int kvb_prefill_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, cons
                      int64_t out_stride_h, int num_q_heads, int num_kv_heads, int head_dim, float scale,
                      int64_t total_q, int64_t total_k, void* stream);
 
+/* ---------------------------------------------------- 8-bit KV cache (e4m3) */
+
+/* The e4m3 form of the paged cache (no reference counterpart): a page holds
+ * the K rows [block_size, num_kv_heads, 128] as e4m3 bytes, the V rows
+ * likewise, and one e8m0 scale byte per row, [num_kv_heads, block_size] for K
+ * and for V; a held value stands for e4m3 * 2^(byte - 127). `block_stride` and
+ * `scale_block_stride` are the distances in BYTES between consecutive blocks
+ * of the value and of the scale arrays.
+ *
+ * kvb_store_kv_fp8: for every token t with slot_mapping[t] != -1, quantise
+ * key[t] and value[t] ([num_kv_heads, 128] bf16, any 16-byte aligned token and
+ * head strides) into slot slot_mapping[t]. The scale of a row is the smallest
+ * power of two (at least 2^-100; 1 for a zero row) that brings its largest
+ * finite magnitude to at most 448; values are rounded to nearest even,
+ * infinities are held as +-448 of the row's scale, NaN as NaN. The slots of a
+ * call (other than -1) are distinct. Slots outside the cache raise the device
+ * slot error and are skipped. */
+int kvb_store_kv_fp8(const void* key, int64_t key_stride_t, int64_t key_stride_h, const void* value,
+                     int64_t value_stride_t, int64_t value_stride_h, void* k_cache, void* v_cache, void* k_scale,
+                     void* v_scale, int64_t num_blocks, int64_t block_stride, int64_t scale_block_stride,
+                     int block_size, int num_kv_heads, int head_dim, const int32_t* slot_mapping, int num_tokens,
+                     void* stream);
+
+/* Read back whole sequences: token j of sequence b (cu_seqlens_k[b] + j, an
+ * int32 prefix sum [batch + 1]) goes to row cu_seqlens_k[b] + j of k_out and
+ * v_out ([total_k, num_kv_heads, 128] bf16, heads packed), exactly. Rows from
+ * cu_seqlens_k[batch] on are left as they are. A block id outside the pool
+ * raises the device block-table error and gives zeros. */
+int kvb_load_kv_fp8(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                    int64_t num_blocks, int64_t block_stride, int64_t scale_block_stride, int block_size,
+                    int num_kv_heads, int head_dim, const int32_t* block_tables, int64_t block_table_stride,
+                    int max_blocks_per_seq, const int32_t* cu_seqlens_k, int batch, int total_k, void* k_out,
+                    int64_t k_out_stride_t, void* v_out, int64_t v_out_stride_t, void* stream);
+
+/* Attention of drafted tokens over the paged cache (no reference counterpart;
+ * one node per sequence is flash_attention_kvcache.py:80-83's decode).
+ * Sequence b has context_lens[b] tokens in the cache, the last T_b =
+ * cu_seqlens_q[b+1] - cu_seqlens_q[b] of them the nodes of its draft; its
+ * queries are rows cu_seqlens_q[b].. of q [total_q, Hq, 128]. Node i sees every
+ * token before the draft and node j where bit j % 32 of word j / 32 of
+ * tree_mask's row (cu_seqlens_q[b] + i; rows mask_stride words apart,
+ * mask_words of each read; one row may serve all, mask_stride 0) is set; with tree_mask NULL it sees nodes 0..i. A row that
+ * sees nothing gives zeros; values of unseen nodes have no influence, whatever
+ * they are. Output rows past cu_seqlens_q[batch] are left as they are.
+ * The cache is bf16 (k_scale = v_scale = NULL; block_stride in elements, as
+ * kvb_paged_decode_attn) or e4m3 with its scales (strides in bytes, as above).
+ * max_seqlen_q: at least the largest T_b (0 only if there are no rows); it
+ * sizes launches. num_kv_heads divides num_q_heads; block_size is a multiple
+ * of 64; 0 < scale < 1e30. `workspace`: kvb_tree_attn_workspace_size bytes,
+ * 16-byte aligned, its content irrelevant before and after; calls that may
+ * overlap on the GPU need one each. */
+int kvb_tree_attn_workspace_size(int num_q_heads, int num_kv_heads, int max_seqlen_q, size_t* bytes);
+int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t total_q, const void* k_cache,
+                  const void* v_cache, const void* k_scale, const void* v_scale, int64_t num_blocks,
+                  int64_t block_stride, int64_t scale_block_stride, int block_size, const int32_t* block_tables,
+                  int64_t block_table_stride, int max_blocks_per_seq, const int32_t* context_lens,
+                  const int32_t* cu_seqlens_q, int max_seqlen_q, const int32_t* tree_mask, int64_t mask_stride,
+                  int mask_words, void* out, int64_t out_stride_t, int64_t out_stride_h, int batch, int num_q_heads,
+                  int num_kv_heads, int head_dim, float scale, void* workspace, size_t workspace_bytes, void* stream);
+
 /* --------------------------------------------------------------------- GEMM */
 
 /* Bytes of scratch kvb_gemm_bf16 needs for this shape: always 0 (a K split
@@ -373,6 +433,20 @@ int kvb_sample_partial(const void* logits, int64_t row_stride, const float* temp
                        int64_t vocab_total, void* stream);
 int kvb_sample_combine(const float* vals, const int64_t* idxs, int world_size, int64_t* out, int batch,
                        void* stream);
+
+/* Log probabilities of given tokens (no reference counterpart): for every row
+ * of logits [rows, vocab] (dtype 0 bf16, 1 fp16, 2 fp32; row_stride elements)
+ * logprobs[r] = log softmax(logits[r])[tokens[r]], ranks[r] = how many entries
+ * come before the token (higher logit, or the same at a lower index; NaN above
+ * everything), entropy[r] = -sum p log p, and the first top_k (<= 32, <= vocab)
+ * entries in that order, top_ids / top_logprobs [rows, top_k]. fp32 inside.
+ * Entries of -inf have probability 0; a row of only -inf has logprobs -inf and
+ * entropy 0; a row with NaN or +inf has NaN for each. tokens[r] = -1 asks for
+ * no token (logprob 0, rank -1); other ids outside the vocabulary do the same
+ * and raise the device token-id error. */
+int kvb_token_logprobs(const void* logits, int dtype, int64_t row_stride, const int64_t* tokens, int rows, int vocab,
+                       int top_k, float* logprobs, int64_t* ranks, float* entropy, int64_t* top_ids,
+                       float* top_logprobs, void* stream);
 
 #if defined(__GNUC__)
 #pragma GCC visibility pop

@@ -293,6 +293,170 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     return out
 
 
+# ------------------------------------------------------------------ 8-bit KV cache
+class _Launch:
+    """The device and stream of a launch: the tensors' device is made current
+    for the call when it is not, and the stream is torch's current one there."""
+
+    __slots__ = ("index", "prev")
+
+    def __init__(self, device: torch.device):
+        self.index = device.index
+
+    def __enter__(self) -> int:
+        self.prev = torch.cuda.current_device()
+        if self.prev != self.index:
+            torch.cuda.set_device(self.index)
+        return torch.cuda.current_stream(self.index).cuda_stream
+
+    def __exit__(self, *exc) -> None:
+        if self.prev != self.index:
+            torch.cuda.set_device(self.prev)
+
+
+def _on(device: torch.device, t: torch.Tensor, name: str, dtype: torch.dtype) -> None:
+    _cuda(t, name, dtype)
+    _req(t.device == device, f"{name} is on {t.device}, the call's other tensors on {device}")
+
+
+_E4M3 = torch.float8_e4m3fn
+_E8M0 = torch.float8_e8m0fnu
+
+
+def _fp8_cache(k_cache, v_cache, k_scale, v_scale, device) -> tuple[int, int, int, int]:
+    """(num_blocks, block_size, num_kv_heads, head_dim) of an e4m3 cache after the layout checks."""
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _on(device, t, n, _E4M3)
+    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        _on(device, t, n, _E8M0)
+    _req(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
+         "k/v caches must be [num_blocks, block_size, num_kv_heads, head_dim] with the same strides")
+    nblk, bs, hkv, hd = k_cache.shape
+    _req(k_cache.stride(1) == hkv * hd and k_cache.stride(2) == hd and k_cache.stride(3) == 1,
+         "cache rows must be packed")
+    _req(k_scale.shape == (nblk, hkv, bs) and v_scale.shape == (nblk, hkv, bs) and
+         k_scale.stride() == v_scale.stride() and k_scale.stride(1) == bs and k_scale.stride(2) == 1,
+         "scales must be [num_blocks, num_kv_heads, block_size] with packed blocks and the same strides")
+    return nblk, bs, hkv, hd
+
+
+def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                      k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """Quantise key/value [N, Hkv, 128] bf16 rows into the e4m3 cache at slot_mapping (-1: skipped)."""
+    dev = key.device
+    _on(dev, key, "key", _BF16)
+    _on(dev, value, "value", _BF16)
+    _on(dev, slot_mapping, "slot_mapping", torch.int32)
+    nblk, bs, hkv, hd = _fp8_cache(k_cache, v_cache, k_scale, v_scale, dev)
+    _req(key.dim() == 3 and key.shape == value.shape and key.shape[1:] == (hkv, hd),
+         "key/value must be [tokens, num_kv_heads, head_dim]")
+    _req(key.stride(2) == 1 and value.stride(2) == 1, "key/value last dim must be contiguous")
+    n = key.shape[0]
+    _req(slot_mapping.dim() == 1 and slot_mapping.numel() == n and slot_mapping.is_contiguous(),
+         "slot_mapping must have one entry per token")
+    with _Launch(dev) as stream:
+        _lib.call("kvb_store_kv_fp8", key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
+                  value.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                  nblk, k_cache.stride(0), k_scale.stride(0), bs, hkv, hd, slot_mapping.data_ptr(), n, stream)
+
+
+def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                     block_tables: torch.Tensor, cu_seqlens_k: torch.Tensor, total_k: int,
+                     k_out: torch.Tensor | None = None,
+                     v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached rows of whole sequences as contiguous bf16 [total_k, Hkv, 128] tensors."""
+    dev = k_cache.device
+    nblk, bs, hkv, hd = _fp8_cache(k_cache, v_cache, k_scale, v_scale, dev)
+    _on(dev, block_tables, "block_tables", torch.int32)
+    _on(dev, cu_seqlens_k, "cu_seqlens_k", torch.int32)
+    _req(cu_seqlens_k.dim() == 1 and cu_seqlens_k.is_contiguous() and cu_seqlens_k.numel() >= 1,
+         "cu_seqlens_k must be [batch + 1]")
+    batch = cu_seqlens_k.numel() - 1
+    _req(block_tables.dim() == 2 and block_tables.stride(1) == 1 and block_tables.shape[0] == batch,
+         "block_tables must be [batch, max_blocks]")
+    total_k = int(total_k)
+    outs = []
+    for t, n in ((k_out, "k_out"), (v_out, "v_out")):
+        if t is None:
+            t = torch.empty(total_k, hkv, hd, dtype=_BF16, device=dev)
+        _on(dev, t, n, _BF16)
+        _req(t.shape == (total_k, hkv, hd) and t.stride(1) == hd and t.stride(2) == 1,
+             f"{n} must be [total_k, num_kv_heads, head_dim] with packed heads")
+        outs.append(t)
+    with _Launch(dev) as stream:
+        _lib.call("kvb_load_kv_fp8", k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                  nblk, k_cache.stride(0), k_scale.stride(0), bs, hkv, hd, block_tables.data_ptr(),
+                  block_tables.stride(0), block_tables.shape[1], cu_seqlens_k.data_ptr(), batch, total_k,
+                  outs[0].data_ptr(), outs[0].stride(0), outs[1].data_ptr(), outs[1].stride(0), stream)
+    return outs[0], outs[1]
+
+
+# ------------------------------------------------------------------ tree attention
+def tree_workspace_bytes(num_q_heads: int, num_kv_heads: int, max_seqlen_q: int) -> int:
+    n = ctypes.c_size_t(0)
+    _lib.call("kvb_tree_attn_workspace_size", num_q_heads, num_kv_heads, max_seqlen_q, ctypes.byref(n))
+    return int(n.value)
+
+
+def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
+                   context_lens: torch.Tensor, cu_seqlens_q: torch.Tensor, max_seqlen_q: int, scale: float,
+                   tree_mask: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
+                   v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Drafted tokens over the paged cache: q [total_q, Hq, 128] -> [total_q, Hq, 128]."""
+    dev = q.device
+    _on(dev, q, "q", _BF16)
+    _on(dev, block_tables, "block_tables", torch.int32)
+    _on(dev, context_lens, "context_lens", torch.int32)
+    _on(dev, cu_seqlens_q, "cu_seqlens_q", torch.int32)
+    _req(q.dim() == 3 and q.stride(2) == 1, "q must be [total_q, heads, head_dim]")
+    total, hq, hd = q.shape
+    _req((k_scale is None) == (v_scale is None), "k_scale and v_scale come together")
+    if k_scale is not None:
+        nblk, bs, hkv, chd = _fp8_cache(k_cache, v_cache, k_scale, v_scale, dev)
+        sstride = k_scale.stride(0)
+    else:
+        _on(dev, k_cache, "k_cache", _BF16)
+        _on(dev, v_cache, "v_cache", _BF16)
+        _req(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
+             "k/v caches must be [num_blocks, block_size, num_kv_heads, head_dim] with the same strides")
+        nblk, bs, hkv, chd = k_cache.shape
+        _req(k_cache.stride(1) == hkv * chd and k_cache.stride(2) == chd and k_cache.stride(3) == 1,
+             "cache rows must be packed")
+        sstride = 0
+    _req(chd == hd, "q and the cache must share head_dim")
+    batch = context_lens.numel()
+    _req(context_lens.dim() == 1 and context_lens.is_contiguous(), "context_lens must be [batch]")
+    _req(cu_seqlens_q.dim() == 1 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.numel() == batch + 1,
+         "cu_seqlens_q must be [batch + 1]")
+    _req(block_tables.dim() == 2 and block_tables.stride(1) == 1 and block_tables.shape[0] == batch,
+         "block_tables must be [batch, max_blocks]")
+    mask_ptr, mask_stride, words = None, 0, 0
+    if tree_mask is not None:
+        _on(dev, tree_mask, "tree_mask", torch.int32)
+        _req(tree_mask.dim() == 2 and tree_mask.shape[0] == total and tree_mask.stride(1) == 1,
+             "tree_mask must be [total_q, words]")
+        words = tree_mask.shape[1]
+        _req(words * 32 >= max_seqlen_q, "tree_mask rows must hold max_seqlen_q bits")
+        mask_ptr, mask_stride = tree_mask.data_ptr(), tree_mask.stride(0)
+    if out is None:
+        out = torch.empty(total, hq, hd, dtype=_BF16, device=dev)
+    else:
+        _on(dev, out, "out", _BF16)
+        _req(out.shape == q.shape and out.stride(2) == 1, "out must have q's shape and contiguous rows")
+    with _Launch(dev) as stream:
+        # scratch of this call alone (torch's allocator orders its reuse on the stream), so calls on
+        # different streams and captured graphs never share it
+        need = tree_workspace_bytes(hq, hkv, int(max_seqlen_q))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _lib.call("kvb_tree_attn", q.data_ptr(), q.stride(0), q.stride(1), total, k_cache.data_ptr(),
+                  v_cache.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
+                  v_scale.data_ptr() if v_scale is not None else None, nblk, k_cache.stride(0), sstride, bs,
+                  block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(),
+                  cu_seqlens_q.data_ptr(), int(max_seqlen_q), mask_ptr, mask_stride, words, out.data_ptr(),
+                  out.stride(0), out.stride(1), batch, hq, hkv, hd, float(scale), ws.data_ptr(), need, stream)
+    return out
+
+
 # ------------------------------------------------------------------ GEMM
 def gemm_workspace_bytes(M: int, N: int, K: int, splits: int = 0) -> int:
     n = ctypes.c_size_t(0)
@@ -485,3 +649,28 @@ def sample_combine(vals: torch.Tensor, idxs: torch.Tensor, out: torch.Tensor) ->
     world, batch = vals.shape
     _lib.call("kvb_sample_combine", vals.data_ptr(), idxs.data_ptr(), world, out.data_ptr(), batch, _stream())
     return out
+
+
+_LOGIT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0):
+    """(logprobs [N], ranks [N], entropy [N], top_ids [N, k], top_logprobs [N, k]) of logits [N, vocab]."""
+    _cuda(logits, "logits")
+    _req(logits.dtype in _LOGIT_TYPES, f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    _req(logits.dim() == 2 and logits.stride(1) == 1, "logits must be [rows, vocab] with contiguous rows")
+    dev = logits.device
+    _on(dev, token_ids, "token_ids", torch.int64)
+    rows, vocab = logits.shape
+    _req(token_ids.shape == (rows,) and token_ids.is_contiguous(), "token_ids must be [rows]")
+    top_k = int(top_k)
+    _req(0 <= top_k <= min(32, vocab), "top_k must be at most 32 and at most the vocabulary")
+    lp, ent = torch.empty(2, rows, dtype=torch.float32, device=dev).unbind(0)
+    rank = torch.empty(rows, dtype=torch.int64, device=dev)
+    ids = torch.empty(rows, top_k, dtype=torch.int64, device=dev)
+    top = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
+    with _Launch(dev) as stream:
+        _lib.call("kvb_token_logprobs", logits.data_ptr(), _LOGIT_TYPES[logits.dtype],
+                  logits.stride(0) if rows > 1 else vocab, token_ids.data_ptr(), rows, vocab, top_k, lp.data_ptr(),
+                  rank.data_ptr(), ent.data_ptr(), ids.data_ptr(), top.data_ptr(), stream)
+    return lp, rank, ent, ids, top

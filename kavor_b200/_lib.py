@@ -38,6 +38,12 @@ SIGNATURES: dict[str, list] = {
     "kvb_sample": [P, L, P, P, P, I, I, P],
     "kvb_sample_partial": [P, L, P, P, P, P, I, I, L, L, P],
     "kvb_sample_combine": [P, P, I, P, I, P],
+    "kvb_token_logprobs": [P, I, L, P, I, I, I, P, P, P, P, P, P],
+    "kvb_store_kv_fp8": [P, L, L, P, L, L, P, P, P, P, L, L, L, I, I, I, P, I, P],
+    "kvb_load_kv_fp8": [P, P, P, P, L, L, L, I, I, I, P, L, I, P, I, I, P, L, P, L, P],
+    "kvb_tree_attn_workspace_size": [I, I, I, POINTER(c_size_t)],
+    "kvb_tree_attn": [P, L, L, L, P, P, P, P, L, L, L, I, P, L, I, P, P, I, P, L, I, P, L, L, I, I, I, I, F, P,
+                      c_size_t, P],
     "kvb_gemm_workspace_size": [I, I, I, I, POINTER(c_size_t)],
     "kvb_gemm_bf16": [P, L, P, L, P, L, I, I, I, I, P, c_size_t, P],
     "kvb_gemm_plan": [I, I, I, I, I, POINTER(c_int)],
@@ -76,7 +82,7 @@ _QUERIES = {
     "kvb_set_pdl", "kvb_gemm_pair_plan", "kvb_comm_ipc_handle_size", "kvb_comm_area_size", "kvb_comm_attach",
     "kvb_comm_has_multicast", "kvb_comm_set_max_blocks", "kvb_comm_result_rows", "kvb_allreduce_plan", "kvb_comm_create", "kvb_comm_open_peers",
     "kvb_comm_data_buffer", "kvb_comm_destroy", "kvb_gemm_sk_workspace_size", "kvb_gemm_sk_plan",
-    "kvb_gemm_sk_set_plan",
+    "kvb_gemm_sk_set_plan", "kvb_tree_attn_workspace_size",
 }
 # Number of launching entry-point calls made so far (per name); used to count
 # the kernels a captured CUDA graph contains.

@@ -39,6 +39,9 @@ int read_device_error_gemm(unsigned*, int);
 int read_device_error_allreduce(unsigned*, int);
 int read_device_error_gemm_pair(unsigned*, int);
 int read_device_error_gemm_sk(unsigned*, int);
+int read_device_error_kv_fp8(unsigned*, int);
+int read_device_error_tree(unsigned*, int);
+int read_device_error_logprobs(unsigned*, int);
 int set_pdl_trigger_elementwise(int);
 int set_pdl_trigger_decode(int);
 int set_pdl_trigger_prefill(int);
@@ -47,6 +50,9 @@ int set_pdl_trigger_gemm(int);
 int set_pdl_trigger_allreduce(int);
 int set_pdl_trigger_gemm_pair(int);
 int set_pdl_trigger_gemm_sk(int);
+int set_pdl_trigger_kv_fp8(int);
+int set_pdl_trigger_tree(int);
+int set_pdl_trigger_logprobs(int);
 
 }  // namespace kvb
 
@@ -62,7 +68,9 @@ extern "C" int kvb_device_error(unsigned* bits, int clear) {
   int (*readers[])(unsigned*, int) = {kvb::read_device_error_elementwise, kvb::read_device_error_decode,
                                       kvb::read_device_error_prefill, kvb::read_device_error_sampler,
                                       kvb::read_device_error_gemm, kvb::read_device_error_allreduce,
-                                      kvb::read_device_error_gemm_pair, kvb::read_device_error_gemm_sk};
+                                      kvb::read_device_error_gemm_pair, kvb::read_device_error_gemm_sk,
+                                      kvb::read_device_error_kv_fp8, kvb::read_device_error_tree,
+                                      kvb::read_device_error_logprobs};
   for (auto fn : readers) {
     int rc = fn(&w, clear);
     if (rc) return rc;
@@ -77,7 +85,8 @@ extern "C" int kvb_set_pdl(int enable) {
   int (*setters[])(int) = {kvb::set_pdl_trigger_elementwise, kvb::set_pdl_trigger_decode,
                            kvb::set_pdl_trigger_prefill, kvb::set_pdl_trigger_sampler, kvb::set_pdl_trigger_gemm,
                            kvb::set_pdl_trigger_allreduce, kvb::set_pdl_trigger_gemm_pair,
-                           kvb::set_pdl_trigger_gemm_sk};
+                           kvb::set_pdl_trigger_gemm_sk, kvb::set_pdl_trigger_kv_fp8, kvb::set_pdl_trigger_tree,
+                           kvb::set_pdl_trigger_logprobs};
   for (auto fn : setters) {
     int rc = fn(enable);
     if (rc) return rc;

@@ -1,0 +1,243 @@
+// The paged KV cache in 8 bits: quantise on write, read back as bf16.
+//
+// A row (one token, one kv head, 128 values) is held as 128 e4m3 bytes and one
+// e8m0 byte c that stands for the scale 2^(c - 127). With e the smallest whole
+// number such that the row's largest finite magnitude is at most 448 * 2^e
+// (448 is the largest e4m3 value; e is clamped to [-100, 120], 0 for a zero
+// row), the held value is e4m3(x / 2^e), rounded to nearest even. A power of
+// two costs a float format no precision (the relative error of a normal value
+// is 2^-4 at any scale) and makes both directions exact: x / 2^e only changes
+// the exponent, so the one rounding is the e4m3 one, and q * 2^e (4 significant
+// bits) is a bf16 value again. Infinities are held as the row's largest value
+// +-448 * 2^e, NaN as NaN; neither counts for the scale.
+//
+// Both kernels are bound by HBM (and, at a decode batch, by one launch):
+// 16 lanes own one row, 16 bytes of bf16 a lane, so a warp moves whole rows
+// with full-width accesses and the row maximum takes four shuffles.
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "../../include/kavor_b200.h"
+
+KVB_DEFINE_ERROR_WORD(kv_fp8)
+
+namespace kvb {
+namespace {
+
+constexpr int kHD = 128;
+constexpr int kThreads = 256;
+constexpr int kRowLanes = 16;
+constexpr int kRowsPerBlock = kThreads / kRowLanes;
+
+struct CacheRef {
+  uint8_t* k;
+  uint8_t* v;
+  uint8_t* ks;
+  uint8_t* vs;
+  int64_t num_blocks, block_stride, scale_stride;  // strides between blocks, bytes
+  int block_size, hkv;
+};
+
+// Largest finite magnitude of 8 bf16 values, as bf16 bits: for positive
+// floats the order of the bits is the order of the values.
+__device__ __forceinline__ uint32_t finite_max8(const uint4& r) {
+  const uint32_t w[4] = {r.x & 0x7fff7fffu, r.y & 0x7fff7fffu, r.z & 0x7fff7fffu, r.w & 0x7fff7fffu};
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m = __vmaxu2(m, w[i] & ~__vcmpgtu2(w[i], 0x7f7f7f7fu));
+  return max(m & 0xffffu, m >> 16);
+}
+
+// Exponent e of the row's scale from its largest magnitude's bf16 bits:
+// 1.m * 2^x <= 1.75 * 2^8 * 2^e, so e = x - 8, or x - 7 when 1.m > 1.75.
+__device__ __forceinline__ int scale_exponent(uint32_t bits) {
+  if (bits == 0) return 0;
+  const int x = (int)(bits >> 7) - 127;
+  const int e = x - 8 + ((bits & 0x7fu) > 0x60u);
+  return max(e, -100);
+}
+
+__device__ __forceinline__ uint2 quantise8(const uint4& r, int e) {
+  const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+  uint32_t q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float2 f = __bfloat1622float2(h[i]);
+    f.x *= inv;
+    f.y *= inv;
+    q[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+  }
+  return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+}
+
+__global__ void __launch_bounds__(kThreads)
+    store_kv_fp8_kernel(const bf16* __restrict__ key, int64_t k_st, int64_t k_sh, const bf16* __restrict__ value,
+                        int64_t v_st, int64_t v_sh, CacheRef c, const int32_t* __restrict__ slots, int64_t rows) {
+  kernel_entry();
+  const int64_t row = (int64_t)blockIdx.x * kRowsPerBlock + threadIdx.x / kRowLanes;
+  const int lane = threadIdx.x % kRowLanes;
+  const int64_t rr = row < rows ? row : rows - 1;  // every lane takes part in the shuffles
+  const int64_t t = rr / c.hkv;
+  const int h = (int)(rr - t * c.hkv);
+  const int32_t slot = slots[t];
+  const uint4 kr = *reinterpret_cast<const uint4*>(key + t * k_st + h * k_sh + lane * 8);
+  const uint4 vr = *reinterpret_cast<const uint4*>(value + t * v_st + h * v_sh + lane * 8);
+  uint32_t mx = finite_max8(kr) | finite_max8(vr) << 16;
+#pragma unroll
+  for (int o = kRowLanes / 2; o > 0; o >>= 1) mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (row >= rows || slot == -1) return;
+  if (slot < 0 || slot >= c.num_blocks * c.block_size) {
+    if (lane == 0) atomicOr(&g_err_kv_fp8, (unsigned)kErrSlot);
+    return;
+  }
+  const int64_t blk = slot / c.block_size;
+  const int off = slot - (int)(blk * c.block_size);
+  const int ek = scale_exponent(mx & 0xffffu), ev = scale_exponent(mx >> 16);
+  const int64_t at = blk * c.block_stride + ((int64_t)off * c.hkv + h) * kHD + lane * 8;
+  *reinterpret_cast<uint2*>(c.k + at) = quantise8(kr, ek);
+  *reinterpret_cast<uint2*>(c.v + at) = quantise8(vr, ev);
+  if (lane < 2) {
+    const int64_t sat = blk * c.scale_stride + (int64_t)h * c.block_size + off;
+    (lane == 0 ? c.ks : c.vs)[sat] = (uint8_t)((lane == 0 ? ek : ev) + 127);
+  }
+}
+
+__device__ __forceinline__ uint4 dequantise8(uint2 q, float scale) {
+  const uint32_t w[2] = {q.x, q.y};
+  uint32_t out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2_raw hr = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w[i >> 1] >> ((i & 1) * 16)), __NV_E4M3);
+    const float2 f = __half22float2(__half2(hr));
+    out[i] = pack_bf16(f.x * scale, f.y * scale);
+  }
+  return make_uint4(out[0], out[1], out[2], out[3]);
+}
+
+constexpr int kLoadTokens = 32;  // flat tokens per CTA
+
+__global__ void __launch_bounds__(kThreads)
+    load_kv_fp8_kernel(CacheRef c, const int32_t* __restrict__ tables, int64_t bt_stride, int max_blocks,
+                       const int32_t* __restrict__ cu, int batch, int total, bf16* __restrict__ ko, int64_t ko_st,
+                       bf16* __restrict__ vo, int64_t vo_st) {
+  kernel_entry();
+  __shared__ int s_blk[kLoadTokens], s_off[kLoadTokens];
+  const int t0 = blockIdx.x * kLoadTokens;
+  // the sequence of the CTA's first token: how many sequences end at or before it
+  int ended = 0;
+  for (int i0 = 0; i0 < batch; i0 += kThreads) {
+    const int i = i0 + threadIdx.x;
+    ended += __syncthreads_count(i < batch && cu[i + 1] <= t0);
+  }
+  if (threadIdx.x < kLoadTokens) {
+    const int t = t0 + threadIdx.x;
+    int blk = -2, off = 0, b = ended;
+    if (t < total) {
+      while (b < batch && cu[b + 1] <= t) ++b;
+      if (b < batch && t >= cu[b]) {  // rows past the last sequence are left as they are
+        const int pos = t - cu[b];
+        const int col = pos / c.block_size;
+        off = pos - col * c.block_size;
+        blk = col < max_blocks ? tables[(int64_t)b * bt_stride + col] : -1;
+        if (blk < 0 || blk >= c.num_blocks) {
+          atomicOr(&g_err_kv_fp8, (unsigned)kErrBlockTable);
+          blk = -1;
+        }
+      }
+    }
+    s_blk[threadIdx.x] = blk;
+    s_off[threadIdx.x] = off;
+  }
+  __syncthreads();
+  const int lane = threadIdx.x % kRowLanes;
+  for (int r = threadIdx.x / kRowLanes; r < kLoadTokens * c.hkv; r += kRowsPerBlock) {
+    const int tt = r / c.hkv, h = r - tt * c.hkv;
+    const int blk = s_blk[tt];
+    if (blk == -2) continue;
+    uint4 ky = make_uint4(0, 0, 0, 0), vy = ky;
+    if (blk >= 0) {
+      const int64_t at = blk * c.block_stride + ((int64_t)s_off[tt] * c.hkv + h) * kHD + lane * 8;
+      const int64_t sat = blk * c.scale_stride + (int64_t)h * c.block_size + s_off[tt];
+      const uint2 kq = *reinterpret_cast<const uint2*>(c.k + at);
+      const uint2 vq = *reinterpret_cast<const uint2*>(c.v + at);
+      ky = dequantise8(kq, __uint_as_float((uint32_t)c.ks[sat] << 23));
+      vy = dequantise8(vq, __uint_as_float((uint32_t)c.vs[sat] << 23));
+    }
+    const int64_t t = t0 + tt;
+    *reinterpret_cast<uint4*>(ko + t * ko_st + h * kHD + lane * 8) = ky;
+    *reinterpret_cast<uint4*>(vo + t * vo_st + h * kHD + lane * 8) = vy;
+  }
+}
+
+inline bool aligned(const void* p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+// Checks shared by both entry points; fills the reference to the cache.
+int cache_ref(CacheRef* c, const char* who, const void* k, const void* v, const void* ks, const void* vs,
+              int64_t num_blocks, int64_t block_stride, int64_t scale_stride, int block_size, int hkv, int head_dim) {
+  if (num_blocks < 0 || num_blocks >= INT32_MAX || block_size <= 0 || hkv <= 0)
+    return set_error(kInvalid, "%s: bad sizes", who);
+  if (head_dim != kHD) return set_error(kUnsupported, "%s: head_dim must be 128", who);
+  if (!k || !v || !ks || !vs) return set_error(kInvalid, "%s: NULL pointer", who);
+  if (!aligned(k, 16) || !aligned(v, 16) || block_stride % 16)
+    return set_error(kInvalid, "%s: the cache and its block stride must be 16-byte aligned", who);
+  if (block_stride < (int64_t)block_size * hkv * kHD || scale_stride < (int64_t)block_size * hkv)
+    return set_error(kInvalid, "%s: block stride smaller than one block", who);
+  *c = CacheRef{(uint8_t*)k, (uint8_t*)v, (uint8_t*)ks, (uint8_t*)vs, num_blocks, block_stride, scale_stride,
+                block_size, hkv};
+  return kOk;
+}
+
+}  // namespace
+}  // namespace kvb
+
+using namespace kvb;
+
+extern "C" int kvb_store_kv_fp8(const void* key, int64_t key_stride_t, int64_t key_stride_h, const void* value,
+                                int64_t value_stride_t, int64_t value_stride_h, void* k_cache, void* v_cache,
+                                void* k_scale, void* v_scale, int64_t num_blocks, int64_t block_stride,
+                                int64_t scale_block_stride, int block_size, int num_kv_heads, int head_dim,
+                                const int32_t* slot_mapping, int num_tokens, void* stream) {
+  if (num_tokens < 0) return set_error(kInvalid, "kvb_store_kv_fp8: bad sizes");
+  if (num_tokens == 0) return kOk;
+  CacheRef c;
+  int rc = cache_ref(&c, "kvb_store_kv_fp8", k_cache, v_cache, k_scale, v_scale, num_blocks, block_stride,
+                     scale_block_stride, block_size, num_kv_heads, head_dim);
+  if (rc) return rc;
+  if (!key || !value || !slot_mapping) return set_error(kInvalid, "kvb_store_kv_fp8: NULL pointer");
+  if (!aligned(key, 16) || !aligned(value, 16) || key_stride_t % 8 || key_stride_h % 8 || value_stride_t % 8 ||
+      value_stride_h % 8)
+    return set_error(kInvalid, "kvb_store_kv_fp8: key/value rows must be 16-byte aligned");
+  const int64_t rows = (int64_t)num_tokens * num_kv_heads;
+  const int64_t grid = (rows + kRowsPerBlock - 1) / kRowsPerBlock;
+  if (grid > INT32_MAX) return set_error(kUnsupported, "kvb_store_kv_fp8: too many rows");
+  return cuda_status(launch_kernel(store_kv_fp8_kernel, dim3((unsigned)grid), dim3(kThreads), 0, (cudaStream_t)stream,
+                                   (const bf16*)key, key_stride_t, key_stride_h, (const bf16*)value, value_stride_t,
+                                   value_stride_h, c, slot_mapping, rows),
+                     "kvb_store_kv_fp8 launch");
+}
+
+extern "C" int kvb_load_kv_fp8(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                               int64_t num_blocks, int64_t block_stride, int64_t scale_block_stride, int block_size,
+                               int num_kv_heads, int head_dim, const int32_t* block_tables,
+                               int64_t block_table_stride, int max_blocks_per_seq, const int32_t* cu_seqlens_k,
+                               int batch, int total_k, void* k_out, int64_t k_out_stride_t, void* v_out,
+                               int64_t v_out_stride_t, void* stream) {
+  if (batch < 0 || total_k < 0 || max_blocks_per_seq < 0) return set_error(kInvalid, "kvb_load_kv_fp8: bad sizes");
+  if (batch == 0 || total_k == 0) return kOk;
+  CacheRef c;
+  int rc = cache_ref(&c, "kvb_load_kv_fp8", k_cache, v_cache, k_scale, v_scale, num_blocks, block_stride,
+                     scale_block_stride, block_size, num_kv_heads, head_dim);
+  if (rc) return rc;
+  if (!block_tables || !cu_seqlens_k || !k_out || !v_out) return set_error(kInvalid, "kvb_load_kv_fp8: NULL pointer");
+  const int64_t row = (int64_t)num_kv_heads * kHD;
+  if (!aligned(k_out, 16) || !aligned(v_out, 16) || k_out_stride_t % 8 || v_out_stride_t % 8 || k_out_stride_t < row ||
+      v_out_stride_t < row)
+    return set_error(kInvalid, "kvb_load_kv_fp8: output rows must be 16-byte aligned and hold all heads");
+  const int grid = (int)(((int64_t)total_k + kLoadTokens - 1) / kLoadTokens);
+  return cuda_status(launch_kernel(load_kv_fp8_kernel, dim3(grid), dim3(kThreads), 0, (cudaStream_t)stream, c,
+                                   block_tables, block_table_stride, max_blocks_per_seq, cu_seqlens_k, batch, total_k,
+                                   (bf16*)k_out, k_out_stride_t, (bf16*)v_out, v_out_stride_t),
+                     "kvb_load_kv_fp8 launch");
+}

@@ -1,0 +1,174 @@
+// Work partition shared by the tree-attention kernels and their merge.
+//
+// A unit is one (sequence, kv head, block of query rows): it walks the
+// sequence's context in tiles of tokens. The tiles of all units, in the order
+// sequence > kv head > row block, form one line that is cut into `parts`
+// contiguous ranges of equal length, one per CTA: every CTA streams the same
+// number of K/V bytes whatever the lengths of the sequences are, and the host
+// needs none of the device's lengths. A unit cut between CTAs leaves fp32
+// partials (unnormalised rows, running maximum and sum) that the merge joins
+// in order, so results do not depend on timing. Included by tree_attn.cu after
+// its error word.
+#pragma once
+
+#include "common.cuh"
+
+namespace kvb {
+namespace tree {
+
+constexpr int kHD = 128;
+
+struct Args {
+  const bf16* q;
+  int64_t q_st, q_sh;
+  int64_t total_q;
+  const int32_t* tables;
+  int64_t bt_stride;
+  int max_blocks;
+  const int32_t* ctx;
+  const int32_t* cu_q;
+  const uint32_t* mask;  // visibility words of each node, NULL: causal chain
+  int64_t mask_stride;
+  int mask_words;
+  bf16* out;
+  int64_t o_st, o_sh;
+  const uint8_t* ks;
+  const uint8_t* vs;
+  int64_t scale_stride;  // bytes between blocks of the scale arrays
+  int batch, hq, hkv, group;
+  int num_blocks, block_size;
+  int parts, rows, tile;  // CTAs of the attention grid, query rows of a unit, tokens of a tile
+  float* part_o;          // [parts][2][rows][128]
+  float* part_m;          // [parts][2][rows]
+  float* part_l;
+  float scale_log2;
+};
+
+struct Seq {
+  int q0, nodes, len;  // first query row, drafted nodes, tokens in the cache (the nodes included)
+  int tiles, blocks;   // tiles of the context, row blocks
+};
+
+// Sequence b of the batch. Lengths the other arguments cannot serve raise an
+// error bit and are cut: a context to its block table, rows outside the query
+// tensor to none.
+__device__ __forceinline__ Seq seq_of(const Args& a, int b, bool report) {
+  Seq s;
+  s.q0 = a.cu_q[b];
+  const int64_t end = a.cu_q[b + 1];
+  s.len = max(a.ctx[b], 0);
+  if (s.q0 < 0 || end < s.q0 || end > a.total_q) {
+    if (report) atomicOr(&g_err_tree, (unsigned)kErrConfig);
+    s.nodes = 0;
+  } else {
+    s.nodes = (int)(end - s.q0);
+  }
+  const int64_t room = (int64_t)a.max_blocks * a.block_size;
+  if (s.len > room) {
+    if (report) atomicOr(&g_err_tree, (unsigned)kErrBlockTable);
+    s.len = (int)room;
+  }
+  s.tiles = (s.len + a.tile - 1) / a.tile;
+  s.blocks = (int)(((int64_t)s.nodes * a.group + a.rows - 1) / a.rows);
+  return s;
+}
+__device__ __forceinline__ int64_t cost_of(const Args& a, const Seq& s) { return (int64_t)s.tiles * s.blocks * a.hkv; }
+
+// Exclusive prefix of each thread's sum over the block, and the total.
+template <int kThreads>
+__device__ __forceinline__ int64_t block_prefix(int64_t mine, int64_t* total) {
+  __shared__ int64_t warp_sums[kThreads / 32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t incl = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t up = __shfl_up_sync(0xffffffffu, incl, o);
+    if (lane >= o) incl += up;
+  }
+  if (lane == 31) warp_sums[warp] = incl;
+  __syncthreads();
+  int64_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += warp_sums[w];
+    all += warp_sums[w];
+  }
+  *total = all;
+  return before + incl - mine;
+}
+
+__device__ __forceinline__ int64_t part_begin(int64_t total, int parts, int p) { return total * p / parts; }
+
+// Where this CTA's range starts: the sequence, the offset in its tiles, and
+// how many tiles the range has. Every thread of the block calls it.
+struct Start {
+  int b;
+  int64_t off, left;
+};
+template <int kThreads>
+__device__ __forceinline__ Start find_start(const Args& a, int part) {
+  __shared__ Start s_start;
+  const int per = (a.batch + kThreads - 1) / kThreads;
+  const int b0 = min(threadIdx.x * per, a.batch), b1 = min(b0 + per, a.batch);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += cost_of(a, seq_of(a, b, part == 0));
+  int64_t total;
+  int64_t at = block_prefix<kThreads>(mine, &total);
+  const int64_t lo = part_begin(total, a.parts, part), hi = part_begin(total, a.parts, part + 1);
+  if (threadIdx.x == 0) s_start = Start{0, 0, 0};
+  __syncthreads();
+  if (lo < hi && at <= lo && lo < at + mine) {
+    for (int b = b0; b < b1; ++b) {
+      const int64_t c = cost_of(a, seq_of(a, b, false));
+      if (lo < at + c) {
+        s_start = Start{b, lo - at, hi - lo};
+        break;
+      }
+      at += c;
+    }
+  }
+  __syncthreads();
+  return s_start;
+}
+
+// Walks a range segment by segment; a segment is the part of one unit inside it.
+struct Walk {
+  int b;
+  int64_t off, left;
+  Seq s;
+  int h, rb, t0, n;  // kv head, row block, first tile, tiles
+
+  __device__ __forceinline__ Walk(const Args& a, const Start& st) : b(st.b), off(st.off), left(st.left) {
+    if (left > 0) s = seq_of(a, b, false);
+  }
+  __device__ __forceinline__ bool next(const Args& a) {
+    if (left <= 0) return false;
+    while (off >= cost_of(a, s)) {
+      off = 0;
+      if (++b >= a.batch) return false;
+      s = seq_of(a, b, false);
+    }
+    const int64_t u = off / s.tiles;
+    t0 = (int)(off - u * s.tiles);
+    h = (int)(u / s.blocks);
+    rb = (int)(u - (int64_t)h * s.blocks);
+    const int64_t room = s.tiles - t0;
+    n = (int)(left < room ? left : room);
+    off += n;
+    left -= n;
+    return true;
+  }
+  __device__ __forceinline__ bool whole() const { return t0 == 0 && n == s.tiles; }
+  // partial slot of a cut segment: 0 when the unit began in an earlier CTA
+  __device__ __forceinline__ int slot() const { return t0 > 0 ? 0 : 1; }
+};
+
+// Does node i of a sequence see node j?
+__device__ __forceinline__ bool sees(const Args& a, int row, int i, int j) {
+  if (!a.mask) return j <= i;
+  const int w = j >> 5;
+  return w < a.mask_words && (a.mask[(int64_t)row * a.mask_stride + w] >> (j & 31)) & 1u;
+}
+
+}  // namespace tree
+}  // namespace kvb
