@@ -294,70 +294,83 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
 
 
 # ------------------------------------------------------------------ 8-bit KV cache
-class _Launch:
-    """The device and stream of a launch: the tensors' device is made current
-    for the call when it is not, and the stream is torch's current one there."""
-
-    __slots__ = ("index", "prev")
-
-    def __init__(self, device: torch.device):
-        self.index = device.index
-
-    def __enter__(self) -> int:
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.index:
-            torch.cuda.set_device(self.index)
-        return torch.cuda.current_stream(self.index).cuda_stream
-
-    def __exit__(self, *exc) -> None:
-        if self.prev != self.index:
-            torch.cuda.set_device(self.prev)
+_current = torch.cuda.current_device
 
 
-def _on(device: torch.device, t: torch.Tensor, name: str, dtype: torch.dtype) -> None:
-    _cuda(t, name, dtype)
-    _req(t.device == device, f"{name} is on {t.device}, the call's other tensors on {device}")
+def _stream_on(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+def _launch(index: int, name: str, *args) -> None:
+    """Entry point ``name`` on the device of the call's tensors (made current
+    for the call when it is not) and torch's current stream there."""
+    prev = _current()
+    if prev == index:
+        _lib.call(name, *args, _stream_on(index))
+        return
+    torch.cuda.set_device(index)
+    try:
+        _lib.call(name, *args, _stream_on(index))
+    finally:
+        torch.cuda.set_device(prev)
+
+
+def _on(index: int, t: torch.Tensor, name: str, dtype: torch.dtype) -> None:
+    if t.dtype is not dtype or t.get_device() != index:
+        _cuda(t, name, dtype)
+        _req(False, f"{name} is on {t.device}, the call's other tensors on device {index}")
+
+
+def _device_index(t: torch.Tensor, name: str) -> int:
+    index = t.get_device()
+    if index < 0:
+        _cuda(t, name)
+    return index
 
 
 _E4M3 = torch.float8_e4m3fn
 _E8M0 = torch.float8_e8m0fnu
 
 
-def _fp8_cache(k_cache, v_cache, k_scale, v_scale, device) -> tuple[int, int, int, int]:
-    """(num_blocks, block_size, num_kv_heads, head_dim) of an e4m3 cache after the layout checks."""
-    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
-        _on(device, t, n, _E4M3)
-    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
-        _on(device, t, n, _E8M0)
-    _req(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
+def _cache_shape(k_cache: torch.Tensor, v_cache: torch.Tensor) -> torch.Size:
+    shape, stride = k_cache.shape, k_cache.stride()
+    _req(len(shape) == 4 and shape == v_cache.shape and stride == v_cache.stride(),
          "k/v caches must be [num_blocks, block_size, num_kv_heads, head_dim] with the same strides")
-    nblk, bs, hkv, hd = k_cache.shape
-    _req(k_cache.stride(1) == hkv * hd and k_cache.stride(2) == hd and k_cache.stride(3) == 1,
-         "cache rows must be packed")
-    _req(k_scale.shape == (nblk, hkv, bs) and v_scale.shape == (nblk, hkv, bs) and
-         k_scale.stride() == v_scale.stride() and k_scale.stride(1) == bs and k_scale.stride(2) == 1,
+    _req(stride[1:] == (shape[2] * shape[3], shape[3], 1), "cache rows must be packed")
+    return shape
+
+
+def _fp8_cache(index: int, k_cache, v_cache, k_scale, v_scale) -> torch.Size:
+    """(num_blocks, block_size, num_kv_heads, head_dim) of an e4m3 cache after the layout checks."""
+    _on(index, k_cache, "k_cache", _E4M3)
+    _on(index, v_cache, "v_cache", _E4M3)
+    _on(index, k_scale, "k_scale", _E8M0)
+    _on(index, v_scale, "v_scale", _E8M0)
+    shape = _cache_shape(k_cache, v_cache)
+    nblk, bs, hkv, _ = shape
+    stride = k_scale.stride()
+    _req(k_scale.shape == (nblk, hkv, bs) == v_scale.shape and stride == v_scale.stride() and stride[1:] == (bs, 1),
          "scales must be [num_blocks, num_kv_heads, block_size] with packed blocks and the same strides")
-    return nblk, bs, hkv, hd
+    return shape
 
 
 def store_kvcache_fp8(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                       k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
     """Quantise key/value [N, Hkv, 128] bf16 rows into the e4m3 cache at slot_mapping (-1: skipped)."""
-    dev = key.device
-    _on(dev, key, "key", _BF16)
-    _on(dev, value, "value", _BF16)
-    _on(dev, slot_mapping, "slot_mapping", torch.int32)
-    nblk, bs, hkv, hd = _fp8_cache(k_cache, v_cache, k_scale, v_scale, dev)
-    _req(key.dim() == 3 and key.shape == value.shape and key.shape[1:] == (hkv, hd),
+    index = _device_index(key, "key")
+    _on(index, key, "key", _BF16)
+    _on(index, value, "value", _BF16)
+    _on(index, slot_mapping, "slot_mapping", torch.int32)
+    nblk, bs, hkv, hd = _fp8_cache(index, k_cache, v_cache, k_scale, v_scale)
+    shape, kst, vst = key.shape, key.stride(), value.stride()
+    _req(len(shape) == 3 and shape == value.shape and shape[1] == hkv and shape[2] == hd,
          "key/value must be [tokens, num_kv_heads, head_dim]")
-    _req(key.stride(2) == 1 and value.stride(2) == 1, "key/value last dim must be contiguous")
-    n = key.shape[0]
-    _req(slot_mapping.dim() == 1 and slot_mapping.numel() == n and slot_mapping.is_contiguous(),
-         "slot_mapping must have one entry per token")
-    with _Launch(dev) as stream:
-        _lib.call("kvb_store_kv_fp8", key.data_ptr(), key.stride(0), key.stride(1), value.data_ptr(), value.stride(0),
-                  value.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                  nblk, k_cache.stride(0), k_scale.stride(0), bs, hkv, hd, slot_mapping.data_ptr(), n, stream)
+    _req(kst[2] == 1 == vst[2], "key/value last dim must be contiguous")
+    n = shape[0]
+    _req(slot_mapping.shape == (n,) and slot_mapping.is_contiguous(), "slot_mapping must have one entry per token")
+    _launch(index, "kvb_store_kv_fp8", key.data_ptr(), kst[0], kst[1], value.data_ptr(), vst[0], vst[1],
+            k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), nblk, k_cache.stride(0),
+            k_scale.stride(0), bs, hkv, hd, slot_mapping.data_ptr(), n)
 
 
 def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
@@ -365,30 +378,31 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
                      k_out: torch.Tensor | None = None,
                      v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached rows of whole sequences as contiguous bf16 [total_k, Hkv, 128] tensors."""
-    dev = k_cache.device
-    nblk, bs, hkv, hd = _fp8_cache(k_cache, v_cache, k_scale, v_scale, dev)
-    _on(dev, block_tables, "block_tables", torch.int32)
-    _on(dev, cu_seqlens_k, "cu_seqlens_k", torch.int32)
+    index = _device_index(k_cache, "k_cache")
+    nblk, bs, hkv, hd = _fp8_cache(index, k_cache, v_cache, k_scale, v_scale)
+    _on(index, block_tables, "block_tables", torch.int32)
+    _on(index, cu_seqlens_k, "cu_seqlens_k", torch.int32)
     _req(cu_seqlens_k.dim() == 1 and cu_seqlens_k.is_contiguous() and cu_seqlens_k.numel() >= 1,
          "cu_seqlens_k must be [batch + 1]")
     batch = cu_seqlens_k.numel() - 1
     _req(block_tables.dim() == 2 and block_tables.stride(1) == 1 and block_tables.shape[0] == batch,
          "block_tables must be [batch, max_blocks]")
     total_k = int(total_k)
-    outs = []
+    _req(total_k >= 0, "total_k must not be negative")
+    if k_out is None:
+        k_out = torch.empty(total_k, hkv, hd, dtype=_BF16, device=k_cache.device)
+    if v_out is None:
+        v_out = torch.empty(total_k, hkv, hd, dtype=_BF16, device=k_cache.device)
     for t, n in ((k_out, "k_out"), (v_out, "v_out")):
-        if t is None:
-            t = torch.empty(total_k, hkv, hd, dtype=_BF16, device=dev)
-        _on(dev, t, n, _BF16)
-        _req(t.shape == (total_k, hkv, hd) and t.stride(1) == hd and t.stride(2) == 1,
+        _on(index, t, n, _BF16)
+        _req(t.shape == (total_k, hkv, hd) and t.stride()[1:] == (hd, 1),
              f"{n} must be [total_k, num_kv_heads, head_dim] with packed heads")
-        outs.append(t)
-    with _Launch(dev) as stream:
-        _lib.call("kvb_load_kv_fp8", k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
-                  nblk, k_cache.stride(0), k_scale.stride(0), bs, hkv, hd, block_tables.data_ptr(),
-                  block_tables.stride(0), block_tables.shape[1], cu_seqlens_k.data_ptr(), batch, total_k,
-                  outs[0].data_ptr(), outs[0].stride(0), outs[1].data_ptr(), outs[1].stride(0), stream)
-    return outs[0], outs[1]
+    _launch(index, "kvb_load_kv_fp8", k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            nblk, k_cache.stride(0), k_scale.stride(0), bs, hkv, hd, block_tables.data_ptr(), block_tables.stride(0),
+            block_tables.shape[1], cu_seqlens_k.data_ptr(), batch, total_k, k_out.data_ptr(),
+            k_out.stride(0) if total_k > 1 else hkv * hd, v_out.data_ptr(),
+            v_out.stride(0) if total_k > 1 else hkv * hd)
+    return k_out, v_out
 
 
 # ------------------------------------------------------------------ tree attention
@@ -403,57 +417,53 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
                    tree_mask: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
                    v_scale: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Drafted tokens over the paged cache: q [total_q, Hq, 128] -> [total_q, Hq, 128]."""
-    dev = q.device
-    _on(dev, q, "q", _BF16)
-    _on(dev, block_tables, "block_tables", torch.int32)
-    _on(dev, context_lens, "context_lens", torch.int32)
-    _on(dev, cu_seqlens_q, "cu_seqlens_q", torch.int32)
-    _req(q.dim() == 3 and q.stride(2) == 1, "q must be [total_q, heads, head_dim]")
+    index = _device_index(q, "q")
+    _on(index, q, "q", _BF16)
+    _on(index, block_tables, "block_tables", torch.int32)
+    _on(index, context_lens, "context_lens", torch.int32)
+    _on(index, cu_seqlens_q, "cu_seqlens_q", torch.int32)
+    _req(q.dim() == 3, "q must be [total_q, heads, head_dim]")
     total, hq, hd = q.shape
+    qst = q.stride()
+    _req(qst[2] == 1, "q must have contiguous rows")
     _req((k_scale is None) == (v_scale is None), "k_scale and v_scale come together")
     if k_scale is not None:
-        nblk, bs, hkv, chd = _fp8_cache(k_cache, v_cache, k_scale, v_scale, dev)
-        sstride = k_scale.stride(0)
+        nblk, bs, hkv, chd = _fp8_cache(index, k_cache, v_cache, k_scale, v_scale)
+        ks_ptr, vs_ptr, sstride = k_scale.data_ptr(), v_scale.data_ptr(), k_scale.stride(0)
     else:
-        _on(dev, k_cache, "k_cache", _BF16)
-        _on(dev, v_cache, "v_cache", _BF16)
-        _req(k_cache.dim() == 4 and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(),
-             "k/v caches must be [num_blocks, block_size, num_kv_heads, head_dim] with the same strides")
-        nblk, bs, hkv, chd = k_cache.shape
-        _req(k_cache.stride(1) == hkv * chd and k_cache.stride(2) == chd and k_cache.stride(3) == 1,
-             "cache rows must be packed")
-        sstride = 0
+        _on(index, k_cache, "k_cache", _BF16)
+        _on(index, v_cache, "v_cache", _BF16)
+        nblk, bs, hkv, chd = _cache_shape(k_cache, v_cache)
+        ks_ptr, vs_ptr, sstride = None, None, 0
     _req(chd == hd, "q and the cache must share head_dim")
     batch = context_lens.numel()
     _req(context_lens.dim() == 1 and context_lens.is_contiguous(), "context_lens must be [batch]")
-    _req(cu_seqlens_q.dim() == 1 and cu_seqlens_q.is_contiguous() and cu_seqlens_q.numel() == batch + 1,
-         "cu_seqlens_q must be [batch + 1]")
+    _req(cu_seqlens_q.shape == (batch + 1,) and cu_seqlens_q.is_contiguous(), "cu_seqlens_q must be [batch + 1]")
     _req(block_tables.dim() == 2 and block_tables.stride(1) == 1 and block_tables.shape[0] == batch,
          "block_tables must be [batch, max_blocks]")
+    max_seqlen_q = int(max_seqlen_q)
     mask_ptr, mask_stride, words = None, 0, 0
     if tree_mask is not None:
-        _on(dev, tree_mask, "tree_mask", torch.int32)
+        _on(index, tree_mask, "tree_mask", torch.int32)
         _req(tree_mask.dim() == 2 and tree_mask.shape[0] == total and tree_mask.stride(1) == 1,
              "tree_mask must be [total_q, words]")
         words = tree_mask.shape[1]
         _req(words * 32 >= max_seqlen_q, "tree_mask rows must hold max_seqlen_q bits")
         mask_ptr, mask_stride = tree_mask.data_ptr(), tree_mask.stride(0)
     if out is None:
-        out = torch.empty(total, hq, hd, dtype=_BF16, device=dev)
+        out = torch.empty(total, hq, hd, dtype=_BF16, device=q.device)
     else:
-        _on(dev, out, "out", _BF16)
+        _on(index, out, "out", _BF16)
         _req(out.shape == q.shape and out.stride(2) == 1, "out must have q's shape and contiguous rows")
-    with _Launch(dev) as stream:
-        # scratch of this call alone (torch's allocator orders its reuse on the stream), so calls on
-        # different streams and captured graphs never share it
-        need = tree_workspace_bytes(hq, hkv, int(max_seqlen_q))
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-        _lib.call("kvb_tree_attn", q.data_ptr(), q.stride(0), q.stride(1), total, k_cache.data_ptr(),
-                  v_cache.data_ptr(), k_scale.data_ptr() if k_scale is not None else None,
-                  v_scale.data_ptr() if v_scale is not None else None, nblk, k_cache.stride(0), sstride, bs,
-                  block_tables.data_ptr(), block_tables.stride(0), block_tables.shape[1], context_lens.data_ptr(),
-                  cu_seqlens_q.data_ptr(), int(max_seqlen_q), mask_ptr, mask_stride, words, out.data_ptr(),
-                  out.stride(0), out.stride(1), batch, hq, hkv, hd, float(scale), ws.data_ptr(), need, stream)
+    # scratch of this call alone (torch's allocator orders its reuse on the stream), so calls on
+    # different streams and captured graphs never share it
+    need = tree_workspace_bytes(hq, hkv, max_seqlen_q)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    ost = out.stride()
+    _launch(index, "kvb_tree_attn", q.data_ptr(), qst[0], qst[1], total, k_cache.data_ptr(), v_cache.data_ptr(),
+            ks_ptr, vs_ptr, nblk, k_cache.stride(0), sstride, bs, block_tables.data_ptr(), block_tables.stride(0),
+            block_tables.shape[1], context_lens.data_ptr(), cu_seqlens_q.data_ptr(), max_seqlen_q, mask_ptr,
+            mask_stride, words, out.data_ptr(), ost[0], ost[1], batch, hq, hkv, hd, float(scale), ws.data_ptr(), need)
     return out
 
 
@@ -656,21 +666,21 @@ _LOGIT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0):
     """(logprobs [N], ranks [N], entropy [N], top_ids [N, k], top_logprobs [N, k]) of logits [N, vocab]."""
-    _cuda(logits, "logits")
-    _req(logits.dtype in _LOGIT_TYPES, f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    index = _device_index(logits, "logits")
+    kind = _LOGIT_TYPES.get(logits.dtype)
+    _req(kind is not None, f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
     _req(logits.dim() == 2 and logits.stride(1) == 1, "logits must be [rows, vocab] with contiguous rows")
-    dev = logits.device
-    _on(dev, token_ids, "token_ids", torch.int64)
+    _on(index, token_ids, "token_ids", torch.int64)
     rows, vocab = logits.shape
     _req(token_ids.shape == (rows,) and token_ids.is_contiguous(), "token_ids must be [rows]")
     top_k = int(top_k)
-    _req(0 <= top_k <= min(32, vocab), "top_k must be at most 32 and at most the vocabulary")
-    lp, ent = torch.empty(2, rows, dtype=torch.float32, device=dev).unbind(0)
-    rank = torch.empty(rows, dtype=torch.int64, device=dev)
-    ids = torch.empty(rows, top_k, dtype=torch.int64, device=dev)
-    top = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
-    with _Launch(dev) as stream:
-        _lib.call("kvb_token_logprobs", logits.data_ptr(), _LOGIT_TYPES[logits.dtype],
-                  logits.stride(0) if rows > 1 else vocab, token_ids.data_ptr(), rows, vocab, top_k, lp.data_ptr(),
-                  rank.data_ptr(), ent.data_ptr(), ids.data_ptr(), top.data_ptr(), stream)
-    return lp, rank, ent, ids, top
+    _req(0 <= top_k <= 32 and top_k <= vocab, "top_k must be at most 32 and at most the vocabulary")
+    dev = logits.device
+    # two allocations: the whole numbers and the 32-bit values
+    whole = torch.empty(rows * (1 + top_k), dtype=torch.int64, device=dev)
+    real = torch.empty(rows * (2 + top_k), dtype=torch.float32, device=dev)
+    at, rt = whole.data_ptr(), real.data_ptr()
+    _launch(index, "kvb_token_logprobs", logits.data_ptr(), kind, logits.stride(0) if rows > 1 else vocab,
+            token_ids.data_ptr(), rows, vocab, top_k, rt, at, rt + 4 * rows, at + 8 * rows, rt + 8 * rows)
+    return (real[:rows], whole[:rows], real[rows:2 * rows], whole[rows:].view(rows, top_k),
+            real[2 * rows:].view(rows, top_k))

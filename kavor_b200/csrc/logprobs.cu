@@ -1,5 +1,5 @@
 // Log probabilities of given tokens, their ranks, each row's entropy and its
-// most likely alternatives, from the logits.
+// most likely alternatives, from one pass over the logits.
 //
 // With m = max x, S = sum e^(x - m), T = sum e^(x - m) (x - m):
 //   logprob_i = (x_i - m) - log S,   entropy = log S - T / S
@@ -8,6 +8,17 @@
 // logprob -inf and entropy 0. A row with a NaN or +inf has NaN for each.
 // Order of the entries: higher logit first, NaN above everything, the lower
 // index on ties (-0 equals +0); rank counts the entries before the token.
+//
+// A cluster of 1..8 CTAs takes a row, each CTA a contiguous part of it in
+// 16-byte vectors, four per thread in flight. Every thread keeps its own
+// reference r near its maximum (moved only when an entry passes r + 10, so the
+// usual vector costs no rescale) and sums S and T against it in 32 bits, with
+// packed 2 x fp32 arithmetic. The alternatives come from the same pass: the
+// k-th largest of the threads' first maxima is a lower bound of the k-th
+// largest entry, so only entries at or above it go to a short list in shared
+// memory (a few hundred of 150 thousand), which warps sort and merge in
+// 32-entry runs. The rank is counted only in vectors whose maximum reaches the
+// token's logit.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -15,108 +26,571 @@
 
 KVB_DEFINE_ERROR_WORD(logprobs)
 
+#include "tcgen05.cuh"
+
 namespace kvb {
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 256;
+constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
+constexpr int kCap = 2048;      // entries of the candidate list
+constexpr float kSlack = 10.f;  // how far an entry may pass a thread's reference
+constexpr float kLog2e = 1.4426950408889634f;
 
-__device__ __forceinline__ float as_float(float x) { return x; }
-__device__ __forceinline__ float as_float(bf16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
+// ------------------------------------------------------------ element types
+template <typename T>
+struct Vec;
+template <>
+struct Vec<float> {
+  static constexpr int kN = 4;
+  static __device__ __forceinline__ float max(const uint4& r) {
+    float a, b;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(__uint_as_float(r.x)), "f"(__uint_as_float(r.y)));
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(__uint_as_float(r.z)), "f"(__uint_as_float(r.w)));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
+    return a;
+  }
+  static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+    v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
+  }
+  static __device__ __forceinline__ float one(const float* p) { return *p; }
+};
+template <>
+struct Vec<bf16> {
+  static constexpr int kN = 8;
+  static __device__ __forceinline__ float max(const uint4& r) {
+    uint32_t a, b;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(r.x), "r"(r.y));
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(r.z), "r"(r.w));
+    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+    float hi = __uint_as_float(a & 0xffff0000u), lo = __uint_as_float(a << 16);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(lo));
+    return hi;
+  }
+  static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] = __uint_as_float(w[i] << 16);
+      v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  static __device__ __forceinline__ float one(const bf16* p) { return __bfloat162float(*p); }
+};
+template <>
+struct Vec<__half> {
+  static constexpr int kN = 8;
+  static __device__ __forceinline__ float max(const uint4& r) {
+    uint32_t a, b;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(r.x), "r"(r.y));
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(r.z), "r"(r.w));
+    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
+    float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(f.x) : "f"(f.y));
+    return f.x;
+  }
+  static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = __half22float2(h[i]);
+      v[2 * i] = f.x;
+      v[2 * i + 1] = f.y;
+    }
+  }
+  static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+};
 
-// Whole number whose order is the order of the logits: NaN highest.
+// ------------------------------------------------------------------- order
+// Whole number whose order is the order of the logits: NaN highest, -0 = +0.
 __device__ __forceinline__ uint32_t order_of(float x) {
   if (x != x) return 0xffffffffu;
-  const uint32_t u = __float_as_uint(x + 0.f);  // -0 becomes +0
+  const uint32_t u = __float_as_uint(x + 0.f);
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// Entries in order: larger is earlier. Distinct for every index.
+__device__ __forceinline__ float value_of(uint32_t o) {
+  if (o == 0xffffffffu) return NAN;
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+// Entries in order: larger is earlier. Distinct for every index, never 0.
 __device__ __forceinline__ uint64_t key_of(float x, int i) {
   return (uint64_t)order_of(x) << 32 | (uint32_t)(0x7fffffff - i);
 }
 
-template <typename T, typename Op>
-__device__ __forceinline__ T block_reduce(T v, Op op, T* sm) {
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
+
+// One step of a bitonic network over the lanes: the pair (lane, lane ^ o)
+// keeps its larger key in the lower lane (desc) or in the higher one.
+__device__ __forceinline__ uint64_t exchange(uint64_t v, int o, bool desc) {
+  const uint64_t w = shfl_xor64(v, o);
+  const bool take_max = ((threadIdx.x & o) == 0) == desc;
+  return (v > w) == take_max ? v : w;
+}
+__device__ __forceinline__ uint64_t sort32(uint64_t v) {  // descending over the lanes
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v = op(v, __shfl_xor_sync(0xffffffffu, v, o));
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = v;
-  __syncthreads();
-  v = sm[0];
+  for (int k = 2; k <= 32; k <<= 1)
 #pragma unroll
-  for (int w = 1; w < kThreads / 32; ++w) v = op(v, sm[w]);
+    for (int o = k >> 1; o > 0; o >>= 1) v = exchange(v, o, (lane & k) == 0);
+  return v;
+}
+// The 32 largest of two descending runs, descending.
+__device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b) {
+  const uint64_t rb = __shfl_sync(0xffffffffu, b, 31 - (threadIdx.x & 31));
+  uint64_t v = a > rb ? a : rb;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = exchange(v, o, true);
   return v;
 }
 
+// ------------------------------------------------------------------ shared
+struct Stats {
+  float m, s, t;
+  unsigned rank, bad;
+};
+struct Shared {
+  uint64_t list[kCap];
+  uint64_t run[kWarps][32];
+  uint64_t top[32];     // this CTA's largest entries, descending, padded with 0
+  Stats warp[kWarps];
+  Stats cta;
+  unsigned count;
+  float thr;
+};
+
+// The 32 largest keys of the block, each warp holding one descending run;
+// the result is in every lane of warp 0 and in sh.top.
+__device__ __forceinline__ void block_merge(Shared& sh, uint64_t v, int runs) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int half = runs >> 1; half > 0; half >>= 1) {
+    if (warp >= half && warp < 2 * half) sh.run[warp][lane] = v;
+    __syncthreads();
+    if (warp < half) v = merge32(v, sh.run[warp + half][lane]);
+  }
+  if (warp == 0) sh.top[lane] = v;
+  __syncthreads();
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void un2(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+
+// One thread's sums against its reference r. S and T hold two partial sums each.
+struct Sums {
+  float r = 0.f, lim = -INFINITY, m = -INFINITY;  // entries above lim move r; lim = -inf: nothing finite seen yet
+  uint64_t S = 0, T = 0;
+  bool bad = false;
+
+  // called before a group whose largest entry is vm > lim, or NaN
+  __device__ __forceinline__ void move(float vm) {
+    if (!(vm < INFINITY)) {  // NaN or +inf
+      bad = true;
+      return;
+    }
+    if (lim != -INFINITY) {
+      const float d = fmaxf(r - vm, -200.f), f = ex2(d * kLog2e);
+      const uint64_t ff = pk2(f, f);
+      T = mul2(fma2(S, pk2(d, d), T), ff);
+      S = mul2(S, ff);
+    }
+    r = vm;
+    lim = vm + kSlack;
+  }
+  template <int N>
+  __device__ __forceinline__ void add(const float* v) {
+    const uint64_t nr = pk2(-r, -r);
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+      float z0, z1, y0, y1;
+      un2(add2(pk2(v[i], v[i + 1]), nr), z0, z1);
+      // keeps p z = 0 for -inf: 2^-288 is 0
+      const uint64_t z = pk2(fmaxf(z0, -200.f), fmaxf(z1, -200.f));
+      un2(mul2(z, pk2(kLog2e, kLog2e)), y0, y1);
+      const uint64_t p = pk2(ex2(y0), ex2(y1));
+      S = add2(S, p);
+      T = fma2(p, z, T);
+    }
+  }
+};
+
+// Entries of a group that come before the token (value t at index tok), the
+// group's first index being i.
+template <int N>
+__device__ __forceinline__ unsigned ahead_of(const float* v, int i, float t, int tok) {
+  unsigned n = 0;
+  if (t != t) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) n += v[j] != v[j] && i + j < tok;
+  } else if (i + N <= tok) {  // ties are before it
+#pragma unroll
+    for (int j = 0; j < N; ++j) n += !(v[j] < t);
+  } else if (i > tok) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) n += !(v[j] <= t);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) n += !(v[j] < t) && (v[j] != t || i + j < tok);
+  }
+  return n;
+}
+
+__device__ __forceinline__ void push(Shared& sh, float x, int i) {
+  const unsigned at = atomicAdd(&sh.count, 1u);
+  if (at < kCap) sh.list[at] = key_of(x, i);
+}
+
+// One CTA's part of a row: vectors [v0, v1) of the aligned body, and for the
+// first CTA the entries before and after the body.
 template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    logprobs_kernel(const T* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ tokens, int vocab,
-                    int top, float* __restrict__ logprob, int64_t* __restrict__ rank, float* __restrict__ entropy,
-                    int64_t* __restrict__ top_ids, float* __restrict__ top_lp) {
-  kernel_entry();
-  __shared__ uint64_t sm_u[kThreads / 32];
-  __shared__ float sm_f[kThreads / 32];
-  const T* x = logits + (int64_t)blockIdx.x * row_stride;
-  const auto add = [](float a, float b) { return a + b; };
-  const auto umax = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
-  const auto uadd = [](uint64_t a, uint64_t b) { return a + b; };
-  const int64_t tok = tokens[blockIdx.x];
-  const bool has = tok >= 0 && tok < vocab;
-  if (!has && tok != -1 && threadIdx.x == 0) atomicOr(&g_err_logprobs, (unsigned)kErrTokenId);
-  const float xt = has ? as_float(x[tok]) : 0.f;
-  const uint64_t kt = has ? key_of(xt, (int)tok) : ~0ull;
-  float m = -INFINITY;
-  uint64_t ahead = 0, best = 0;
-  for (int i = threadIdx.x; i < vocab; i += kThreads) {
-    const float v = as_float(x[i]);
-    m = v != v || m != m ? NAN : fmaxf(m, v);
-    const uint64_t k = key_of(v, i);
-    best = k > best ? k : best;
-    ahead += k > kt;
+struct Part {
+  const T* x;
+  const uint4* body;
+  int head, v0, v1, vocab, edges;  // edges: entries outside the body (0 except for the first CTA)
+  __device__ __forceinline__ int edge_index(int e) const {
+    return e < head ? e : vocab - (edges - e);
   }
-  m = block_reduce(m, [](float a, float b) { return a != a || b != b ? NAN : fmaxf(a, b); }, sm_f);
-  ahead = block_reduce(ahead, uadd, sm_u);
-  const float ref = m == -INFINITY ? 0.f : m;
-  float S = 0.f, E = 0.f;
-  for (int i = threadIdx.x; i < vocab; i += kThreads) {
-    const float z = as_float(x[i]) - ref;
-    const float p = expf(z);
-    S += p;
-    E += p == 0.f ? 0.f : p * z;
+};
+
+// Everything at or above thr goes to the list.
+template <typename T>
+__device__ __noinline__ void collect(Shared& sh, const Part<T>& p, float thr) {
+  constexpr int N = Vec<T>::kN;
+  for (int v = p.v0 + threadIdx.x; v < p.v1; v += kThreads) {
+    const uint4 raw = p.body[v];
+    if (Vec<T>::max(raw) < thr) continue;
+    float f[N];
+    Vec<T>::unpack(raw, f);
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (!(f[j] < thr)) push(sh, f[j], p.head + v * N + j);
   }
-  S = block_reduce(S, add, sm_f);
-  E = block_reduce(E, add, sm_f);
-  const float lse = logf(S);
-  if (threadIdx.x == 0) {
-    logprob[blockIdx.x] = has ? (xt == -INFINITY && m == m && m != INFINITY ? -INFINITY : xt - ref - lse) : 0.f;
-    rank[blockIdx.x] = has ? (int64_t)ahead : -1;
-    entropy[blockIdx.x] = m == -INFINITY ? 0.f : lse - E / S;
+  if (threadIdx.x < p.edges) {
+    const int i = p.edge_index(threadIdx.x);
+    const float f = Vec<T>::one(p.x + i);
+    if (!(f < thr)) push(sh, f, i);
   }
-  uint64_t last = ~0ull;
-  for (int j = 0; j < top; ++j) {
-    if (j > 0) {
-      best = 0;
-      for (int i = threadIdx.x; i < vocab; i += kThreads) {
-        const uint64_t k = key_of(as_float(x[i]), i);
-        if (k < last && k > best) best = k;
+}
+
+// The top entries by one scan per entry: for rows in which more than the list
+// holds tie for a place.
+template <typename T>
+__device__ __noinline__ void top_by_scans(Shared& sh, const Part<T>& p, int top) {
+  constexpr int N = Vec<T>::kN;
+  uint64_t last = ~0ull, mine = 0;
+  for (int k = 0; k < top; ++k) {
+    uint64_t best = 0;
+    for (int v = p.v0 + threadIdx.x; v < p.v1; v += kThreads) {
+      float f[N];
+      Vec<T>::unpack(p.body[v], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const uint64_t key = key_of(f[j], p.head + v * N + j);
+        if (key < last && key > best) best = key;
       }
     }
-    last = block_reduce(best, umax, sm_u);
-    if (threadIdx.x == 0) {
-      const int id = 0x7fffffff - (int)(uint32_t)last;
-      const float v = as_float(x[id]);
-      top_ids[(int64_t)blockIdx.x * top + j] = id;
-      top_lp[(int64_t)blockIdx.x * top + j] = v == -INFINITY && m == m && m != INFINITY ? -INFINITY : v - ref - lse;
+    if (threadIdx.x < p.edges) {
+      const int i = p.edge_index(threadIdx.x);
+      const uint64_t key = key_of(Vec<T>::one(p.x + i), i);
+      if (key < last && key > best) best = key;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      const uint64_t w = shfl_xor64(best, o);
+      best = w > best ? w : best;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) sh.run[threadIdx.x >> 5][0] = best;
+    __syncthreads();
+    last = 0;
+    for (int w = 0; w < kWarps; ++w) last = sh.run[w][0] > last ? sh.run[w][0] : last;
+    if ((threadIdx.x & 31) == k) mine = last;
+    if (last == 0) break;  // the part has no more entries
+  }
+  if (threadIdx.x < 32) sh.top[threadIdx.x] = mine;
+  __syncthreads();
+}
+
+// Sorts the list's entries into sh.top.
+__device__ __forceinline__ void sort_list(Shared& sh, unsigned n) {
+  uint64_t best = 0;
+  for (unsigned b = (threadIdx.x >> 5) * 32; b < n; b += kThreads) {  // uniform for a warp
+    const unsigned at = b + (threadIdx.x & 31);
+    const uint64_t v = sort32(at < n ? sh.list[at] : 0ull);
+    best = b < kThreads ? v : merge32(best, v);
+  }
+  block_merge(sh, best, kWarps);
+}
+
+__device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
+  Stats o;
+  o.m = fmaxf(a.m, b.m);
+  o.rank = a.rank + b.rank;
+  o.bad = a.bad | b.bad;
+  const float da = a.m == -INFINITY ? -200.f : fmaxf(a.m - o.m, -200.f);
+  const float db = b.m == -INFINITY ? -200.f : fmaxf(b.m - o.m, -200.f);
+  const float fa = ex2(da * kLog2e), fb = ex2(db * kLog2e);
+  o.s = a.s * fa + b.s * fb;
+  o.t = (a.t + da * a.s) * fa + (b.t + db * b.s) * fb;
+  return o;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 4)
+    logprobs_kernel(const T* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ tokens, int vocab,
+                    int top, int parts, float* __restrict__ logprob, int64_t* __restrict__ rank,
+                    float* __restrict__ entropy, int64_t* __restrict__ top_ids, float* __restrict__ top_lp) {
+  kernel_entry();
+  constexpr int N = Vec<T>::kN;
+  __shared__ Shared sh;
+  const int row = blockIdx.x / parts, part = blockIdx.x - row * parts;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Part<T> p;
+  p.x = logits + (int64_t)row * row_stride;
+  p.vocab = vocab;
+  const int mis = (int)(((uintptr_t)p.x & 15) / sizeof(T));
+  p.head = min(mis ? N - mis : 0, vocab);
+  const int nvec = (vocab - p.head) / N;
+  p.body = reinterpret_cast<const uint4*>(p.x + p.head);
+  p.edges = part == 0 ? vocab - nvec * N : 0;  // < 2 N
+  p.v0 = (int)((int64_t)nvec * part / parts);
+  p.v1 = (int)((int64_t)nvec * (part + 1) / parts);
+
+  const int64_t tk = tokens[row];
+  const bool has = tk >= 0 && tk < vocab;
+  const int tok = has ? (int)tk : 0;
+  const float t = Vec<T>::one(p.x + tok);
+  if (threadIdx.x == 0) {
+    sh.count = 0;
+    if (!has && tk != -1 && part == 0) atomicOr(&g_err_logprobs, (unsigned)kErrTokenId);
+  }
+
+  // block b of 256 vectors: a step takes one from each quarter of the part, so
+  // the first step samples all of it
+  const int quarter = ((p.v1 - p.v0 + kThreads - 1) / kThreads + 3) / 4;
+  Sums s;
+  unsigned ahead = 0;
+  float thr = INFINITY;
+  for (int step = 0; step < quarter; ++step) {
+    uint4 raw[4];
+    bool in[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int v = p.v0 + (u * quarter + step) * kThreads + threadIdx.x;
+      in[u] = v < p.v1;
+      raw[u] = in[u] ? __ldcs(p.body + v) : make_uint4(0, 0, 0, 0);
+    }
+    float vm[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) vm[u] = in[u] ? Vec<T>::max(raw[u]) : -INFINITY;
+    if (step == 0 && top > 0) {
+      uint64_t best = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (in[u]) {
+          const uint64_t key = key_of(vm[u], 0);
+          best = key > best ? key : best;
+        }
+      block_merge(sh, sort32(best), kWarps);
+      const uint64_t kth = sh.top[top - 1];
+      thr = kth == 0 ? -INFINITY : value_of((uint32_t)(kth >> 32));
+      if (thr != thr) thr = INFINITY;  // enough NaN entries: only they (and +inf) can be among the first
+      __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (!in[u]) continue;
+      const int i = p.head + (p.v0 + (u * quarter + step) * kThreads + threadIdx.x) * N;
+      float f[N];
+      Vec<T>::unpack(raw[u], f);
+      if (!(vm[u] <= s.lim)) s.move(vm[u]);
+      s.m = fmaxf(s.m, vm[u]);
+      s.template add<N>(f);
+      if (has && !(vm[u] < t)) ahead += ahead_of<N>(f, i, t, tok);
+      if (top > 0 && !(vm[u] < thr)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (!(f[j] < thr)) push(sh, f[j], i + j);
+      }
     }
   }
+  if (quarter == 0) thr = -INFINITY;  // no vectors: every edge entry is a candidate
+  if (quarter == 0) __syncthreads();
+  if (threadIdx.x < p.edges) {
+    const int i = p.edge_index(threadIdx.x);
+    const float f[2] = {Vec<T>::one(p.x + i), -INFINITY};
+    if (!(f[0] <= s.lim)) s.move(f[0]);
+    s.m = fmaxf(s.m, f[0]);
+    s.add<2>(f);
+    if (has) ahead += ahead_of<1>(f, i, t, tok);
+    if (top > 0 && !(f[0] < thr)) push(sh, f[0], i);
+  }
+
+  // ------------------------------------------------------ join the sums
+  Stats st;
+  {
+    float s0, s1, t0, t1;
+    un2(s.S, s0, s1);
+    un2(s.T, t0, t1);
+    // from the thread's reference to its maximum
+    const float d = s.lim == -INFINITY ? 0.f : fminf(s.r - s.m, 0.f), f = ex2(d * kLog2e);
+    st.m = s.bad ? INFINITY : s.m;
+    st.s = (s0 + s1) * f;
+    st.t = (t0 + t1 + d * (s0 + s1)) * f;
+    st.rank = ahead;
+    st.bad = s.bad;
+    if (s.lim == -INFINITY) st.m = -INFINITY, st.s = st.t = 0.f;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stats w;
+    w.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    w.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    w.t = __shfl_xor_sync(0xffffffffu, st.t, o);
+    w.rank = __shfl_xor_sync(0xffffffffu, st.rank, o);
+    w.bad = __shfl_xor_sync(0xffffffffu, st.bad, o);
+    st = join(st, w);
+  }
+  if (lane == 0) sh.warp[warp] = st;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kWarps; ++w) st = join(st, sh.warp[w]);
+    sh.cta = st;
+  }
+
+  // ------------------------------------------------- the part's top entries
+  if (top > 0) {
+    unsigned n = sh.count;
+    bool scans = false;
+    for (int tries = 0; n > kCap; ++tries) {
+      // more candidates than the list holds: raise the bound to the list's own
+      // k-th largest and look again; a tie, or entries that rise along the row
+      // and so overflow again, go without the list
+      sort_list(sh, kCap);
+      const float next = value_of((uint32_t)(sh.top[top - 1] >> 32));
+      __syncthreads();
+      if (!(next > thr) || tries == 2) {
+        scans = true;
+        break;
+      }
+      thr = next;
+      if (threadIdx.x == 0) sh.count = 0;
+      __syncthreads();
+      collect(sh, p, thr);
+      __syncthreads();
+      n = sh.count;
+    }
+    if (scans)
+      top_by_scans(sh, p, top);
+    else
+      sort_list(sh, n);
+  } else {
+    __syncthreads();
+  }
+
+  // -------------------------------------------------------- join the cluster
+  if (parts > 1) {
+    tc::cluster_sync_all();
+    if (part == 0) {
+      if (warp < parts) {
+        const uint32_t top_at = tc::map_to_rank(smem_u32(&sh.top[lane]), warp);
+        uint64_t v;
+        asm volatile("ld.shared::cluster.b64 %0, [%1];" : "=l"(v) : "r"(top_at) : "memory");
+        sh.run[warp][lane] = v;
+        if (lane < (int)(sizeof(Stats) / 4)) {
+          const uint32_t at = tc::map_to_rank(smem_u32(reinterpret_cast<uint32_t*>(&sh.cta) + lane), warp);
+          uint32_t w;
+          asm volatile("ld.shared::cluster.b32 %0, [%1];" : "=r"(w) : "r"(at) : "memory");
+          reinterpret_cast<uint32_t*>(&sh.warp[warp])[lane] = w;
+        }
+      }
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        Stats a = sh.warp[0];
+        for (int c = 1; c < parts; ++c) a = join(a, sh.warp[c]);
+        sh.cta = a;
+      }
+      const uint64_t v = warp < parts ? sh.run[warp][lane] : 0;
+      __syncthreads();
+      block_merge(sh, v, parts);
+    }
+    tc::cluster_sync_all();  // the other CTAs' shared memory is read until here
+    if (part != 0) return;
+  }
+  if (warp == 0) {
+    const Stats a = sh.cta;
+    const float lse = logf(a.s);
+    const auto lp_of = [&](float x) { return a.bad ? NAN : x == -INFINITY ? -INFINITY : (x - a.m) - lse; };
+    if (lane == 0) {
+      logprob[row] = has ? lp_of(t) : 0.f;
+      rank[row] = has ? (int64_t)a.rank : -1;
+      entropy[row] = a.bad ? NAN : a.m == -INFINITY ? 0.f : lse - a.t / a.s;
+    }
+    if (lane < top) {
+      const uint64_t k = sh.top[lane];
+      top_ids[(int64_t)row * top + lane] = 0x7fffffff - (int)(uint32_t)k;
+      top_lp[(int64_t)row * top + lane] = lp_of(value_of((uint32_t)(k >> 32)));
+    }
+  }
+}
+
+// CTAs per row: one when the rows alone give every SM its four, else as many
+// (of 2, 4, 8, the portable cluster sizes) as still fit one wave and leave
+// each CTA a step's worth of vectors.
+int parts_for(int rows, int vectors) {
+  const int slots = 4 * device_sm_count();
+  int parts = 1;
+  while (parts < 8 && (int64_t)rows * parts * 2 <= slots && vectors / (parts * 2) >= kThreads) parts *= 2;
+  return parts;
 }
 
 template <typename T>
 int launch(const void* logits, int64_t row_stride, const int64_t* tokens, int rows, int vocab, int top, float* logprob,
            int64_t* rank, float* entropy, int64_t* top_ids, float* top_lp, cudaStream_t st) {
-  return cuda_status(launch_kernel(logprobs_kernel<T>, dim3(rows), dim3(kThreads), 0, st, (const T*)logits, row_stride,
-                                   tokens, vocab, top, logprob, rank, entropy, top_ids, top_lp),
+  const int parts = parts_for(rows, vocab / Vec<T>::kN);
+  if ((int64_t)rows * parts > INT32_MAX) return set_error(kUnsupported, "kvb_token_logprobs: too many rows");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)rows * parts);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  unsigned n = 0;
+  attr[n].id = cudaLaunchAttributeClusterDimension;
+  attr[n].val.clusterDim.x = (unsigned)parts;
+  attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+  ++n;
+  if (pdl_enabled()) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
+  }
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  return cuda_status(cudaLaunchKernelEx(&cfg, logprobs_kernel<T>, (const T*)logits, row_stride, tokens, vocab, top,
+                                        parts, logprob, rank, entropy, top_ids, top_lp),
                      "kvb_token_logprobs launch");
 }
 
