@@ -15,10 +15,10 @@
 // usual vector costs no rescale) and sums S and T against it in 32 bits, with
 // packed 2 x fp32 arithmetic. The alternatives come from the same pass: the
 // k-th largest of the threads' first maxima is a lower bound of the k-th
-// largest entry, so only entries at or above it go to a short list in shared
-// memory (a few hundred of 150 thousand), which warps sort and merge in
-// 32-entry runs. The rank is counted only in vectors whose maximum reaches the
-// token's logit.
+// largest entry, so only vectors that reach it are noted in a short list in
+// shared memory (a few hundred of 19 thousand) and looked at again at the end,
+// when warps sort and merge their entries in 32-entry runs. The rank is counted
+// only in vectors whose maximum reaches the token's logit.
 #include <cuda_fp16.h>
 
 #include "common.cuh"
@@ -55,7 +55,22 @@ struct Vec<float> {
     v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
   }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
+  // entries above t (kOrEqual: or equal to it), NaN among them
+  template <bool kOrEqual>
+  static __device__ __forceinline__ unsigned above(const uint4& r, float t) {
+    float v[4];
+    unpack(r, v);
+    unsigned n = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) n += kOrEqual ? !(v[j] < t) : !(v[j] <= t);
+    return n;
+  }
 };
+
+// one bit per 16-bit half of four compare masks
+__device__ __forceinline__ unsigned count_masks(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __popc((a & 0x00010001u) | (b & 0x00020002u) | (c & 0x00040004u) | (d & 0x00080008u));
+}
 template <>
 struct Vec<bf16> {
   static constexpr int kN = 8;
@@ -77,6 +92,13 @@ struct Vec<bf16> {
     }
   }
   static __device__ __forceinline__ float one(const bf16* p) { return __bfloat162float(*p); }
+  template <bool kOrEqual>
+  static __device__ __forceinline__ unsigned above(const uint4& r, float t) {
+    const __nv_bfloat162 tt = __float2bfloat162_rn(t);  // exact: t is one of the entries
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+    return kOrEqual ? count_masks(__hgeu2_mask(h[0], tt), __hgeu2_mask(h[1], tt), __hgeu2_mask(h[2], tt), __hgeu2_mask(h[3], tt))
+                    : count_masks(__hgtu2_mask(h[0], tt), __hgtu2_mask(h[1], tt), __hgtu2_mask(h[2], tt), __hgtu2_mask(h[3], tt));
+  }
 };
 template <>
 struct Vec<__half> {
@@ -100,6 +122,13 @@ struct Vec<__half> {
     }
   }
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
+  template <bool kOrEqual>
+  static __device__ __forceinline__ unsigned above(const uint4& r, float t) {
+    const __half2 tt = __float2half2_rn(t);  // exact: t is one of the entries
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    return kOrEqual ? count_masks(__hgeu2_mask(h[0], tt), __hgeu2_mask(h[1], tt), __hgeu2_mask(h[2], tt), __hgeu2_mask(h[3], tt))
+                    : count_masks(__hgtu2_mask(h[0], tt), __hgtu2_mask(h[1], tt), __hgtu2_mask(h[2], tt), __hgtu2_mask(h[3], tt));
+  }
 };
 
 // ------------------------------------------------------------------- order
@@ -150,13 +179,13 @@ struct Stats {
   unsigned rank, bad;
 };
 struct Shared {
-  uint64_t list[kCap];
+  uint64_t list[kCap];  // candidates
+  int vecs[kCap];       // vectors that hold one
   uint64_t run[kWarps][32];
   uint64_t top[32];     // this CTA's largest entries, descending, padded with 0
   Stats warp[kWarps];
   Stats cta;
-  unsigned count;
-  float thr;
+  unsigned count, noted;
 };
 
 // The 32 largest keys of the block, each warp holding one descending run;
@@ -237,25 +266,10 @@ struct Sums {
   }
 };
 
-// Entries of a group that come before the token (value t at index tok), the
-// group's first index being i.
-template <int N>
-__device__ __forceinline__ unsigned ahead_of(const float* v, int i, float t, int tok) {
-  unsigned n = 0;
-  if (t != t) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) n += v[j] != v[j] && i + j < tok;
-  } else if (i + N <= tok) {  // ties are before it
-#pragma unroll
-    for (int j = 0; j < N; ++j) n += !(v[j] < t);
-  } else if (i > tok) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) n += !(v[j] <= t);
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) n += !(v[j] < t) && (v[j] != t || i + j < tok);
-  }
-  return n;
+// Does entry (v, i) come before the token (value t at index tok)?
+__device__ __forceinline__ bool is_ahead(float v, int i, float t, int tok) {
+  if (t != t) return v != v && i < tok;
+  return !(v < t) && (v != t || i < tok);
 }
 
 __device__ __forceinline__ void push(Shared& sh, float x, int i) {
@@ -275,15 +289,38 @@ struct Part {
   }
 };
 
-// Everything at or above thr goes to the list.
+// The rare paths of a vector read it again instead of keeping the loop's
+// registers: inlined four times they made the loop miss the instruction cache.
+template <typename T>
+__device__ __noinline__ unsigned ahead_one_by_one(const Part<T>& p, int v, float t, int tok) {
+  constexpr int N = Vec<T>::kN;
+  unsigned n = 0;
+#pragma unroll 1
+  for (int j = 0; j < N; ++j) n += is_ahead(Vec<T>::one(p.x + p.head + v * N + j), p.head + v * N + j, t, tok);
+  return n;
+}
+
+// Notes a vector that holds a candidate.
+__device__ __forceinline__ void note(Shared& sh, int v) {
+  const unsigned at = atomicAdd(&sh.noted, 1u);
+  if (at < kCap) sh.vecs[at] = v;
+}
+
+// Every vector with an entry at or above thr is noted.
 template <typename T>
 __device__ __noinline__ void collect(Shared& sh, const Part<T>& p, float thr) {
+  for (int v = p.v0 + threadIdx.x; v < p.v1; v += kThreads)
+    if (!(Vec<T>::max(p.body[v]) < thr)) note(sh, v);
+}
+
+// The entries at or above thr of the first n noted vectors, and of the edges, go to the list.
+template <typename T>
+__device__ __noinline__ void expand(Shared& sh, const Part<T>& p, unsigned n, float thr) {
   constexpr int N = Vec<T>::kN;
-  for (int v = p.v0 + threadIdx.x; v < p.v1; v += kThreads) {
-    const uint4 raw = p.body[v];
-    if (Vec<T>::max(raw) < thr) continue;
+  for (unsigned a = threadIdx.x; a < n; a += kThreads) {
+    const int v = sh.vecs[a];
     float f[N];
-    Vec<T>::unpack(raw, f);
+    Vec<T>::unpack(p.body[v], f);
 #pragma unroll
     for (int j = 0; j < N; ++j)
       if (!(f[j] < thr)) push(sh, f[j], p.head + v * N + j);
@@ -293,6 +330,7 @@ __device__ __noinline__ void collect(Shared& sh, const Part<T>& p, float thr) {
     const float f = Vec<T>::one(p.x + i);
     if (!(f < thr)) push(sh, f, i);
   }
+  __syncthreads();
 }
 
 // The top entries by one scan per entry: for rows in which more than the list
@@ -384,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   const int tok = has ? (int)tk : 0;
   const float t = Vec<T>::one(p.x + tok);
   if (threadIdx.x == 0) {
-    sh.count = 0;
+    sh.count = sh.noted = 0;
     if (!has && tk != -1 && part == 0) atomicOr(&g_err_logprobs, (unsigned)kErrTokenId);
   }
 
@@ -423,30 +461,32 @@ __global__ void __launch_bounds__(kThreads, 4)
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       if (!in[u]) continue;
-      const int i = p.head + (p.v0 + (u * quarter + step) * kThreads + threadIdx.x) * N;
+      const int v = p.v0 + (u * quarter + step) * kThreads + threadIdx.x, i = p.head + v * N;
       float f[N];
       Vec<T>::unpack(raw[u], f);
       if (!(vm[u] <= s.lim)) s.move(vm[u]);
       s.m = fmaxf(s.m, vm[u]);
       s.template add<N>(f);
-      if (has && !(vm[u] < t)) ahead += ahead_of<N>(f, i, t, tok);
-      if (top > 0 && !(vm[u] < thr)) {
-#pragma unroll
-        for (int j = 0; j < N; ++j)
-          if (!(f[j] < thr)) push(sh, f[j], i + j);
+      if (has && !(vm[u] < t)) {
+        // a vector before the token counts its ties, one after it does not
+        if (t == t && i + N <= tok)
+          ahead += Vec<T>::template above<true>(raw[u], t);
+        else if (t == t && i > tok)
+          ahead += Vec<T>::template above<false>(raw[u], t);
+        else
+          ahead += ahead_one_by_one(p, v, t, tok);
       }
+      if (!(vm[u] < thr)) note(sh, v);
     }
   }
   if (quarter == 0) thr = -INFINITY;  // no vectors: every edge entry is a candidate
-  if (quarter == 0) __syncthreads();
   if (threadIdx.x < p.edges) {
     const int i = p.edge_index(threadIdx.x);
     const float f[2] = {Vec<T>::one(p.x + i), -INFINITY};
     if (!(f[0] <= s.lim)) s.move(f[0]);
     s.m = fmaxf(s.m, f[0]);
     s.add<2>(f);
-    if (has) ahead += ahead_of<1>(f, i, t, tok);
-    if (top > 0 && !(f[0] < thr)) push(sh, f[0], i);
+    if (has) ahead += is_ahead(f[0], i, t, tok);
   }
 
   // ------------------------------------------------------ join the sums
@@ -483,30 +523,27 @@ __global__ void __launch_bounds__(kThreads, 4)
 
   // ------------------------------------------------- the part's top entries
   if (top > 0) {
-    unsigned n = sh.count;
-    bool scans = false;
-    for (int tries = 0; n > kCap; ++tries) {
-      // more candidates than the list holds: raise the bound to the list's own
+    for (int tries = 0;; ++tries) {
+      const unsigned noted = sh.noted;
+      expand(sh, p, min(noted, (unsigned)kCap), thr);
+      const unsigned n = sh.count;
+      sort_list(sh, min(n, (unsigned)kCap));
+      if (noted <= kCap && n <= kCap) break;
+      // more candidates than the lists hold: raise the bound to the list's own
       // k-th largest and look again; a tie, or entries that rise along the row
-      // and so overflow again, go without the list
-      sort_list(sh, kCap);
+      // and so overflow again, go without the lists
       const float next = value_of((uint32_t)(sh.top[top - 1] >> 32));
       __syncthreads();
       if (!(next > thr) || tries == 2) {
-        scans = true;
+        top_by_scans(sh, p, top);
         break;
       }
       thr = next;
-      if (threadIdx.x == 0) sh.count = 0;
+      if (threadIdx.x == 0) sh.count = sh.noted = 0;
       __syncthreads();
       collect(sh, p, thr);
       __syncthreads();
-      n = sh.count;
     }
-    if (scans)
-      top_by_scans(sh, p, top);
-    else
-      sort_list(sh, n);
   } else {
     __syncthreads();
   }
