@@ -3,7 +3,7 @@
 //
 // With m = max x, S = sum e^(x - m), T = sum e^(x - m) (x - m):
 //   logprob_i = (x_i - m) - log S,   entropy = log S - T / S
-// (both terms of the entropy are non-negative, so nothing cancels). An entry of
+// (summed against a reference within 10 of the maximum, so at most 10 cancels). An entry of
 // -inf has probability 0 and adds 0 to both sums; a row of only -inf has
 // logprob -inf and entropy 0. A row with a NaN or +inf has NaN for each.
 // Order of the entries: higher logit first, NaN above everything, the lower
@@ -44,6 +44,11 @@ struct Vec;
 template <>
 struct Vec<float> {
   static constexpr int kN = 4;
+  static constexpr uint32_t kNegInf = 0xff800000u;
+  static constexpr float kLowest = -3.402823466e38f;
+  static __device__ __forceinline__ uint32_t floor_word(uint32_t w) {
+    return __float_as_uint(fmaxf(__uint_as_float(w), kLowest));
+  }
   static __device__ __forceinline__ float max(const uint4& r) {
     float a, b;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(__uint_as_float(r.x)), "f"(__uint_as_float(r.y)));
@@ -74,6 +79,13 @@ __device__ __forceinline__ unsigned count_masks(uint32_t a, uint32_t b, uint32_t
 template <>
 struct Vec<bf16> {
   static constexpr int kN = 8;
+  static constexpr uint32_t kNegInf = 0xff80ff80u;
+  static constexpr float kLowest = -3.38953139e38f;
+  static __device__ __forceinline__ uint32_t floor_word(uint32_t w) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xff7fff7fu));
+    return r;
+  }
   static __device__ __forceinline__ float max(const uint4& r) {
     uint32_t a, b;
     asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(r.x), "r"(r.y));
@@ -103,6 +115,13 @@ struct Vec<bf16> {
 template <>
 struct Vec<__half> {
   static constexpr int kN = 8;
+  static constexpr uint32_t kNegInf = 0xfc00fc00u;
+  static constexpr float kLowest = -65504.f;
+  static __device__ __forceinline__ uint32_t floor_word(uint32_t w) {
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xfbfffbffu));
+    return r;
+  }
   static __device__ __forceinline__ float max(const uint4& r) {
     uint32_t a, b;
     asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(r.x), "r"(r.y));
@@ -175,7 +194,7 @@ __device__ __forceinline__ uint64_t merge32(uint64_t a, uint64_t b) {
 
 // ------------------------------------------------------------------ shared
 struct Stats {
-  float m, s, t;
+  float m, s, t;  // reference (the largest of the threads'), sums against it; m = -inf: nothing finite
   unsigned rank, bad;
 };
 struct Shared {
@@ -230,7 +249,7 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 
 // One thread's sums against its reference r. S and T hold two partial sums each.
 struct Sums {
-  float r = 0.f, lim = -INFINITY, m = -INFINITY;  // entries above lim move r; lim = -inf: nothing finite seen yet
+  float r = 0.f, lim = -INFINITY;  // entries above lim move r; lim = -inf: nothing finite seen yet
   uint64_t S = 0, T = 0;
   bool bad = false;
 
@@ -249,15 +268,14 @@ struct Sums {
     r = vm;
     lim = vm + kSlack;
   }
+  // finite entries (p = 0 for the far ones)
   template <int N>
   __device__ __forceinline__ void add(const float* v) {
     const uint64_t nr = pk2(-r, -r);
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      float z0, z1, y0, y1;
-      un2(add2(pk2(v[i], v[i + 1]), nr), z0, z1);
-      // keeps p z = 0 for -inf: 2^-288 is 0
-      const uint64_t z = pk2(fmaxf(z0, -200.f), fmaxf(z1, -200.f));
+      const uint64_t z = add2(pk2(v[i], v[i + 1]), nr);
+      float y0, y1;
       un2(mul2(z, pk2(kLog2e, kLog2e)), y0, y1);
       const uint64_t p = pk2(ex2(y0), ex2(y1));
       S = add2(S, p);
@@ -265,6 +283,16 @@ struct Sums {
     }
   }
 };
+
+// A vector's entries, -inf as the type's lowest value: its weight is 0 beside
+// any larger entry, and 0 * z stays 0. (Parts where nothing is larger, or where
+// z could overflow, are summed again entry by entry.)
+template <typename T>
+__device__ __forceinline__ void unpack_finite(const uint4& raw, float* f) {
+  Vec<T>::unpack(make_uint4(Vec<T>::floor_word(raw.x), Vec<T>::floor_word(raw.y), Vec<T>::floor_word(raw.z),
+                            Vec<T>::floor_word(raw.w)),
+                 f);
+}
 
 // Does entry (v, i) come before the token (value t at index tok)?
 __device__ __forceinline__ bool is_ahead(float v, int i, float t, int tok) {
@@ -289,14 +317,13 @@ struct Part {
   }
 };
 
-// The rare paths of a vector read it again instead of keeping the loop's
-// registers: inlined four times they made the loop miss the instruction cache.
+// Entries of the vector at x (first index i) that come before the token, for the
+// one vector that holds it and for a NaN token.
 template <typename T>
-__device__ __noinline__ unsigned ahead_one_by_one(const Part<T>& p, int v, float t, int tok) {
-  constexpr int N = Vec<T>::kN;
+__device__ __noinline__ unsigned ahead_one_by_one(const T* x, int i, float t, int tok) {
   unsigned n = 0;
 #pragma unroll 1
-  for (int j = 0; j < N; ++j) n += is_ahead(Vec<T>::one(p.x + p.head + v * N + j), p.head + v * N + j, t, tok);
+  for (int j = 0; j < Vec<T>::kN; ++j) n += is_ahead(Vec<T>::one(x + j), i + j, t, tok);
   return n;
 }
 
@@ -396,6 +423,58 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
   return o;
 }
 
+__device__ __forceinline__ Stats stats_of(const Sums& s, unsigned ahead) {
+  float s0, s1, t0, t1;
+  un2(s.S, s0, s1);
+  un2(s.T, t0, t1);
+  const bool none = s.lim == -INFINITY;
+  return Stats{none ? -INFINITY : s.r, none ? 0.f : s0 + s1, none ? 0.f : t0 + t1, ahead, (unsigned)s.bad};
+}
+
+// The block's statistics, in every thread; a fixed order of joins.
+__device__ __forceinline__ Stats block_join(Shared& sh, Stats st) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    Stats w;
+    w.m = __shfl_xor_sync(0xffffffffu, st.m, o);
+    w.s = __shfl_xor_sync(0xffffffffu, st.s, o);
+    w.t = __shfl_xor_sync(0xffffffffu, st.t, o);
+    w.rank = __shfl_xor_sync(0xffffffffu, st.rank, o);
+    w.bad = __shfl_xor_sync(0xffffffffu, st.bad, o);
+    st = join(st, w);
+  }
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = st;
+  __syncthreads();
+  st = sh.warp[0];
+  for (int w = 1; w < kWarps; ++w) st = join(st, sh.warp[w]);
+  return st;
+}
+
+// The part's sums again, entry by entry, for parts of which the largest entry
+// is the type's lowest value (-inf must not count beside it) or so large that
+// differences overflow.
+template <typename T>
+__device__ __noinline__ Stats sum_one_by_one(Shared& sh, const Part<T>& p, unsigned ahead) {
+  float m = -INFINITY, S = 0.f, E = 0.f;
+  for (int pass = 0; pass < 2; ++pass) {
+    const auto take = [&](float v) {
+      if (v == -INFINITY) return;
+      if (pass == 0) {
+        m = fmaxf(m, v);
+      } else {
+        const float z = fmaxf(v - m, -200.f), w = ex2(z * kLog2e);
+        S += w;
+        E += w * z;
+      }
+    };
+    for (int i = p.head + p.v0 * Vec<T>::kN + threadIdx.x; i < p.head + p.v1 * Vec<T>::kN; i += kThreads)
+      take(Vec<T>::one(p.x + i));
+    if (threadIdx.x < p.edges) take(Vec<T>::one(p.x + p.edge_index(threadIdx.x)));
+  }
+  return block_join(sh, Stats{m, S, E, ahead, 0u});
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4)
     logprobs_kernel(const T* __restrict__ logits, int64_t row_stride, const int64_t* __restrict__ tokens, int vocab,
@@ -406,21 +485,18 @@ __global__ void __launch_bounds__(kThreads, 4)
   __shared__ Shared sh;
   const int row = blockIdx.x / parts, part = blockIdx.x - row * parts;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  Part<T> p;
-  p.x = logits + (int64_t)row * row_stride;
-  p.vocab = vocab;
-  const int mis = (int)(((uintptr_t)p.x & 15) / sizeof(T));
-  p.head = min(mis ? N - mis : 0, vocab);
-  const int nvec = (vocab - p.head) / N;
-  p.body = reinterpret_cast<const uint4*>(p.x + p.head);
-  p.edges = part == 0 ? vocab - nvec * N : 0;  // < 2 N
-  p.v0 = (int)((int64_t)nvec * part / parts);
-  p.v1 = (int)((int64_t)nvec * (part + 1) / parts);
+  const T* x = logits + (int64_t)row * row_stride;
+  const int mis = (int)(((uintptr_t)x & 15) / sizeof(T));
+  const int head = min(mis ? N - mis : 0, vocab);
+  const int nvec = (vocab - head) / N;
+  const uint4* body = reinterpret_cast<const uint4*>(x + head);
+  const int edges = part == 0 ? vocab - nvec * N : 0;  // < 2 N
+  const int v0 = (int)((int64_t)nvec * part / parts), v1 = (int)((int64_t)nvec * (part + 1) / parts);
 
   const int64_t tk = tokens[row];
   const bool has = tk >= 0 && tk < vocab;
   const int tok = has ? (int)tk : 0;
-  const float t = Vec<T>::one(p.x + tok);
+  const float t = Vec<T>::one(x + tok);
   if (threadIdx.x == 0) {
     sh.count = sh.noted = 0;
     if (!has && tk != -1 && part == 0) atomicOr(&g_err_logprobs, (unsigned)kErrTokenId);
@@ -428,27 +504,28 @@ __global__ void __launch_bounds__(kThreads, 4)
 
   // block b of 256 vectors: a step takes one from each quarter of the part, so
   // the first step samples all of it
-  const int quarter = ((p.v1 - p.v0 + kThreads - 1) / kThreads + 3) / 4;
+  const int quarter = ((v1 - v0 + kThreads - 1) / kThreads + 3) / 4;
   Sums s;
   unsigned ahead = 0;
-  float thr = INFINITY;
+  float thr = INFINITY, bound = -INFINITY;  // bound: least entry that needs a second look (lim, t or thr)
+  const float t_bound = !has ? INFINITY : t != t ? -INFINITY : t;
   for (int step = 0; step < quarter; ++step) {
     uint4 raw[4];
-    bool in[4];
+    const int vs = v0 + step * kThreads + threadIdx.x;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int v = p.v0 + (u * quarter + step) * kThreads + threadIdx.x;
-      in[u] = v < p.v1;
-      raw[u] = in[u] ? __ldcs(p.body + v) : make_uint4(0, 0, 0, 0);
+      const int v = vs + u * quarter * kThreads;
+      raw[u] = v < v1 ? __ldcs(body + v)
+                      : make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
     }
     float vm[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) vm[u] = in[u] ? Vec<T>::max(raw[u]) : -INFINITY;
+    for (int u = 0; u < 4; ++u) vm[u] = Vec<T>::max(raw[u]);
     if (step == 0 && top > 0) {
       uint64_t best = 0;
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (in[u]) {
+        if (vs + u * quarter * kThreads < v1) {
           const uint64_t key = key_of(vm[u], 0);
           best = key > best ? key : best;
         }
@@ -460,66 +537,45 @@ __global__ void __launch_bounds__(kThreads, 4)
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if (!in[u]) continue;
-      const int v = p.v0 + (u * quarter + step) * kThreads + threadIdx.x, i = p.head + v * N;
-      float f[N];
-      Vec<T>::unpack(raw[u], f);
-      if (!(vm[u] <= s.lim)) s.move(vm[u]);
-      s.m = fmaxf(s.m, vm[u]);
-      s.template add<N>(f);
-      if (has && !(vm[u] < t)) {
-        // a vector before the token counts its ties, one after it does not
-        if (t == t && i + N <= tok)
-          ahead += Vec<T>::template above<true>(raw[u], t);
-        else if (t == t && i > tok)
-          ahead += Vec<T>::template above<false>(raw[u], t);
-        else
-          ahead += ahead_one_by_one(p, v, t, tok);
+      if (!(vm[u] < bound)) {
+        if (!(vm[u] <= s.lim)) s.move(vm[u]);
+        bound = fminf(fminf(s.lim, t_bound), thr);
+        const int v = vs + u * quarter * kThreads, i = head + v * N;
+        if (v < v1) {
+          if (has && !(vm[u] < t)) {
+            // a vector before the token counts its ties, one after it does not
+            if (t == t && i + N <= tok)
+              ahead += Vec<T>::template above<true>(raw[u], t);
+            else if (t == t && i > tok)
+              ahead += Vec<T>::template above<false>(raw[u], t);
+            else
+              ahead += ahead_one_by_one<T>(x + i, i, t, tok);
+          }
+          if (!(vm[u] < thr)) note(sh, v);
+        }
       }
-      if (!(vm[u] < thr)) note(sh, v);
+      float f[N];
+      unpack_finite<T>(raw[u], f);
+      s.template add<N>(f);
     }
   }
   if (quarter == 0) thr = -INFINITY;  // no vectors: every edge entry is a candidate
-  if (threadIdx.x < p.edges) {
+  const Part<T> p = {x, body, head, v0, v1, vocab, edges};
+  if (threadIdx.x < edges) {
     const int i = p.edge_index(threadIdx.x);
-    const float f[2] = {Vec<T>::one(p.x + i), -INFINITY};
-    if (!(f[0] <= s.lim)) s.move(f[0]);
-    s.m = fmaxf(s.m, f[0]);
-    s.add<2>(f);
-    if (has) ahead += is_ahead(f[0], i, t, tok);
+    const float v = Vec<T>::one(x + i);
+    if (!(v <= s.lim)) s.move(v);
+    const float f[2] = {fmaxf(v, Vec<T>::kLowest), Vec<T>::kLowest};
+    if (s.lim != -INFINITY) s.add<2>(f);
+    if (has) ahead += is_ahead(v, i, t, tok);
   }
 
   // ------------------------------------------------------ join the sums
-  Stats st;
-  {
-    float s0, s1, t0, t1;
-    un2(s.S, s0, s1);
-    un2(s.T, t0, t1);
-    // from the thread's reference to its maximum
-    const float d = s.lim == -INFINITY ? 0.f : fminf(s.r - s.m, 0.f), f = ex2(d * kLog2e);
-    st.m = s.bad ? INFINITY : s.m;
-    st.s = (s0 + s1) * f;
-    st.t = (t0 + t1 + d * (s0 + s1)) * f;
-    st.rank = ahead;
-    st.bad = s.bad;
-    if (s.lim == -INFINITY) st.m = -INFINITY, st.s = st.t = 0.f;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats w;
-    w.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    w.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    w.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-    w.rank = __shfl_xor_sync(0xffffffffu, st.rank, o);
-    w.bad = __shfl_xor_sync(0xffffffffu, st.bad, o);
-    st = join(st, w);
-  }
-  if (lane == 0) sh.warp[warp] = st;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < kWarps; ++w) st = join(st, sh.warp[w]);
-    sh.cta = st;
-  }
+  Stats st = stats_of(s, ahead);
+  st = block_join(sh, st);
+  if (!st.bad && (st.m <= Vec<T>::kLowest || st.m > 1e30f) && st.m != -INFINITY)
+    st = sum_one_by_one(sh, p, ahead);
+  if (threadIdx.x == 0) sh.cta = st;
 
   // ------------------------------------------------- the part's top entries
   if (top > 0) {
