@@ -36,7 +36,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kCap = 2048;      // entries of the candidate list
 constexpr float kSlack = 10.f;  // how far an entry may pass a thread's reference
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 // ------------------------------------------------------------ element types
 template <typename T>
@@ -45,9 +45,9 @@ template <>
 struct Vec<float> {
   static constexpr int kN = 4;
   static constexpr uint32_t kNegInf = 0xff800000u;
-  static constexpr float kLowest = -3.402823466e38f;
+  static constexpr float kFloor = -1e38f;
   static __device__ __forceinline__ uint32_t floor_word(uint32_t w) {
-    return __float_as_uint(fmaxf(__uint_as_float(w), kLowest));
+    return __float_as_uint(fmaxf(__uint_as_float(w), kFloor));
   }
   static __device__ __forceinline__ float max(const uint4& r) {
     float a, b;
@@ -80,10 +80,10 @@ template <>
 struct Vec<bf16> {
   static constexpr int kN = 8;
   static constexpr uint32_t kNegInf = 0xff80ff80u;
-  static constexpr float kLowest = -3.38953139e38f;
+  static constexpr float kFloor = -9.96920997e37f;
   static __device__ __forceinline__ uint32_t floor_word(uint32_t w) {
     uint32_t r;
-    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xff7fff7fu));
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xfe96fe96u));
     return r;
   }
   static __device__ __forceinline__ float max(const uint4& r) {
@@ -116,7 +116,7 @@ template <>
 struct Vec<__half> {
   static constexpr int kN = 8;
   static constexpr uint32_t kNegInf = 0xfc00fc00u;
-  static constexpr float kLowest = -65504.f;
+  static constexpr float kFloor = -65504.f;
   static __device__ __forceinline__ uint32_t floor_word(uint32_t w) {
     uint32_t r;
     asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xfbfffbffu));
@@ -247,10 +247,13 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   return r;
 }
 
-// One thread's sums against its reference r. S and T hold two partial sums each.
+// One thread's sums against its reference r, in powers of two: with L =
+// log2(e) and c = -r L, S = sum 2^y and T = sum 2^y y over y = x L + c, one FMA
+// per entry. c is rounded; its residue is put right in the end. S and T hold two
+// partial sums each.
 struct Sums {
   float r = 0.f, lim = -INFINITY;  // entries above lim move r; lim = -inf: nothing finite seen yet
-  uint64_t S = 0, T = 0;
+  uint64_t c = 0, S = 0, T = 0;
   bool bad = false;
 
   // called before a group whose largest entry is vm > lim, or NaN
@@ -259,36 +262,39 @@ struct Sums {
       bad = true;
       return;
     }
+    const float nc = -vm * kLog2e;
     if (lim != -INFINITY) {
-      const float d = fmaxf(r - vm, -200.f), f = ex2(d * kLog2e);
+      float old, unused;
+      un2(c, old, unused);
+      const float d = fmaxf(nc - old, -300.f), f = ex2(d);
       const uint64_t ff = pk2(f, f);
       T = mul2(fma2(S, pk2(d, d), T), ff);
       S = mul2(S, ff);
     }
     r = vm;
+    c = pk2(nc, nc);
     lim = vm + kSlack;
   }
-  // finite entries (p = 0 for the far ones)
+  // entries of at least the type's floor (p = 0 for the far ones)
   template <int N>
-  __device__ __forceinline__ void add(const float* v) {
-    const uint64_t nr = pk2(-r, -r);
+  __device__ __forceinline__ void add(const float* v, uint64_t L2) {
 #pragma unroll
     for (int i = 0; i < N; i += 2) {
-      const uint64_t z = add2(pk2(v[i], v[i + 1]), nr);
+      const uint64_t y = fma2(pk2(v[i], v[i + 1]), L2, c);
       float y0, y1;
-      un2(mul2(z, pk2(kLog2e, kLog2e)), y0, y1);
+      un2(y, y0, y1);
       const uint64_t p = pk2(ex2(y0), ex2(y1));
       S = add2(S, p);
-      T = fma2(p, z, T);
+      T = fma2(p, y, T);
     }
   }
 };
 
-// A vector's entries, -inf as the type's lowest value: its weight is 0 beside
-// any larger entry, and 0 * z stays 0. (Parts where nothing is larger, or where
-// z could overflow, are summed again entry by entry.)
+// A vector's entries, those below the type's floor raised to it: the weight is
+// 0 beside any ordinary entry, and 0 * y stays 0. (Parts where nothing is above
+// the floor, or where y could overflow, are summed again entry by entry.)
 template <typename T>
-__device__ __forceinline__ void unpack_finite(const uint4& raw, float* f) {
+__device__ __forceinline__ void unpack_floored(const uint4& raw, float* f) {
   Vec<T>::unpack(make_uint4(Vec<T>::floor_word(raw.x), Vec<T>::floor_word(raw.y), Vec<T>::floor_word(raw.z),
                             Vec<T>::floor_word(raw.w)),
                  f);
@@ -424,11 +430,15 @@ __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
 }
 
 __device__ __forceinline__ Stats stats_of(const Sums& s, unsigned ahead) {
-  float s0, s1, t0, t1;
+  float s0, s1, t0, t1, c, unused;
   un2(s.S, s0, s1);
   un2(s.T, t0, t1);
+  un2(s.c, c, unused);
   const bool none = s.lim == -INFINITY;
-  return Stats{none ? -INFINITY : s.r, none ? 0.f : s0 + s1, none ? 0.f : t0 + t1, ahead, (unsigned)s.bad};
+  // 2^y stands for 2^(y + rest): c is -r L without its residue
+  const float rest = none ? 0.f : fmaf(-s.r, kLog2e, -c), f = ex2(rest), S = (s0 + s1) * f;
+  return Stats{none ? -INFINITY : s.r, none ? 0.f : S, none ? 0.f : ((t0 + t1) * f + rest * S) * kLn2, ahead,
+               (unsigned)s.bad};
 }
 
 // The block's statistics, in every thread; a fixed order of joins.
@@ -452,8 +462,8 @@ __device__ __forceinline__ Stats block_join(Shared& sh, Stats st) {
 }
 
 // The part's sums again, entry by entry, for parts of which the largest entry
-// is the type's lowest value (-inf must not count beside it) or so large that
-// differences overflow.
+// is at the type's floor (-inf must not count beside it) or so large that the
+// powers' arguments overflow.
 template <typename T>
 __device__ __noinline__ Stats sum_one_by_one(Shared& sh, const Part<T>& p, unsigned ahead) {
   float m = -INFINITY, S = 0.f, E = 0.f;
@@ -502,78 +512,90 @@ __global__ void __launch_bounds__(kThreads, 4)
     if (!has && tk != -1 && part == 0) atomicOr(&g_err_logprobs, (unsigned)kErrTokenId);
   }
 
-  // block b of 256 vectors: a step takes one from each quarter of the part, so
-  // the first step samples all of it
-  const int quarter = ((v1 - v0 + kThreads - 1) / kThreads + 3) / 4;
+  // A step takes four blocks of 256 vectors, one from each quarter of the part's
+  // whole steps, so the first step samples all of it; the last step takes what is left.
+  const int quarter = (v1 - v0) / (4 * kThreads);
+  const uint64_t L2 = pk2(kLog2e, kLog2e);
   Sums s;
   unsigned ahead = 0;
   float thr = INFINITY, bound = -INFINITY;  // bound: least entry that needs a second look (lim, t or thr)
   const float t_bound = !has ? INFINITY : t != t ? -INFINITY : t;
-  for (int step = 0; step < quarter; ++step) {
-    uint4 raw[4];
-    const int vs = v0 + step * kThreads + threadIdx.x;
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int v = vs + u * quarter * kThreads;
-      raw[u] = v < v1 ? __ldcs(body + v)
-                      : make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
-    }
-    float vm[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) vm[u] = Vec<T>::max(raw[u]);
-    if (step == 0 && top > 0) {
-      uint64_t best = 0;
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (vs + u * quarter * kThreads < v1) {
-          const uint64_t key = key_of(vm[u], 0);
-          best = key > best ? key : best;
-        }
-      block_merge(sh, sort32(best), kWarps);
+  const auto sample = [&](float m) {  // m: the thread's largest of the first step
+    if (top > 0) {
+      block_merge(sh, sort32(m == -INFINITY ? 0ull : key_of(m, 0)), kWarps);
       const uint64_t kth = sh.top[top - 1];
       thr = kth == 0 ? -INFINITY : value_of((uint32_t)(kth >> 32));
       if (thr != thr) thr = INFINITY;  // enough NaN entries: only they (and +inf) can be among the first
       __syncthreads();
     }
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      if (!(vm[u] < bound)) {
-        if (!(vm[u] <= s.lim)) s.move(vm[u]);
-        bound = fminf(fminf(s.lim, t_bound), thr);
-        const int v = vs + u * quarter * kThreads, i = head + v * N;
-        if (v < v1) {
-          if (has && !(vm[u] < t)) {
-            // a vector before the token counts its ties, one after it does not
-            if (t == t && i + N <= tok)
-              ahead += Vec<T>::template above<true>(raw[u], t);
-            else if (t == t && i > tok)
-              ahead += Vec<T>::template above<false>(raw[u], t);
-            else
-              ahead += ahead_one_by_one<T>(x + i, i, t, tok);
-          }
-          if (!(vm[u] < thr)) note(sh, v);
+  };
+  const auto take = [&](const uint4& raw, float vm, int v) {
+    if (!(vm < bound)) {
+      if (!(vm <= s.lim)) s.move(vm);
+      bound = fminf(fminf(s.lim, t_bound), thr);
+      const int i = head + v * N;
+      if (v < v1) {
+        if (has && !(vm < t)) {
+          // a vector before the token counts its ties, one after it does not
+          if (t == t && i + N <= tok)
+            ahead += Vec<T>::template above<true>(raw, t);
+          else if (t == t && i > tok)
+            ahead += Vec<T>::template above<false>(raw, t);
+          else
+            ahead += ahead_one_by_one<T>(x + i, i, t, tok);
         }
+        if (!(vm < thr)) note(sh, v);
       }
-      float f[N];
-      unpack_finite<T>(raw[u], f);
-      s.template add<N>(f);
     }
+    float f[N];
+    unpack_floored<T>(raw, f);
+    s.template add<N>(f, L2);
+  };
+  const auto max_nan = [](float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+    return m;
+  };
+  for (int step = 0; step < quarter; ++step) {
+    uint4 raw[4];
+    float vm[4];
+    const int vs = v0 + step * kThreads + threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) raw[u] = __ldcs(body + vs + u * quarter * kThreads);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) vm[u] = Vec<T>::max(raw[u]);
+    if (step == 0) sample(max_nan(max_nan(vm[0], vm[1]), max_nan(vm[2], vm[3])));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) take(raw[u], vm[u], vs + u * quarter * kThreads);
   }
-  if (quarter == 0) thr = -INFINITY;  // no vectors: every edge entry is a candidate
+  {
+    uint4 raw[4];
+    float vm[4];
+    const int vs = v0 + quarter * 4 * kThreads + threadIdx.x;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      raw[u] = vs + u * kThreads < v1 ? __ldcs(body + vs + u * kThreads)
+                                      : make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) vm[u] = Vec<T>::max(raw[u]);
+    if (quarter == 0) sample(max_nan(max_nan(vm[0], vm[1]), max_nan(vm[2], vm[3])));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) take(raw[u], vm[u], vs + u * kThreads);
+  }
   const Part<T> p = {x, body, head, v0, v1, vocab, edges};
   if (threadIdx.x < edges) {
     const int i = p.edge_index(threadIdx.x);
     const float v = Vec<T>::one(x + i);
     if (!(v <= s.lim)) s.move(v);
-    const float f[2] = {fmaxf(v, Vec<T>::kLowest), Vec<T>::kLowest};
-    if (s.lim != -INFINITY) s.add<2>(f);
+    const float f[2] = {fmaxf(v, Vec<T>::kFloor), Vec<T>::kFloor};
+    if (s.lim != -INFINITY) s.add<2>(f, L2);
     if (has) ahead += is_ahead(v, i, t, tok);
   }
 
   // ------------------------------------------------------ join the sums
   Stats st = stats_of(s, ahead);
   st = block_join(sh, st);
-  if (!st.bad && (st.m <= Vec<T>::kLowest || st.m > 1e30f) && st.m != -INFINITY)
+  if (!st.bad && (st.m <= Vec<T>::kFloor || st.m > 1e30f) && st.m != -INFINITY)
     st = sum_one_by_one(sh, p, ahead);
   if (threadIdx.x == 0) sh.cta = st;
 
