@@ -14,10 +14,10 @@
 // reference r near its maximum (moved only when an entry passes r + 10, so the
 // usual vector costs no rescale) and sums S and T against it in 32 bits, with
 // packed 2 x fp32 arithmetic. The alternatives come from the same pass: the
-// k-th largest of the threads' first maxima is a lower bound of the k-th
-// largest entry, so only vectors that reach it are noted in a short list in
-// shared memory (a few hundred of 19 thousand) and looked at again at the end,
-// when warps sort and merge their entries in 32-entry runs. The rank is counted
+// k-th largest of the warps' four largest first maxima is a lower bound of the
+// k-th largest entry, so each thread marks those of its vectors that reach it
+// (a few hundred of 19 thousand), one bit each, and only they are looked at again
+// at the end, when warps sort and merge their entries in 32-entry runs. The rank is counted
 // only in vectors whose maximum reaches the token's logit.
 #include <cuda_fp16.h>
 
@@ -205,6 +205,7 @@ struct Shared {
   Stats warp[kWarps];
   Stats cta;
   unsigned count, noted;
+  uint32_t four[32];
 };
 
 // The 32 largest keys of the block, each warp holding one descending run;
@@ -252,16 +253,17 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // per entry. c is rounded; its residue is put right in the end. S and T hold two
 // partial sums each.
 struct Sums {
-  float r = 0.f, lim = -INFINITY;  // entries above lim move r; lim = -inf: nothing finite seen yet
+  float r = 0.f, lim = -INFINITY;  // entries above lim move r; lim = -inf: nothing above the floor seen yet
   uint64_t c = 0, S = 0, T = 0;
   bool bad = false;
 
   // called before a group whose largest entry is vm > lim, or NaN
-  __device__ __forceinline__ void move(float vm) {
+  __device__ __forceinline__ void move(float vm, float floor) {
     if (!(vm < INFINITY)) {  // NaN or +inf
       bad = true;
       return;
     }
+    if (vm <= floor) return;  // weighs nothing beside an ordinary entry (and its c could overflow)
     const float nc = -vm * kLog2e;
     if (lim != -INFINITY) {
       float old, unused;
@@ -337,6 +339,44 @@ __device__ __noinline__ unsigned ahead_one_by_one(const T* x, int i, float t, in
 __device__ __forceinline__ void note(Shared& sh, int v) {
   const unsigned at = atomicAdd(&sh.noted, 1u);
   if (at < kCap) sh.vecs[at] = v;
+}
+
+// The set bits of a thread's marks: bit b of mark u is the vector first + u * apart + b * kThreads.
+__device__ __forceinline__ void note_marks(Shared& sh, uint32_t (&marks)[4], int first, int apart) {
+  const unsigned n = __popc(marks[0]) + __popc(marks[1]) + __popc(marks[2]) + __popc(marks[3]);
+  if (n == 0) return;
+  unsigned at = atomicAdd(&sh.noted, n);
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    for (; marks[u] && at < kCap; ++at) {
+      const int b = __ffs(marks[u]) - 1;
+      marks[u] &= marks[u] - 1;
+      sh.vecs[at] = first + u * apart + b * kThreads;
+    }
+    marks[u] = 0;
+  }
+}
+
+// A lower bound of the k-th largest of the block's values (k <= 32) that at
+// least k of them reach: the k-th largest of each warp's four largest. Only
+// distinct values of a warp count, so ties lower it; NaN counts as +inf.
+__device__ __forceinline__ float block_bound(Shared& sh, float m, int k) {
+  static_assert(kWarps * 4 == 32, "one value a lane");
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t o = order_of(m != m ? INFINITY : m);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t best = __reduce_max_sync(0xffffffffu, o);
+    if (lane == 0) sh.four[warp * 4 + j] = best;
+    if (o == best) o = 0;  // below every value
+  }
+  __syncthreads();
+  const uint32_t mine = sh.four[lane];
+  int reach = 0;
+#pragma unroll
+  for (int j = 0; j < 32; ++j) reach += sh.four[j] >= mine;
+  const uint32_t kth = __reduce_max_sync(0xffffffffu, reach >= k ? mine : 0u);
+  return kth <= order_of(-INFINITY) ? -INFINITY : value_of(kth);
 }
 
 // Every vector with an entry at or above thr is noted.
@@ -416,6 +456,36 @@ __device__ __forceinline__ void sort_list(Shared& sh, unsigned n) {
   block_merge(sh, best, kWarps);
 }
 
+// The least value above x (x not NaN or +inf).
+__device__ __forceinline__ float next_up(float x) { return value_of(order_of(x) + 1); }
+
+// Adds entries equal to tie, in index order, to a list of fewer than top
+// entries above it until it holds top; the part has enough of them.
+template <typename T>
+__device__ __noinline__ void fill_ties(Shared& sh, const Part<T>& p, float tie, unsigned top) {
+  constexpr int N = Vec<T>::kN, kChunk = 1024 / N;  // the list has room for a chunk of ties
+  if (threadIdx.x < p.edges) {
+    const int i = p.edge_index(threadIdx.x);
+    const float f = Vec<T>::one(p.x + i);
+    if (f == tie) push(sh, f, i);
+  }
+  for (int v0 = p.v0; v0 < p.v1; v0 += kChunk) {
+    __syncthreads();
+    if (sh.count >= top + p.edges) break;  // the edges may come after the body
+    __syncthreads();
+    const int v = v0 + threadIdx.x;
+    if (threadIdx.x < kChunk && v < p.v1) {
+      float f[N];
+      Vec<T>::unpack(p.body[v], f);
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (f[j] == tie) push(sh, f[j], p.head + v * N + j);
+    }
+  }
+  __syncthreads();
+  sort_list(sh, min(sh.count, (unsigned)kCap));
+}
+
 __device__ __forceinline__ Stats join(const Stats& a, const Stats& b) {
   Stats o;
   o.m = fmaxf(a.m, b.m);
@@ -461,8 +531,8 @@ __device__ __forceinline__ Stats block_join(Shared& sh, Stats st) {
   return st;
 }
 
-// The part's sums again, entry by entry, for parts of which the largest entry
-// is at the type's floor (-inf must not count beside it) or so large that the
+// The part's sums again, entry by entry, for parts that hold nothing above the
+// type's floor (-inf must not count beside it) or entries so large that the
 // powers' arguments overflow.
 template <typename T>
 __device__ __noinline__ Stats sum_one_by_one(Shared& sh, const Part<T>& p, unsigned ahead) {
@@ -518,21 +588,13 @@ __global__ void __launch_bounds__(kThreads, 4)
   const uint64_t L2 = pk2(kLog2e, kLog2e);
   Sums s;
   unsigned ahead = 0;
-  float thr = INFINITY, bound = -INFINITY;  // bound: least entry that needs a second look (lim, t or thr)
+  float thr = INFINITY, bound = -INFINITY;  // bound: least entry that needs a second look
   const float t_bound = !has ? INFINITY : t != t ? -INFINITY : t;
-  const auto sample = [&](float m) {  // m: the thread's largest of the first step
-    if (top > 0) {
-      block_merge(sh, sort32(m == -INFINITY ? 0ull : key_of(m, 0)), kWarps);
-      const uint64_t kth = sh.top[top - 1];
-      thr = kth == 0 ? -INFINITY : value_of((uint32_t)(kth >> 32));
-      if (thr != thr) thr = INFINITY;  // enough NaN entries: only they (and +inf) can be among the first
-      __syncthreads();
-    }
-  };
+  uint32_t marks[4] = {0u, 0u, 0u, 0u};  // vectors of this thread that reach thr
   const auto take = [&](const uint4& raw, float vm, int v) {
     if (!(vm < bound)) {
-      if (!(vm <= s.lim)) s.move(vm);
-      bound = fminf(fminf(s.lim, t_bound), thr);
+      if (!(vm <= s.lim)) s.move(vm, Vec<T>::kFloor);
+      bound = fminf(s.lim, t_bound);
       const int i = head + v * N;
       if (v < v1) {
         if (has && !(vm < t)) {
@@ -544,7 +606,6 @@ __global__ void __launch_bounds__(kThreads, 4)
           else
             ahead += ahead_one_by_one<T>(x + i, i, t, tok);
         }
-        if (!(vm < thr)) note(sh, v);
       }
     }
     float f[N];
@@ -564,10 +625,18 @@ __global__ void __launch_bounds__(kThreads, 4)
     for (int u = 0; u < 4; ++u) raw[u] = __ldcs(body + vs + u * quarter * kThreads);
 #pragma unroll
     for (int u = 0; u < 4; ++u) vm[u] = Vec<T>::max(raw[u]);
-    if (step == 0) sample(max_nan(max_nan(vm[0], vm[1]), max_nan(vm[2], vm[3])));
+    if (top > 0) {
+      if (step == 0) thr = block_bound(sh, max_nan(max_nan(vm[0], vm[1]), max_nan(vm[2], vm[3])), top);
+      const int b = step % 32;
+      if (b == 0 && step > 0) note_marks(sh, marks, vs - 32 * kThreads, quarter * kThreads);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) marks[u] |= vm[u] < thr ? 0u : 1u << b;
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) take(raw[u], vm[u], vs + u * quarter * kThreads);
   }
+  if (top > 0 && quarter > 0)
+    note_marks(sh, marks, v0 + (quarter - 1) / 32 * 32 * kThreads + threadIdx.x, quarter * kThreads);
   {
     uint4 raw[4];
     float vm[4];
@@ -578,7 +647,12 @@ __global__ void __launch_bounds__(kThreads, 4)
                                       : make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
 #pragma unroll
     for (int u = 0; u < 4; ++u) vm[u] = Vec<T>::max(raw[u]);
-    if (quarter == 0) sample(max_nan(max_nan(vm[0], vm[1]), max_nan(vm[2], vm[3])));
+    if (top > 0) {
+      if (quarter == 0) thr = block_bound(sh, max_nan(max_nan(vm[0], vm[1]), max_nan(vm[2], vm[3])), top);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (!(vm[u] < thr) && vs + u * kThreads < v1) note(sh, vs + u * kThreads);
+    }
 #pragma unroll
     for (int u = 0; u < 4; ++u) take(raw[u], vm[u], vs + u * kThreads);
   }
@@ -586,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   if (threadIdx.x < edges) {
     const int i = p.edge_index(threadIdx.x);
     const float v = Vec<T>::one(x + i);
-    if (!(v <= s.lim)) s.move(v);
+    if (!(v <= s.lim)) s.move(v, Vec<T>::kFloor);
     const float f[2] = {fmaxf(v, Vec<T>::kFloor), Vec<T>::kFloor};
     if (s.lim != -INFINITY) s.add<2>(f, L2);
     if (has) ahead += is_ahead(v, i, t, tok);
@@ -595,28 +669,34 @@ __global__ void __launch_bounds__(kThreads, 4)
   // ------------------------------------------------------ join the sums
   Stats st = stats_of(s, ahead);
   st = block_join(sh, st);
-  if (!st.bad && (st.m <= Vec<T>::kFloor || st.m > 1e30f) && st.m != -INFINITY)
+  if (!st.bad && (st.m == -INFINITY || st.m > 1e30f))
     st = sum_one_by_one(sh, p, ahead);
   if (threadIdx.x == 0) sh.cta = st;
 
   // ------------------------------------------------- the part's top entries
   if (top > 0) {
+    float tie = NAN;
     for (int tries = 0;; ++tries) {
       const unsigned noted = sh.noted;
       expand(sh, p, min(noted, (unsigned)kCap), thr);
       const unsigned n = sh.count;
       sort_list(sh, min(n, (unsigned)kCap));
-      if (noted <= kCap && n <= kCap) break;
-      // more candidates than the lists hold: raise the bound to the list's own
-      // k-th largest and look again; a tie, or entries that rise along the row
-      // and so overflow again, go without the lists
+      if (noted <= kCap && n <= kCap) {
+        if (tie == tie && n < (unsigned)top) fill_ties(sh, p, tie, top);
+        break;
+      }
+      // More candidates than the lists hold: raise the bound to the list's own
+      // k-th largest and look again, or, when that is a tie, past the tie, to
+      // fill up with its first entries. Rows that rise along their length and
+      // so overflow each time go without the lists.
       const float next = value_of((uint32_t)(sh.top[top - 1] >> 32));
       __syncthreads();
-      if (!(next > thr) || tries == 2) {
+      if (tries == 3 || !(thr < INFINITY) || next != next) {
         top_by_scans(sh, p, top);
         break;
       }
-      thr = next;
+      tie = next > thr ? NAN : thr;
+      thr = next > thr ? next : next_up(thr);
       if (threadIdx.x == 0) sh.count = sh.noted = 0;
       __syncthreads();
       collect(sh, p, thr);

@@ -542,6 +542,35 @@ def test_logprobs_ties_banned_entries_and_empty_rows(dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows", [1, 9])
+def test_logprobs_long_rows_with_few_allowed_entries_or_many_ties(dtype, rows):
+    """Masked vocabularies (constrained decoding), constant and rising rows: more entries tie for a place among the
+    alternatives than any candidate list holds."""
+    vocab = 100_003
+    low = torch.finfo(dtype).min
+    fills = [-math.inf, low, -10000.0, 0.0]
+    x = torch.empty(9, vocab, dtype=dtype)
+    allowed = torch.randint(0, vocab, (5,), generator=gen(7))
+    for i, f in enumerate(fills):
+        x[i] = f
+        x[i, allowed] = torch.randn(5, generator=gen(8)).to(dtype) + 1
+    x[4] = -math.inf
+    x[4, ::2] = low
+    x[5] = (torch.arange(vocab) / 50).to(dtype)             # rising, with ties in the 16-bit types
+    x[6] = -3.0
+    x[6, ::37] = 2.0                                        # thousands tie for the first places
+    x[7] = torch.randn(vocab, generator=gen(9)).to(dtype)
+    x[7, torch.rand(vocab, generator=gen(10)) < 0.3] = -math.inf
+    x[8] = -math.inf
+    x[8, -3:] = low                                         # only the lowest value is left, at the end
+    if rows == 1:
+        for i in range(9):
+            check_logprobs(x[i:i + 1], allowed[:1], 32 if i % 2 else 3)
+    else:
+        check_logprobs(x, torch.randint(0, vocab, (9,), generator=gen(11)), 20)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 def test_logprobs_rows_with_nan_or_inf(dtype):
     from kavor_b200.layers.sampler import token_logprobs
 
