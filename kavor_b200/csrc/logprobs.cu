@@ -752,13 +752,16 @@ __global__ void __launch_bounds__(kThreads, 4)
   }
 }
 
-// CTAs per row: one when the rows alone give every SM its four, else as many
-// (of 2, 4, 8, the portable cluster sizes) as still fit one wave and leave
-// each CTA a step's worth of vectors.
+// CTAs per row (1, 2, 4 or 8, the portable cluster sizes). More parts shorten
+// the stream of a row but repeat its fixed work, so eight only while each CTA has
+// an SM, four up to two CTAs an SM, two up to four (at 151936 bf16 entries and 20
+// alternatives, us for 1/2/4/8 parts: 16 rows 22/16/12/11, 74 rows 24/18/17/23,
+// 148 rows 30/23/29/38, 256 rows 36/31/38/56, 400 rows 41/47/55/83), and only
+// while a part keeps a block of vectors.
 int parts_for(int rows, int vectors) {
-  const int slots = 4 * device_sm_count();
-  int parts = 1;
-  while (parts < 8 && (int64_t)rows * parts * 2 <= slots && vectors / (parts * 2) >= kThreads) parts *= 2;
+  const int64_t sms = device_sm_count();
+  int parts = (int64_t)rows * 8 <= sms ? 8 : (int64_t)rows * 4 <= 2 * sms ? 4 : (int64_t)rows * 2 <= 4 * sms ? 2 : 1;
+  while (parts > 1 && vectors / parts < kThreads) parts /= 2;
   return parts;
 }
 
