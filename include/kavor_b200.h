@@ -239,7 +239,7 @@ int kvb_load_kv_fp8(const void* k_cache, const void* v_cache, const void* k_scal
  * of 64; 0 < scale < 1e30. `workspace`: kvb_tree_attn_workspace_size bytes,
  * 16-byte aligned, its content irrelevant before and after; calls that may
  * overlap on the GPU need one each. */
-int kvb_tree_attn_workspace_size(int num_q_heads, int num_kv_heads, int max_seqlen_q, size_t* bytes);
+int kvb_tree_attn_workspace_size(int batch, int num_q_heads, int num_kv_heads, int max_seqlen_q, size_t* bytes);
 int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride_h, int64_t total_q, const void* k_cache,
                   const void* v_cache, const void* k_scale, const void* v_scale, int64_t num_blocks,
                   int64_t block_stride, int64_t scale_block_stride, int block_size, const int32_t* block_tables,

@@ -406,9 +406,9 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
 
 
 # ------------------------------------------------------------------ tree attention
-def tree_workspace_bytes(num_q_heads: int, num_kv_heads: int, max_seqlen_q: int) -> int:
+def tree_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, max_seqlen_q: int) -> int:
     n = ctypes.c_size_t(0)
-    _lib.call("kvb_tree_attn_workspace_size", num_q_heads, num_kv_heads, max_seqlen_q, ctypes.byref(n))
+    _lib.call("kvb_tree_attn_workspace_size", batch, num_q_heads, num_kv_heads, max_seqlen_q, ctypes.byref(n))
     return int(n.value)
 
 
@@ -457,7 +457,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         _req(out.shape == q.shape and out.stride(2) == 1, "out must have q's shape and contiguous rows")
     # scratch of this call alone (torch's allocator orders its reuse on the stream), so calls on
     # different streams and captured graphs never share it
-    need = tree_workspace_bytes(hq, hkv, max_seqlen_q)
+    need = tree_workspace_bytes(batch, hq, hkv, max_seqlen_q)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     ost = out.stride()
     _launch(index, "kvb_tree_attn", q.data_ptr(), qst[0], qst[1], total, k_cache.data_ptr(), v_cache.data_ptr(),

@@ -41,7 +41,7 @@ SIGNATURES: dict[str, list] = {
     "kvb_token_logprobs": [P, I, L, P, I, I, I, P, P, P, P, P, P],
     "kvb_store_kv_fp8": [P, L, L, P, L, L, P, P, P, P, L, L, L, I, I, I, P, I, P],
     "kvb_load_kv_fp8": [P, P, P, P, L, L, L, I, I, I, P, L, I, P, I, I, P, L, P, L, P],
-    "kvb_tree_attn_workspace_size": [I, I, I, POINTER(c_size_t)],
+    "kvb_tree_attn_workspace_size": [I, I, I, I, POINTER(c_size_t)],
     "kvb_tree_attn": [P, L, L, L, P, P, P, P, L, L, L, I, P, L, I, P, P, I, P, L, I, P, L, L, I, I, I, I, F, P,
                       c_size_t, P],
     "kvb_gemm_workspace_size": [I, I, I, I, POINTER(c_size_t)],

@@ -30,19 +30,26 @@ using tree::kHD;
 using tree::Walk;
 
 // ------------------------------------------------------------- warp-MMA kernel
-// 16 query rows (nodes x query heads of one kv head) per unit, 64-token tiles
-// staged by TMA; each of four consumer warps takes 16 tokens of a tile.
-constexpr int kRows = 16;
+// 8 NT query rows (nodes x query heads of one kv head) per unit, 64-token tiles
+// staged by TMA; each of four consumer warps takes 16 tokens of a tile. Tokens
+// (then head dims) are the MMAs' 16-row side and query rows their 8-column side,
+// S^T = K Q^T and O^T = V^T P^T, so a decode step's 4 to 8 query heads fill the
+// instructions and K and V are converted once for all rows. e4m3 bytes become
+// halves in registers (exact); two 8x8 register transposes turn the weights from
+// S^T's layout to P^T's.
 constexpr int kTile = 64;
 constexpr int kWarps = 4;
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kScratchStride = kHD + 4;  // fp32 row of the warp merge, padded against bank conflicts
 
-template <bool kFp8>
+template <bool kFp8, int NT>
 struct Cfg {
+  static constexpr int kRows = 8 * NT;
   static constexpr int kKV = kTile * kHD * (kFp8 ? 1 : 2);  // bytes of a K (or V) tile
   static constexpr int kStage = 2 * kKV;
-  static constexpr int kStages = kFp8 ? 5 : 3;
+  // CTAs an SM holds, and stages that fit its shared memory then
+  static constexpr int kCtas = kFp8 ? (NT == 1 ? 4 : 3) : 2;
+  static constexpr int kStages = kFp8 ? (NT == 1 ? 3 : 4) : 3;
   static constexpr int kSmem = kStages * kStage + kRows * kScratchStride * 4 + 1024;
 };
 
@@ -66,28 +73,39 @@ __device__ __forceinline__ void mma_f16_16816(float* d, const uint32_t* a, uint3
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// two e4m3 bytes -> two halves (exact)
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"((unsigned short)two));
-  return r;
+// four e4m3 bytes -> halves (exact)
+__device__ __forceinline__ void e4m3x4_to_half(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(four));
 }
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr));
+// Transpose of an 8x8 matrix of 16-bit values held one row per four lanes.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t addr) {
+  unsigned short v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
   return v;
 }
-
-template <bool kFp8>
-__global__ void __launch_bounds__(kThreads, 2)
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+template <bool kFp8, int NT>
+__global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
     tree_warp_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                      const __grid_constant__ Args a) {
-  using C = Cfg<kFp8>;
+  using C = Cfg<kFp8, NT>;
+  constexpr int kRows = C::kRows;
   kernel_entry();
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[C::kStages];
@@ -162,22 +180,23 @@ __global__ void __launch_bounds__(kThreads, 2)
   }
 
   // -------------------------------------------------------------- consumers
-  const int r = lane >> 2, j4 = lane & 3;  // rows r and r + 8, column group of the MMA fragments
+  // Lane (g, j4): tokens g and g + 8 of the warp's sixteen and query rows
+  // 8 t + 2 j4, + 1 of S^T; the same rows and the dims of dim_of() of O^T.
+  const int g = lane >> 2, j4 = lane & 3, mi = lane >> 3;
   const int tok0 = warp * 16;
   uint32_t it = 0;
   bool ok = true;
   while (w.next(a)) {
     const int base = w.s.len - w.s.nodes;  // position of node 0 (negative: earlier nodes are not in the cache)
-    int node[2], qrow[2];
-    float rscale[2];
-    uint32_t qa[8][4];
+    uint32_t qb[NT][8][2];
+    float rscale[NT][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int R = w.rb * kRows + r + i * 8;
-      node[i] = R / a.group;
-      const bool in = node[i] < w.s.nodes;
-      qrow[i] = w.s.q0 + (in ? node[i] : 0);
-      const bf16* qp = a.q + (int64_t)qrow[i] * a.q_st + (int64_t)(w.h * a.group + (in ? R - node[i] * a.group : 0)) * a.q_sh;
+    for (int t = 0; t < NT; ++t) {
+      // B fragments: this lane loads row 8 t + g
+      const int R = w.rb * kRows + t * 8 + g, node = R / a.group;
+      const bool in = node < w.s.nodes;
+      const bf16* qp = a.q + (int64_t)(w.s.q0 + (in ? node : 0)) * a.q_st +
+                       (int64_t)(w.h * a.group + (in ? R - node * a.group : 0)) * a.q_sh;
       if constexpr (kFp8) {
         // the row over a power of two as halves: exact to 2^-25 of its largest
         // finite value, which is brought to [1, 2)
@@ -194,27 +213,34 @@ __global__ void __launch_bounds__(kThreads, 2)
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         const int e = min(max((int)(mx >> 7) - 127, -100), 100);
         const float inv = pow2(-e);
-        rscale[i] = a.scale_log2 * pow2(e);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].x));
           const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&raw[ks].y));
-          qa[ks][i] = pack_half(x.x * inv, x.y * inv);
-          qa[ks][2 + i] = pack_half(y.x * inv, y.y * inv);
+          qb[t][ks][0] = pack_half(x.x * inv, x.y * inv);
+          qb[t][ks][1] = pack_half(y.x * inv, y.y * inv);
         }
+        const float mine = a.scale_log2 * pow2(e);
+        rscale[t][0] = __shfl_sync(0xffffffffu, mine, j4 * 8);
+        rscale[t][1] = __shfl_sync(0xffffffffu, mine, j4 * 8 + 4);
       } else {
-        rscale[i] = a.scale_log2;
+        rscale[t][0] = rscale[t][1] = a.scale_log2;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          qa[ks][i] = in ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + j4 * 2) : 0u;
-          qa[ks][2 + i] = in ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + j4 * 2 + 8) : 0u;
+          qb[t][ks][0] = in ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + j4 * 2) : 0u;
+          qb[t][ks][1] = in ? *reinterpret_cast<const uint32_t*>(qp + ks * 16 + j4 * 2 + 8) : 0u;
         }
       }
     }
-    float o[16][4];
+    float o[NT][8][4];
+    float m_run[NT][2], l_run[NT][2];
 #pragma unroll
-    for (int n = 0; n < 16; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) o[t][c][0] = o[t][c][1] = o[t][c][2] = o[t][c][3] = 0.f;
+      m_run[t][0] = m_run[t][1] = -INFINITY;
+      l_run[t][0] = l_run[t][1] = 0.f;
+    }
 
     for (int jt = 0; jt < w.n && ok; ++jt, ++it) {
       const int s = it % C::kStages;
@@ -249,106 +275,115 @@ __global__ void __launch_bounds__(kThreads, 2)
         odd_v = __any_sync(0xffffffffu, odd_v);
       }
 
-      float sc[2][4];
+      // S^T: element 2 h + i is token g + 8 h, row 8 t + 2 j4 + i
+      float sc[NT][4];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.f;
-      const int mi = lane >> 3;
+      for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
       if constexpr (kFp8) {
         // k-step ks covers 16 dims; lane j4 holds dims 4 j4 .. 4 j4 + 3 of it,
-        // for Q and K alike (any order of the dims gives the same sum)
+        // for K and Q alike (any order of the dims gives the same sum)
 #pragma unroll
         for (int kp = 0; kp < 4; ++kp) {
           uint32_t b[4];
           ldmatrix_x4(swz_fp8(kb, tok0 + (lane & 7) + ((mi & 1) << 3), kp * 2 + (mi >> 1)), b[0], b[1], b[2], b[3]);
 #pragma unroll
-          for (int q = 0; q < 4; ++q)
-            mma_f16_16816(sc[q & 1], qa[kp * 2 + (q >> 1)], e4m3x2_to_half2(b[q]), e4m3x2_to_half2(b[q] >> 16));
+          for (int q = 0; q < 2; ++q) {
+            uint32_t ka[4];
+            e4m3x4_to_half(b[2 * q], ka[0], ka[2]);
+            e4m3x4_to_half(b[2 * q + 1], ka[1], ka[3]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma_f16_16816(sc[t], ka, qb[t][kp * 2 + q][0], qb[t][kp * 2 + q][1]);
+          }
         }
       } else {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          uint32_t b0, b1, b2, b3;
-          ldmatrix_x4(swz_bf16(kb, tok0 + (lane & 7) + ((mi >> 1) << 3), ks * 2 + (mi & 1)), b0, b1, b2, b3);
-          mma_bf16_16816(sc[0], qa[ks], b0, b1);
-          mma_bf16_16816(sc[1], qa[ks], b2, b3);
+          uint32_t ka[4];
+          ldmatrix_x4(swz_bf16(kb, tok0 + (lane & 7) + ((mi & 1) << 3), ks * 2 + (mi >> 1)), ka[0], ka[1], ka[2], ka[3]);
+#pragma unroll
+          for (int t = 0; t < NT; ++t) mma_bf16_16816(sc[t], ka, qb[t][ks][0], qb[t][ks][1]);
         }
       }
 
-      float ev[2][2], inv_v[2][2];  // V exponents of this lane's four tokens
+      float inv_v[2];  // 2^-exponent of the V rows of this lane's tokens
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (kFp8) {
+          const uint32_t kc = scales[s][0][tok0 + g + 8 * h], vc = scales[s][1][tok0 + g + 8 * h];
+          const float ksc = __uint_as_float(kc << 23);
+          const float ev = __uint_as_float(0x4b000000u | vc) - (8388608.f + 127.f);  // vc - 127
+          inv_v[h] = __uint_as_float((254u - vc) << 23);
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int t = tok0 + j * 8 + j4 * 2 + e;
-          if constexpr (kFp8) {
-            const int kc = scales[s][0][t], vc = scales[s][1][t];
-            const float ksc = __uint_as_float((uint32_t)kc << 23);
-            ev[j][e] = (float)(vc - 127);
-            inv_v[j][e] = __uint_as_float((uint32_t)(254 - vc) << 23);
-            sc[j][e] = fmaf(sc[j][e], rscale[0] * ksc, ev[j][e]);
-            sc[j][2 + e] = fmaf(sc[j][2 + e], rscale[1] * ksc, ev[j][e]);
-          } else {
-            inv_v[j][e] = 1.f;
-            sc[j][e] *= rscale[0];
-            sc[j][2 + e] *= rscale[1];
-          }
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) sc[t][2 * h + i] = fmaf(sc[t][2 * h + i], rscale[t][i] * ksc, ev);
+        } else {
+#pragma unroll
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) sc[t][2 * h + i] *= rscale[t][i];
         }
-      uint32_t hidden = 0;  // bit j * 4 + half * 2 + e: that score is masked
+      }
+      uint32_t hidden = 0;  // bit 4 t + 2 h + i: that score is masked
       if (p0 + 16 > base) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int h = 0; h < 2; ++h) {
+          const int pos = p0 + g + 8 * h;
+          if (kFp8 && !(inv_v[h] >= 0.f && inv_v[h] < INFINITY)) inv_v[h] = 0.f;  // stale scale bytes
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int pos = p0 + j * 8 + j4 * 2 + e;
+          for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-              const bool seen = pos < base || (pos < w.s.len && tree::sees(a, qrow[i], node[i], pos - base));
+              const int node = (w.rb * kRows + t * 8 + 2 * j4 + i) / a.group;
+              const bool seen = pos < base || (pos < w.s.len && node < w.s.nodes &&
+                                               tree::sees(a, w.s.q0 + node, node, pos - base));
               if (!seen) {
-                sc[j][i * 2 + e] = -INFINITY;
-                hidden |= 1u << (j * 4 + i * 2 + e);
+                sc[t][2 * h + i] = -INFINITY;
+                hidden |= 1u << (4 * t + 2 * h + i);
               }
             }
-          }
+        }
       }
-      float p[2][4], corr[2];
+      float corr[NT][2];
+      bool moved = false;  // a maximum of the warp's rows rose
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float mx = fmaxf(fmaxf(sc[0][2 * i], sc[0][2 * i + 1]), fmaxf(sc[1][2 * i], sc[1][2 * i + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m_new = fmaxf(m_run[i], mx);
-        const float ref = m_new == -INFINITY ? 0.f : m_new;
-        corr[i] = exp2f(m_run[i] - ref);
-        float sum = 0.f;
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int i = 0; i < 2; ++i) {
+          float mx = fmaxf(sc[t][i], sc[t][2 + i]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float m_new = fmaxf(m_run[t][i], mx);
+          const float ref = m_new == -INFINITY ? 0.f : m_new;
+          moved |= mx > m_run[t][i];
+          corr[t][i] = ex2(m_run[t][i] - ref);
+          const float x0 = ex2(sc[t][i] - ref), x1 = ex2(sc[t][2 + i] - ref);
+          sc[t][i] = x0;
+          sc[t][2 + i] = x1;
+          l_run[t][i] = fmaf(l_run[t][i], corr[t][i], kFp8 ? fmaf(x0, inv_v[0], x1 * inv_v[1]) : x0 + x1);
+          m_run[t][i] = m_new;
+        }
+      if (__any_sync(0xffffffffu, moved)) {  // rarely after a row's first tiles; otherwise every factor is 1
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float x = exp2f(sc[j][2 * i + e] - ref);
-            p[j][2 * i + e] = x;
-            // a masked weight is 0 whatever scale byte stands beside it
-            sum += kFp8 ? (x == 0.f ? 0.f : x * inv_v[j][e]) : x;
-          }
-        l_run[i] = l_run[i] * corr[i] + sum;
-        m_run[i] = m_new;
-      }
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int n = 0; n < 16; ++n) {
-        o[n][0] *= corr[0];
-        o[n][1] *= corr[0];
-        o[n][2] *= corr[1];
-        o[n][3] *= corr[1];
+          for (int c = 0; c < 8; ++c)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[t][c][i] *= corr[t][i & 1];
       }
       if (!odd_v) {
-        // P is rounded to the type of the V operand: bf16, or half (2^-12) for e4m3
-        const uint32_t pa[4] = {kFp8 ? pack_half(p[0][0], p[0][1]) : pack_bf16(p[0][0], p[0][1]),
-                                kFp8 ? pack_half(p[0][2], p[0][3]) : pack_bf16(p[0][2], p[0][3]),
-                                kFp8 ? pack_half(p[1][0], p[1][1]) : pack_bf16(p[1][0], p[1][1]),
-                                kFp8 ? pack_half(p[1][2], p[1][3]) : pack_bf16(p[1][2], p[1][3])};
+        // the weights are rounded to the type of the V operand: bf16, or half (2^-12) for e4m3
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            pb[t][h] = transpose8(kFp8 ? pack_half(sc[t][2 * h], sc[t][2 * h + 1]) : pack_bf16(sc[t][2 * h], sc[t][2 * h + 1]));
         if constexpr (kFp8) {
           // A transposed 8x8 of 16-bit elements gives a lane two tokens of a
-          // pair of dims; a byte permutation pairs the tokens of each dim.
-          // Accumulator 2c holds the even dims of 16-dim chunk c, 2c+1 the odd.
+          // pair of dims; a byte permutation pairs the tokens of each dim. Row
+          // g of the MMA is dim 2 g of the 16-dim chunk, row g + 8 dim 2 g + 1.
 #pragma unroll
           for (int cp = 0; cp < 4; ++cp) {
             uint32_t b[4];
@@ -356,56 +391,49 @@ __global__ void __launch_bounds__(kThreads, 2)
                               b[3]);
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-              const uint32_t lo = __byte_perm(b[2 * q], 0, 0x3120), hi = __byte_perm(b[2 * q + 1], 0, 0x3120);
-              mma_f16_16816(o[4 * cp + 2 * q], pa, e4m3x2_to_half2(lo), e4m3x2_to_half2(hi));
-              mma_f16_16816(o[4 * cp + 2 * q + 1], pa, e4m3x2_to_half2(lo >> 16), e4m3x2_to_half2(hi >> 16));
+              uint32_t va[4];
+              e4m3x4_to_half(__byte_perm(b[2 * q], 0, 0x3120), va[0], va[1]);
+              e4m3x4_to_half(__byte_perm(b[2 * q + 1], 0, 0x3120), va[2], va[3]);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma_f16_16816(o[t][2 * cp + q], va, pb[t][0], pb[t][1]);
             }
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            uint32_t b0, b1, b2, b3;
-            ldmatrix_x4_trans(swz_bf16(vb, tok0 + (lane & 7) + ((mi & 1) << 3), 2 * i + (mi >> 1)), b0, b1, b2, b3);
-            mma_bf16_16816(o[2 * i], pa, b0, b1);
-            mma_bf16_16816(o[2 * i + 1], pa, b2, b3);
+          for (int c = 0; c < 8; ++c) {
+            uint32_t va[4];
+            ldmatrix_x4_trans(swz_bf16(vb, tok0 + (lane & 7) + ((mi >> 1) << 3), 2 * c + (mi & 1)), va[0], va[1], va[2],
+                              va[3]);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) mma_bf16_16816(o[t][c], va, pb[t][0], pb[t][1]);
           }
         }
       } else {
         // a drafted V row that is not finite: add only what each row sees, token
         // by token (rare, so it is written for size)
 #pragma unroll 1
-        for (int t = 0; t < 16; ++t) {
-          const int src = (lane & ~3) | ((t & 7) >> 1), jj = t >> 3, e = t & 1;
-          float pt[2];
-          bool see[2];
+        for (int tk = 0; tk < 16; ++tk) {
+          const int src = (tk & 7) * 4 + j4, h = tk >> 3;
+          const uint32_t hid = __shfl_sync(0xffffffffu, hidden, src);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const float mine = jj ? (e ? p[1][2 * i + 1] : p[1][2 * i]) : (e ? p[0][2 * i + 1] : p[0][2 * i]);
-            // every lane of the quad offers its own value for (jj, e); take the owner's
-            pt[i] = __shfl_sync(0xffffffffu, mine, src);
-            see[i] = !((__shfl_sync(0xffffffffu, hidden, src) >> (jj * 4 + i * 2 + e)) & 1u);
-          }
+          for (int t = 0; t < NT; ++t) {
+            const float p0t = __shfl_sync(0xffffffffu, h ? sc[t][2] : sc[t][0], src);
+            const float p1t = __shfl_sync(0xffffffffu, h ? sc[t][3] : sc[t][1], src);
+            const bool see0 = !((hid >> (4 * t + 2 * h)) & 1u), see1 = !((hid >> (4 * t + 2 * h + 1)) & 1u);
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            if constexpr (kFp8) {
-              const uint32_t x = lds32(swz_fp8(vb, tok0 + t, c) + j4 * 4);
-#pragma unroll
-              for (int d = 0; d < 4; ++d) {
-                const uint32_t h2 = e4m3x2_to_half2(x >> (8 * d) & 0xffu);
-                const float v = __low2float(*reinterpret_cast<const __half2*>(&h2));
-                float* acc = o[2 * c + (d & 1)];
-                if (see[0]) acc[d >> 1] += pt[0] * v;
-                if (see[1]) acc[2 + (d >> 1)] += pt[1] * v;
+            for (int c = 0; c < 8; ++c) {
+              float v0, v1;  // this lane's two dims of chunk c
+              if constexpr (kFp8) {
+                uint32_t h01, unused;
+                e4m3x4_to_half(lds16(swz_fp8(vb, tok0 + tk, c) + g * 2), h01, unused);
+                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h01));
+                v0 = v.x, v1 = v.y;
+              } else {
+                v0 = __uint_as_float(lds16(swz_bf16(vb, tok0 + tk, 2 * c) + g * 2) << 16);
+                v1 = __uint_as_float(lds16(swz_bf16(vb, tok0 + tk, 2 * c + 1) + g * 2) << 16);
               }
-            } else {
-#pragma unroll
-              for (int hf = 0; hf < 2; ++hf) {
-                const uint32_t x = lds32(swz_bf16(vb, tok0 + t, 2 * c + hf) + j4 * 4);
-                const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&x));
-                float* acc = o[2 * c + hf];
-                if (see[0]) acc[0] += pt[0] * v.x, acc[1] += pt[0] * v.y;
-                if (see[1]) acc[2] += pt[1] * v.x, acc[3] += pt[1] * v.y;
-              }
+              if (see0) o[t][c][0] += p0t * v0, o[t][c][2] += p0t * v1;
+              if (see1) o[t][c][1] += p1t * v0, o[t][c][3] += p1t * v1;
             }
           }
         }
@@ -419,64 +447,60 @@ __global__ void __launch_bounds__(kThreads, 2)
 
     // ------------------------------------------- join the four warps' tokens
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 1);
-      l_run[i] += __shfl_xor_sync(0xffffffffu, l_run[i], 2);
-      if (j4 == 0) {
-        mw[warp][r + i * 8] = m_run[i];
-        lw[warp][r + i * 8] = l_run[i];
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) l_run[t][i] += __shfl_xor_sync(0xffffffffu, l_run[t][i], d);
+        if (g == 0) {
+          mw[warp][t * 8 + 2 * j4 + i] = m_run[t][i];
+          lw[warp][t * 8 + 2 * j4 + i] = l_run[t][i];
+        }
       }
-    }
     named_bar_sync(1, kWarps * 32);
-    float f[2];
+    float f[NT][2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      float M = -INFINITY;
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int v = 0; v < kWarps; ++v) M = fmaxf(M, mw[v][r + i * 8]);
-      f[i] = m_run[i] == -INFINITY ? 0.f : exp2f(m_run[i] - M);
-    }
+      for (int i = 0; i < 2; ++i) {
+        float M = -INFINITY;
+#pragma unroll
+        for (int v = 0; v < kWarps; ++v) M = fmaxf(M, mw[v][t * 8 + 2 * j4 + i]);
+        // a warp whose tokens were all masked contributes nothing (its rows are 0)
+        f[t][i] = m_run[t][i] == -INFINITY ? 0.f : ex2(m_run[t][i] - M);
+      }
 #pragma unroll 1
     for (int turn = 0; turn < kWarps; ++turn) {
       if (warp == turn) {
 #pragma unroll
-        for (int c = 0; c < 8; ++c)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            // both types: accumulators 2c and 2c+1 hold four dims of chunk c per row
-            float v[4];
-            int d[2];
-            if constexpr (kFp8) {
-              v[0] = o[2 * c][2 * i], v[1] = o[2 * c + 1][2 * i], v[2] = o[2 * c][2 * i + 1], v[3] = o[2 * c + 1][2 * i + 1];
-              d[0] = c * 16 + j4 * 4, d[1] = d[0] + 2;
-            } else {
-              v[0] = o[2 * c][2 * i], v[1] = o[2 * c][2 * i + 1], v[2] = o[2 * c + 1][2 * i], v[3] = o[2 * c + 1][2 * i + 1];
-              d[0] = c * 16 + j4 * 2, d[1] = d[0] + 8;
-            }
+          for (int c = 0; c < 8; ++c)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              float2* at = reinterpret_cast<float2*>(scratch + (r + i * 8) * kScratchStride + d[x]);
-              // a warp whose tokens were all masked contributes nothing (its rows are 0)
-              float2 add = make_float2(v[2 * x] * f[i], v[2 * x + 1] * f[i]);
-              if (turn > 0) {
-                const float2 old = *at;
-                add.x += old.x;
-                add.y += old.y;
+            for (int i = 0; i < 2; ++i) {
+              float* at = scratch + (t * 8 + 2 * j4 + i) * kScratchStride + c * 16;
+              const float v0 = o[t][c][i] * f[t][i], v1 = o[t][c][2 + i] * f[t][i];
+              if constexpr (kFp8) {
+                float2* p2 = reinterpret_cast<float2*>(at + 2 * g);
+                const float2 old = turn > 0 ? *p2 : make_float2(0.f, 0.f);
+                *p2 = make_float2(old.x + v0, old.y + v1);
+              } else {
+                at[g] = (turn > 0 ? at[g] : 0.f) + v0;
+                at[8 + g] = (turn > 0 ? at[8 + g] : 0.f) + v1;
               }
-              *at = add;
             }
-          }
       }
       named_bar_sync(1, kWarps * 32);
     }
-    const int row = threadIdx.x >> 3, d0 = (threadIdx.x & 7) * 16;
+    constexpr int kDims = kRows;  // dims of a thread: 128 threads share kRows x 128 values
+    const int row = threadIdx.x / (kHD / kDims), d0 = threadIdx.x % (kHD / kDims) * kDims;
     const int R = w.rb * kRows + row;
     const int nd = R / a.group;
     float M = -INFINITY, L = 0.f;
 #pragma unroll
     for (int v = 0; v < kWarps; ++v) M = fmaxf(M, mw[v][row]);
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v) L += mw[v][row] == -INFINITY ? 0.f : exp2f(mw[v][row] - M) * lw[v][row];
+    for (int v = 0; v < kWarps; ++v) L += mw[v][row] == -INFINITY ? 0.f : ex2(mw[v][row] - M) * lw[v][row];
     if (!ok) M = -INFINITY, L = 0.f;
     const float* sp = scratch + row * kScratchStride + d0;
     if (nd < w.s.nodes) {
@@ -484,7 +508,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const float inv = L == 0.f ? 0.f : 1.f / L;  // nothing seen: 0
         bf16* op = a.out + (int64_t)(w.s.q0 + nd) * a.o_st + (int64_t)(w.h * a.group + R - nd * a.group) * a.o_sh + d0;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kDims / 8; ++c) {
           uint4 y;
           y.x = pack_bf16(sp[8 * c] * inv, sp[8 * c + 1] * inv);
           y.y = pack_bf16(sp[8 * c + 2] * inv, sp[8 * c + 3] * inv);
@@ -496,7 +520,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         const int64_t pr = ((int64_t)blockIdx.x * 2 + w.slot()) * kRows + row;
         float4* dst = reinterpret_cast<float4*>(a.part_o + pr * kHD + d0);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) dst[c] = make_float4(sp[4 * c], sp[4 * c + 1], sp[4 * c + 2], sp[4 * c + 3]);
+        for (int c = 0; c < kDims / 4; ++c) dst[c] = make_float4(sp[4 * c], sp[4 * c + 1], sp[4 * c + 2], sp[4 * c + 3]);
         if (d0 == 0) {
           a.part_m[pr] = M;
           a.part_l[pr] = L;
@@ -508,69 +532,104 @@ __global__ void __launch_bounds__(kThreads, 2)
 }
 
 // ------------------------------------------------------------------- merge
-// One warp per query row: joins the partials of a unit that was cut between
-// CTAs, in CTA order, and writes zeros for a sequence with an empty context.
-// Rows whose unit was whole have been written already.
+// Joins the partials of units that were cut between CTAs, in an order that does
+// not depend on timing, and writes zeros for sequences with an empty context.
+// Rows whose unit was whole have been written already. A warp takes a row of a
+// few partials; the eight warps of a block share a row of many.
 constexpr int kMergeWarps = 8;
+constexpr int kFew = 16;
 
-__global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __grid_constant__ Args a) {
-  kernel_entry();
-  __shared__ int64_t s_first;
-  const int b = blockIdx.y;
-  const int per = (a.batch + kMergeWarps * 32 - 1) / (kMergeWarps * 32);
-  const int b0 = min(threadIdx.x * per, a.batch), b1 = min(b0 + per, a.batch);
-  int64_t mine = 0;
-  for (int i = b0; i < b1; ++i) mine += tree::cost_of(a, tree::seq_of(a, i, false));
-  int64_t total;
-  int64_t at = tree::block_prefix<kMergeWarps * 32>(mine, &total);
-  if (b0 <= b && b < b1) {
-    for (int i = b0; i < b; ++i) at += tree::cost_of(a, tree::seq_of(a, i, false));
-    s_first = at;
-  }
-  __syncthreads();
-  const tree::Seq s = tree::seq_of(a, b, false);
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = (int64_t)s.nodes * a.hq;
-  for (int64_t i = (int64_t)blockIdx.x * kMergeWarps + (threadIdx.x >> 5); i < rows;
-       i += (int64_t)gridDim.x * kMergeWarps) {
-    const int nd = (int)(i / a.hq), head = (int)(i - (int64_t)nd * a.hq);
-    bf16* op = a.out + (int64_t)(s.q0 + nd) * a.o_st + (int64_t)head * a.o_sh + lane * 4;
-    if (s.tiles == 0) {
-      *reinterpret_cast<uint2*>(op) = make_uint2(0u, 0u);
-      continue;
-    }
-    const int h = head / a.group;
-    const int64_t R = (int64_t)nd * a.group + head - h * a.group;
-    const int rb = (int)(R / a.rows), row = (int)(R - (int64_t)rb * a.rows);
-    const int64_t lo = s_first + ((int64_t)h * s.blocks + rb) * s.tiles, hi = lo + s.tiles;
-    int c = (int)(lo * a.parts / total);  // the part that holds tile lo
-    while (c + 1 < a.parts && tree::part_begin(total, a.parts, c + 1) <= lo) ++c;
-    while (c > 0 && tree::part_begin(total, a.parts, c) > lo) --c;
-    if (tree::part_begin(total, a.parts, c + 1) >= hi) continue;  // whole
-    float M = -INFINITY, L = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int slot = 1;; ++c, slot = 0) {
-      const int64_t pb = tree::part_begin(total, a.parts, c), pe = tree::part_begin(total, a.parts, c + 1);
-      if (pb >= hi) break;
-      if (pe > pb) {
-        const int64_t pr = ((int64_t)c * 2 + slot) * a.rows + row;
-        const float m = a.part_m[pr], l = a.part_l[pr];
-        if (m != -INFINITY) {
-          const float4 x = *reinterpret_cast<const float4*>(a.part_o + pr * kHD + lane * 4);
-          const float m_new = fmaxf(M, m);
-          const float f0 = exp2f(M - m_new), f1 = exp2f(m - m_new);
-          L = L * f0 + l * f1;
-          acc.x = acc.x * f0 + x.x * f1;
-          acc.y = acc.y * f0 + x.y * f1;
-          acc.z = acc.z * f0 + x.z * f1;
-          acc.w = acc.w * f0 + x.w * f1;
-          M = m_new;
-        }
+struct Joined {
+  float m, l;
+  float4 o;
+};
+__device__ __forceinline__ void join(Joined& x, float m, float l, const float4& o) {
+  const float m_new = fmaxf(x.m, m);
+  // a part in which the row saw nothing (m = -inf) adds 0
+  const float f0 = x.m == -INFINITY ? 0.f : ex2(x.m - m_new), f1 = m == -INFINITY ? 0.f : ex2(m - m_new);
+  x.l = x.l * f0 + l * f1;
+  x.o.x = x.o.x * f0 + o.x * f1;
+  x.o.y = x.o.y * f0 + o.y * f1;
+  x.o.z = x.o.z * f0 + o.z * f1;
+  x.o.w = x.o.w * f0 + o.w * f1;
+  x.m = m_new;
+}
+// Parts c0 + k, k = k0, k0 + step, .. < n of a row; loads of four parts in flight.
+__device__ __forceinline__ Joined join_parts(const Args& a, int c0, int n, int k0, int step, int row, int lane) {
+  Joined x = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int k = k0; k < n; k += 4 * step) {
+    float m[4], l[4];
+    float4 o[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int kk = k + u * step;
+      m[u] = -INFINITY;
+      l[u] = 0.f;
+      o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (kk < n) {
+        // the unit's first part holds its beginning (slot 1), the others follow on (slot 0)
+        const int64_t pr = ((int64_t)(c0 + kk) * 2 + (kk == 0)) * a.rows + row;
+        m[u] = a.part_m[pr];
+        l[u] = a.part_l[pr];
+        o[u] = *reinterpret_cast<const float4*>(a.part_o + pr * kHD + lane * 4);
       }
-      if (c + 1 >= a.parts) break;
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    *reinterpret_cast<uint2*>(op) = make_uint2(pack_bf16(acc.x * inv, acc.y * inv), pack_bf16(acc.z * inv, acc.w * inv));
+#pragma unroll
+    for (int u = 0; u < 4; ++u) join(x, m[u], l[u], o[u]);
+  }
+  return x;
+}
+
+__global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __grid_constant__ Args a, int rows_per_block) {
+  kernel_entry();
+  __shared__ Joined s_join[kMergeWarps][32];
+  const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const tree::Seq s = tree::seq_of(a, b, false);
+  const int64_t rows = (int64_t)s.nodes * a.hq;
+  const int64_t first = a.first[b], range = tree::range_of(a.first[a.batch], a.parts);
+  for (int64_t i0 = (int64_t)blockIdx.x * rows_per_block; i0 < rows; i0 += (int64_t)gridDim.x * rows_per_block) {
+    // where the parts of row i are
+    int c0 = 0, n = 0, row = 0;
+    bf16* op = nullptr;
+    const auto locate = [&](int64_t i) {
+      const int nd = (int)(i / a.hq), head = (int)(i - (int64_t)nd * a.hq), h = head / a.group;
+      op = a.out + (int64_t)(s.q0 + nd) * a.o_st + (int64_t)head * a.o_sh + lane * 4;
+      if (s.tiles == 0) {
+        n = 0;
+        return;
+      }
+      const int64_t R = (int64_t)nd * a.group + head - h * a.group;
+      const int rb = (int)(R / a.rows);
+      row = (int)(R - (int64_t)rb * a.rows);
+      const int64_t lo = first + ((int64_t)h * s.blocks + rb) * s.tiles;
+      c0 = (int)(lo / range);
+      n = (int)((lo + s.tiles - 1) / range) - c0 + 1;
+    };
+    const auto write = [&](const Joined& x) {
+      const float inv = x.l == 0.f ? 0.f : 1.f / x.l;
+      *reinterpret_cast<uint2*>(op) =
+          make_uint2(pack_bf16(x.o.x * inv, x.o.y * inv), pack_bf16(x.o.z * inv, x.o.w * inv));
+    };
+    const int mine = min((int64_t)rows_per_block, rows - i0);
+    if (warp < mine) {
+      locate(i0 + warp);
+      if (n == 0)
+        *reinterpret_cast<uint2*>(op) = make_uint2(0u, 0u);
+      else if (n > 1 && n <= kFew)
+        write(join_parts(a, c0, n, 0, 1, row, lane));
+    }
+    for (int r = 0; r < mine; ++r) {
+      locate(i0 + r);
+      if (n <= kFew) continue;  // the same for the whole block
+      s_join[warp][lane] = join_parts(a, c0, n, warp, kMergeWarps, row, lane);
+      __syncthreads();
+      if (warp == 0) {
+        Joined x = s_join[0][lane];
+        for (int w = 1; w < kMergeWarps; ++w) join(x, s_join[w][lane].m, s_join[w][lane].l, s_join[w][lane].o);
+        write(x);
+      }
+      __syncthreads();
+    }
   }
 }
 
@@ -586,25 +645,30 @@ int encode_pages(CUtensorMap* map, const void* base, bool fp8, int64_t num_block
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = enc(map, fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                    const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                   CU_TENSOR_MAP_SWIZZLE_128B,
+                   // an e4m3 row of one head is 128 bytes: a wider fetch would bring the next head's
+                   fp8 ? CU_TENSOR_MAP_L2_PROMOTION_L2_128B : CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(kEncode, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
   return kOk;
 }
 
-size_t workspace_bytes(int parts, int rows) { return (size_t)parts * 2 * rows * (kHD + 2) * sizeof(float); }
+size_t workspace_bytes(int parts, int rows, int batch) {
+  return (size_t)parts * 2 * rows * (kHD + 2) * sizeof(float) + ((size_t)batch + 2) * sizeof(int64_t);
+}
 
-template <bool kFp8>
+template <bool kFp8, int NT>
 int launch_warp(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e, "kvb_tree_attn: cudaGetDevice");
   if (dev >= 64 || !((done.load() >> dev) & 1ull)) {
-    e = cudaFuncSetAttribute(tree_warp_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<kFp8>::kSmem);
+    e = cudaFuncSetAttribute(tree_warp_kernel<kFp8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (Cfg<kFp8, NT>::kSmem));
     if (e != cudaSuccess) return cuda_status(e, "kvb_tree_attn: shared memory attribute");
     if (dev < 64) done.fetch_or(1ull << dev);
   }
-  e = launch_kernel(tree_warp_kernel<kFp8>, dim3(a.parts), dim3(kThreads), Cfg<kFp8>::kSmem, st, km, vm, a);
+  e = launch_kernel(tree_warp_kernel<kFp8, NT>, dim3(a.parts), dim3(kThreads), (Cfg<kFp8, NT>::kSmem), st, km, vm, a);
   return cuda_status(e, "kvb_tree_attn launch");
 }
 
@@ -613,11 +677,12 @@ int launch_warp(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, cud
 
 using namespace kvb;
 
-extern "C" int kvb_tree_attn_workspace_size(int num_q_heads, int num_kv_heads, int max_seqlen_q, size_t* bytes) {
+extern "C" int kvb_tree_attn_workspace_size(int batch, int num_q_heads, int num_kv_heads, int max_seqlen_q,
+                                            size_t* bytes) {
   if (!bytes) return set_error(kInvalid, "kvb_tree_attn_workspace_size: bytes is NULL");
-  if (num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_seqlen_q < 0)
+  if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_seqlen_q < 0)
     return set_error(kInvalid, "kvb_tree_attn_workspace_size: bad sizes");
-  *bytes = workspace_bytes(2 * device_sm_count(), kRows);
+  *bytes = workspace_bytes(4 * device_sm_count(), 16, batch);
   return kOk;
 }
 
@@ -657,10 +722,13 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   if (!(scale > 0.f) || scale > 1e30f) return set_error(kInvalid, "kvb_tree_attn: scale must be positive and finite");
 
   Args a = {};
-  a.rows = kRows;
+  const int group = num_q_heads / num_kv_heads;
+  a.rows = (int64_t)group * max_seqlen_q <= 8 ? 8 : 16;
   a.tile = kTile;
-  a.parts = 2 * device_sm_count();
-  const size_t need = workspace_bytes(a.parts, a.rows);
+  // what the SMs hold: one wave
+  a.parts = device_sm_count() * (a.rows == 8 ? (fp8 ? Cfg<true, 1>::kCtas : Cfg<false, 1>::kCtas)
+                                             : (fp8 ? Cfg<true, 2>::kCtas : Cfg<false, 2>::kCtas));
+  const size_t need = workspace_bytes(a.parts, a.rows, batch);
   if (!workspace || workspace_bytes_given < need)
     return set_error(kWorkspace, "kvb_tree_attn: workspace of %zu bytes needed, %zu given", need,
                      workspace ? workspace_bytes_given : (size_t)0);
@@ -686,10 +754,11 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   a.batch = batch;
   a.hq = num_q_heads;
   a.hkv = num_kv_heads;
-  a.group = num_q_heads / num_kv_heads;
+  a.group = group;
   a.num_blocks = (int)num_blocks;
   a.block_size = block_size;
-  a.part_o = (float*)workspace;
+  a.first = (int64_t*)workspace;
+  a.part_o = (float*)workspace + (((size_t)batch + 1) * 2 + 3) / 4 * 4;
   a.part_m = a.part_o + (size_t)a.parts * 2 * a.rows * kHD;
   a.part_l = a.part_m + (size_t)a.parts * 2 * a.rows;
   a.scale_log2 = scale * 1.4426950408889634f;
@@ -698,10 +767,16 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   const int64_t bytes = block_stride * (fp8 ? 1 : 2);
   int rc = encode_pages(&km, k_cache, fp8, num_blocks, bytes, block_size, num_kv_heads, a.tile);
   if (!rc) rc = encode_pages(&vm, v_cache, fp8, num_blocks, bytes, block_size, num_kv_heads, a.tile);
-  if (!rc) rc = fp8 ? launch_warp<true>(km, vm, a, (cudaStream_t)stream) : launch_warp<false>(km, vm, a, (cudaStream_t)stream);
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (!rc)
+    rc = a.rows == 8 ? (fp8 ? launch_warp<true, 1>(km, vm, a, st) : launch_warp<false, 1>(km, vm, a, st))
+                     : (fp8 ? launch_warp<true, 2>(km, vm, a, st) : launch_warp<false, 2>(km, vm, a, st));
   if (rc) return rc;
-  const int64_t mrows = ((int64_t)max_seqlen_q * num_q_heads + kMergeWarps - 1) / kMergeWarps;
-  return cuda_status(launch_kernel(tree_merge_kernel, dim3((unsigned)(mrows < 4096 ? mrows : 4096), (unsigned)batch),
-                                   dim3(kMergeWarps * 32), 0, (cudaStream_t)stream, a),
+  // rows of many partials come with few rows in all: a block each then
+  const int64_t mrows = (int64_t)max_seqlen_q * num_q_heads;
+  const int rpb = mrows * batch <= 8 * device_sm_count() ? 1 : kMergeWarps;
+  const int64_t mblocks = (mrows + rpb - 1) / rpb;
+  return cuda_status(launch_kernel(tree_merge_kernel, dim3((unsigned)(mblocks < 8192 ? mblocks : 8192), (unsigned)batch),
+                                   dim3(kMergeWarps * 32), 0, st, a, rpb),
                      "kvb_tree_attn merge launch");
 }

@@ -2,10 +2,10 @@
 //
 // A unit is one (sequence, kv head, block of query rows): it walks the
 // sequence's context in tiles of tokens. The tiles of all units, in the order
-// sequence > kv head > row block, form one line that is cut into `parts`
-// contiguous ranges of equal length, one per CTA: every CTA streams the same
-// number of K/V bytes whatever the lengths of the sequences are, and the host
-// needs none of the device's lengths. A unit cut between CTAs leaves fp32
+// sequence > kv head > row block, form one line that is cut into ranges of
+// equal length, one per CTA (at most `parts`): every CTA streams the same number
+// of K/V bytes whatever the lengths of the sequences are, and the host needs
+// none of the device's lengths. A unit cut between CTAs leaves fp32
 // partials (unnormalised rows, running maximum and sum) that the merge joins
 // in order, so results do not depend on timing. Included by tree_attn.cu after
 // its error word.
@@ -41,6 +41,7 @@ struct Args {
   float* part_o;          // [parts][2][rows][128]
   float* part_m;          // [parts][2][rows]
   float* part_l;
+  int64_t* first;         // [batch + 1]: tiles before each sequence, written for the merge
   float scale_log2;
 };
 
@@ -97,10 +98,12 @@ __device__ __forceinline__ int64_t block_prefix(int64_t mine, int64_t* total) {
   return before + incl - mine;
 }
 
-__device__ __forceinline__ int64_t part_begin(int64_t total, int parts, int p) { return total * p / parts; }
+// Tiles of a range; part p holds [p * range, (p + 1) * range) of the line.
+__device__ __forceinline__ int64_t range_of(int64_t total, int parts) { return (total + parts - 1) / parts; }
 
 // Where this CTA's range starts: the sequence, the offset in its tiles, and
-// how many tiles the range has. Every thread of the block calls it.
+// how many tiles the range has. Every thread of the block calls it; block 0
+// leaves the line's prefix sums for the merge.
 struct Start {
   int b;
   int64_t off, left;
@@ -114,18 +117,17 @@ __device__ __forceinline__ Start find_start(const Args& a, int part) {
   for (int b = b0; b < b1; ++b) mine += cost_of(a, seq_of(a, b, part == 0));
   int64_t total;
   int64_t at = block_prefix<kThreads>(mine, &total);
-  const int64_t lo = part_begin(total, a.parts, part), hi = part_begin(total, a.parts, part + 1);
+  const int64_t range = range_of(total, a.parts), lo = range * part, hi = min(lo + range, total);
   if (threadIdx.x == 0) s_start = Start{0, 0, 0};
   __syncthreads();
-  if (lo < hi && at <= lo && lo < at + mine) {
+  if (part == 0 || (lo < hi && at <= lo && lo < at + mine)) {
     for (int b = b0; b < b1; ++b) {
       const int64_t c = cost_of(a, seq_of(a, b, false));
-      if (lo < at + c) {
-        s_start = Start{b, lo - at, hi - lo};
-        break;
-      }
+      if (part == 0) a.first[b] = at;
+      if (at <= lo && lo < min(at + c, hi)) s_start = Start{b, lo - at, hi - lo};
       at += c;
     }
+    if (part == 0 && threadIdx.x == 0) a.first[a.batch] = total;
   }
   __syncthreads();
   return s_start;

@@ -104,9 +104,9 @@ def test_empty_work_is_success(lib, name, change):
 
 def test_workspace_size(lib):
     n = ctypes.c_size_t(0)
-    assert lib.kvb_tree_attn_workspace_size(32, 8, 16, ctypes.byref(n)) == 0 and n.value > 0
-    assert lib.kvb_tree_attn_workspace_size(33, 8, 16, ctypes.byref(n)) == INVALID
-    assert lib.kvb_tree_attn_workspace_size(32, 8, 16, None) == INVALID
+    assert lib.kvb_tree_attn_workspace_size(4, 32, 8, 16, ctypes.byref(n)) == 0 and n.value > 0
+    assert lib.kvb_tree_attn_workspace_size(4, 33, 8, 16, ctypes.byref(n)) == INVALID
+    assert lib.kvb_tree_attn_workspace_size(4, 32, 8, 16, None) == INVALID
 
 
 def test_wrappers_refuse_cpu_tensors():
