@@ -30,14 +30,13 @@ using tree::kHD;
 using tree::Walk;
 
 // ------------------------------------------------------------- warp-MMA kernel
-// 8 NT query rows (nodes x query heads of one kv head) per unit, 64-token tiles
-// staged by TMA; each of four consumer warps takes 16 tokens of a tile. Tokens
+// 8 NT query rows (nodes x query heads of one kv head) per unit, tiles of 64 KT
+// tokens staged by TMA; each of four consumer warps takes 16 KT tokens of a tile. Tokens
 // (then head dims) are the MMAs' 16-row side and query rows their 8-column side,
 // S^T = K Q^T and O^T = V^T P^T, so a decode step's 4 to 8 query heads fill the
 // instructions and K and V are converted once for all rows. e4m3 bytes become
 // halves in registers (exact); two 8x8 register transposes turn the weights from
 // S^T's layout to P^T's.
-constexpr int kTile = 64;
 constexpr int kWarps = 4;
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kScratchStride = kHD + 4;  // fp32 row of the warp merge, padded against bank conflicts
@@ -45,25 +44,35 @@ constexpr int kScratchStride = kHD + 4;  // fp32 row of the warp merge, padded a
 template <bool kFp8, int NT>
 struct Cfg {
   static constexpr int kRows = 8 * NT;
+  // e4m3 tiles hold twice the tokens: as many bytes a stage, and two chains of
+  // MMAs a warp, whose softmax steps overlap
+  static constexpr int KT = kFp8 ? 2 : 1;
+  static constexpr int kTile = 64 * KT;
   static constexpr int kKV = kTile * kHD * (kFp8 ? 1 : 2);  // bytes of a K (or V) tile
   static constexpr int kStage = 2 * kKV;
   // CTAs an SM holds, and stages that fit its shared memory then
-  static constexpr int kCtas = kFp8 ? (NT == 1 ? 4 : 3) : 2;
-  static constexpr int kStages = kFp8 ? (NT == 1 ? 3 : 4) : 3;
+  static constexpr int kCtas = kFp8 && NT == 1 ? 3 : 2;
+  static constexpr int kStages = kFp8 && NT == 1 ? 2 : 3;
   static constexpr int kSmem = kStages * kStage + kRows * kScratchStride * 4 + 1024;
 };
 
-__device__ __forceinline__ uint32_t swz_bf16(uint32_t base, int row, int chunk) {
-  return base + (chunk >> 3) * (kTile * 128) + row * 128 + ((((chunk & 7) ^ (row & 7))) << 4);
-}
-__device__ __forceinline__ uint32_t swz_fp8(uint32_t base, int row, int chunk) {
-  return base + row * 128 + ((chunk ^ (row & 7)) << 4);
+// 16-byte chunk of a token's row in a tile: e4m3 rows are 128 bytes; bf16 rows
+// two halves of 64 dims, a half tile apart. 128-byte swizzle.
+template <bool kFp8>
+__device__ __forceinline__ uint32_t swz(uint32_t base, int row, int chunk) {
+  if constexpr (kFp8) return base + row * 128 + ((chunk ^ (row & 7)) << 4);
+  return base + (chunk >> 3) * (64 * 128) + row * 128 + ((((chunk & 7) ^ (row & 7))) << 4);
 }
 
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
+}
+
+// Adds bytes to the transactions the barrier's current phase waits for.
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
 __device__ __forceinline__ void mma_f16_16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1) {
@@ -105,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
     tree_warp_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                      const __grid_constant__ Args a) {
   using C = Cfg<kFp8, NT>;
-  constexpr int kRows = C::kRows;
+  constexpr int kRows = C::kRows, KT = C::KT, kTile = C::kTile;
   kernel_entry();
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[C::kStages];
@@ -144,31 +153,44 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
             break;
           }
           const int tok = (w.t0 + j) * kTile;
-          if (tok / a.block_size != col) {
-            col = tok / a.block_size;
-            blk = a.tables[(int64_t)w.b * a.bt_stride + col];  // col < max_blocks: the length is cut to the table
-            bad = blk < 0 || blk >= a.num_blocks;
-            if (bad) {
-              atomicOr(&g_err_tree, (unsigned)kErrBlockTable);
-              blk = a.num_blocks;  // out of the tensor map: TMA fills zeros
-            }
-          }
-          const int off = tok - col * a.block_size;
           const uint32_t st = smem_u32(smem + s * C::kStage);
           const uint32_t fb = smem_u32(&full_bar[s]);
-          if (kFp8 && bad) {  // a block outside the pool reads zeros, of scale 1
-            for (int i = 0; i < 2 * kTile / 4; ++i) reinterpret_cast<uint32_t*>(&scales[s][0][0])[i] = 0x7f7f7f7fu;
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before a later copy into the same bytes
-          }
-          mbar_arrive_expect_tx(fb, C::kStage + (kFp8 && !bad ? 2 * kTile : 0));
-          tma_load_4d(st, &kmap, 0, w.h, off, blk, fb, pol);
-          if constexpr (!kFp8) tma_load_4d(st + C::kKV / 2, &kmap, 64, w.h, off, blk, fb, pol);
-          tma_load_4d(st + C::kKV, &vmap, 0, w.h, off, blk, fb, pol);
-          if constexpr (!kFp8) tma_load_4d(st + C::kKV + C::kKV / 2, &vmap, 64, w.h, off, blk, fb, pol);
-          if (kFp8 && !bad) {
-            const int64_t so = blk * a.scale_stride + (int64_t)w.h * a.block_size + off;
-            bulk_load(smem_u32(&scales[s][0][0]), a.ks + so, kTile, fb);
-            bulk_load(smem_u32(&scales[s][1][0]), a.vs + so, kTile, fb);
+          // a tile is one box, or two when the pages hold 64 tokens (their second
+          // half may lie past the sequence: it is read as zeros then)
+          const int boxes = kTile / a.box;
+          for (int x = 0; x < boxes; ++x) {
+            const int at = tok + x * a.box;
+            if (at / a.block_size != col) {
+              col = at / a.block_size;
+              const bool past = at >= w.s.len;
+              blk = past ? -1 : a.tables[(int64_t)w.b * a.bt_stride + col];  // len is cut to the table
+              bad = blk < 0 || blk >= a.num_blocks;
+              if (bad) {
+                if (!past) atomicOr(&g_err_tree, (unsigned)kErrBlockTable);
+                blk = a.num_blocks;  // out of the tensor map: TMA fills zeros
+              }
+            }
+            const int off = at - col * a.block_size;
+            if (kFp8 && bad) {  // a block outside the pool reads zeros, of scale 1
+              for (int i = 0; i < 2; ++i)
+                for (int k = 0; k < a.box / 4; ++k) reinterpret_cast<uint32_t*>(&scales[s][i][x * a.box])[k] = 0x7f7f7f7fu;
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before a later copy into the same bytes
+            }
+            const uint32_t bytes = 2 * (C::kKV / boxes) + (kFp8 && !bad ? 2 * a.box : 0);
+            if (x + 1 < boxes)
+              mbar_expect_tx(fb, bytes);
+            else
+              mbar_arrive_expect_tx(fb, bytes);
+            const uint32_t kd = st + x * a.box * 128, vd = kd + C::kKV;
+            tma_load_4d(kd, &kmap, 0, w.h, off, blk, fb, pol);
+            if constexpr (!kFp8) tma_load_4d(kd + C::kKV / 2, &kmap, 64, w.h, off, blk, fb, pol);
+            tma_load_4d(vd, &vmap, 0, w.h, off, blk, fb, pol);
+            if constexpr (!kFp8) tma_load_4d(vd + C::kKV / 2, &vmap, 64, w.h, off, blk, fb, pol);
+            if (kFp8 && !bad) {
+              const int64_t so = blk * a.scale_stride + (int64_t)w.h * a.block_size + off;
+              bulk_load(smem_u32(&scales[s][0][x * a.box]), a.ks + so, a.box, fb);
+              bulk_load(smem_u32(&scales[s][1][x * a.box]), a.vs + so, a.box, fb);
+            }
           }
         }
       }
@@ -183,7 +205,15 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
   // Lane (g, j4): tokens g and g + 8 of the warp's sixteen and query rows
   // 8 t + 2 j4, + 1 of S^T; the same rows and the dims of dim_of() of O^T.
   const int g = lane >> 2, j4 = lane & 3, mi = lane >> 3;
-  const int tok0 = warp * 16;
+  const int tok0 = warp * 16 * KT;
+  // shared-memory offsets of this lane's rows in ldmatrix: 4 pairs of chunks;
+  // chunks of a bf16 row's other half and the other tokens are constants apart
+  uint32_t koff[4], voff[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    koff[i] = swz<kFp8>(0, tok0 + (lane & 7) + ((mi & 1) << 3), i * 2 + (mi >> 1));
+    voff[i] = kFp8 ? koff[i] : swz<kFp8>(0, tok0 + (lane & 7) + ((mi >> 1) << 3), i * 2 + (mi & 1));
+  }
   uint32_t it = 0;
   bool ok = true;
   while (w.next(a)) {
@@ -251,14 +281,15 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
       const uint32_t kb = smem_u32(smem + s * C::kStage), vb = kb + C::kKV;
       const int p0 = (w.t0 + jt) * kTile + tok0;  // position of this warp's first token
       bool odd_v = false;                          // a node's V row holds a value that is not finite
-      if (p0 + 16 > base) {
+      const bool tail = p0 + 16 * KT > base;
+      if (tail) {
         // The warp's tokens reach into the draft or past the context. Rows past
         // the context hold stale bytes (possibly NaN): zero them, since a zero
         // weight does not cancel NaN. Drafted rows may be hidden from some of
         // the query rows: look for values that a zero weight would not cancel.
-        for (int idx = lane; idx < 16 * (kFp8 ? 8 : 16); idx += 32) {
+        for (int idx = lane; idx < 16 * KT * (kFp8 ? 8 : 16); idx += 32) {
           const int row = kFp8 ? idx >> 3 : idx >> 4, chunk = kFp8 ? idx & 7 : idx & 15;
-          const uint32_t ad = kFp8 ? swz_fp8(vb, tok0 + row, chunk) : swz_bf16(vb, tok0 + row, chunk);
+          const uint32_t ad = swz<kFp8>(vb, tok0 + row, chunk);
           if (p0 + row >= w.s.len) {
             asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(ad), "r"(0u) : "memory");
           } else if (p0 + row >= base) {
@@ -275,73 +306,84 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
         odd_v = __any_sync(0xffffffffu, odd_v);
       }
 
-      // S^T: element 2 h + i is token g + 8 h, row 8 t + 2 j4 + i
-      float sc[NT][4];
+      // S^T of 16 tokens k: element 2 h + i is token 16 k + g + 8 h, row 8 t + 2 j4 + i
+      float sc[KT][NT][4];
 #pragma unroll
-      for (int t = 0; t < NT; ++t) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+      for (int k = 0; k < KT; ++k)
+#pragma unroll
+        for (int t = 0; t < NT; ++t) sc[k][t][0] = sc[k][t][1] = sc[k][t][2] = sc[k][t][3] = 0.f;
       if constexpr (kFp8) {
         // k-step ks covers 16 dims; lane j4 holds dims 4 j4 .. 4 j4 + 3 of it,
         // for K and Q alike (any order of the dims gives the same sum)
 #pragma unroll
-        for (int kp = 0; kp < 4; ++kp) {
-          uint32_t b[4];
-          ldmatrix_x4(swz_fp8(kb, tok0 + (lane & 7) + ((mi & 1) << 3), kp * 2 + (mi >> 1)), b[0], b[1], b[2], b[3]);
+        for (int kp = 0; kp < 4; ++kp)
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            uint32_t ka[4];
-            e4m3x4_to_half(b[2 * q], ka[0], ka[2]);
-            e4m3x4_to_half(b[2 * q + 1], ka[1], ka[3]);
+          for (int k = 0; k < KT; ++k) {
+            uint32_t b[4];
+            ldmatrix_x4(kb + koff[kp] + k * 2048, b[0], b[1], b[2], b[3]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_f16_16816(sc[t], ka, qb[t][kp * 2 + q][0], qb[t][kp * 2 + q][1]);
+            for (int q = 0; q < 2; ++q) {
+              uint32_t ka[4];
+              e4m3x4_to_half(b[2 * q], ka[0], ka[2]);
+              e4m3x4_to_half(b[2 * q + 1], ka[1], ka[3]);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) mma_f16_16816(sc[k][t], ka, qb[t][kp * 2 + q][0], qb[t][kp * 2 + q][1]);
+            }
           }
-        }
       } else {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           uint32_t ka[4];
-          ldmatrix_x4(swz_bf16(kb, tok0 + (lane & 7) + ((mi & 1) << 3), ks * 2 + (mi >> 1)), ka[0], ka[1], ka[2], ka[3]);
+          ldmatrix_x4(kb + koff[ks & 3] + (ks >> 2) * (64 * 128), ka[0], ka[1], ka[2], ka[3]);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) mma_bf16_16816(sc[t], ka, qb[t][ks][0], qb[t][ks][1]);
+          for (int t = 0; t < NT; ++t) mma_bf16_16816(sc[0][t], ka, qb[t][ks][0], qb[t][ks][1]);
         }
       }
 
-      float inv_v[2];  // 2^-exponent of the V rows of this lane's tokens
+      float inv_v[KT][2];  // 2^-exponent of the V rows of this lane's tokens
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if constexpr (kFp8) {
-          const uint32_t kc = scales[s][0][tok0 + g + 8 * h], vc = scales[s][1][tok0 + g + 8 * h];
-          const float ksc = __uint_as_float(kc << 23);
-          const float ev = __uint_as_float(0x4b000000u | vc) - (8388608.f + 127.f);  // vc - 127
-          inv_v[h] = __uint_as_float((254u - vc) << 23);
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) sc[t][2 * h + i] = fmaf(sc[t][2 * h + i], rscale[t][i] * ksc, ev);
-        } else {
-#pragma unroll
-          for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) sc[t][2 * h + i] *= rscale[t][i];
-        }
-      }
-      uint32_t hidden = 0;  // bit 4 t + 2 h + i: that score is masked
-      if (p0 + 16 > base) {
+      for (int k = 0; k < KT; ++k)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int pos = p0 + g + 8 * h;
-          if (kFp8 && !(inv_v[h] >= 0.f && inv_v[h] < INFINITY)) inv_v[h] = 0.f;  // stale scale bytes
+          if constexpr (kFp8) {
+            const int tk = tok0 + k * 16 + g + 8 * h;
+            const uint32_t kc = scales[s][0][tk], vc = scales[s][1][tk];
+            const float ksc = __uint_as_float(kc << 23);
+            const float ev = __uint_as_float(0x4b000000u | vc) - (8388608.f + 127.f);  // vc - 127
+            inv_v[k][h] = __uint_as_float((254u - vc) << 23);
 #pragma unroll
-          for (int t = 0; t < NT; ++t)
+            for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int node = (w.rb * kRows + t * 8 + 2 * j4 + i) / a.group;
-              const bool seen = pos < base || (pos < w.s.len && node < w.s.nodes &&
-                                               tree::sees(a, w.s.q0 + node, node, pos - base));
-              if (!seen) {
-                sc[t][2 * h + i] = -INFINITY;
-                hidden |= 1u << (4 * t + 2 * h + i);
+              for (int i = 0; i < 2; ++i) sc[k][t][2 * h + i] = fmaf(sc[k][t][2 * h + i], rscale[t][i] * ksc, ev);
+          } else {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) sc[k][t][2 * h + i] *= rscale[t][i];
+          }
+        }
+      uint32_t hidden[KT];  // bit 4 t + 2 h + i: that score is masked
+      if (tail) {
+#pragma unroll
+        for (int k = 0; k < KT; ++k) {
+          hidden[k] = 0;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int pos = p0 + k * 16 + g + 8 * h;
+            if (kFp8 && !(inv_v[k][h] >= 0.f && inv_v[k][h] < INFINITY)) inv_v[k][h] = 0.f;  // stale scale bytes
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int node = (w.rb * kRows + t * 8 + 2 * j4 + i) / a.group;
+                const bool seen = pos < base || (pos < w.s.len && node < w.s.nodes &&
+                                                 tree::sees(a, w.s.q0 + node, node, pos - base));
+                if (!seen) {
+                  sc[k][t][2 * h + i] = -INFINITY;
+                  hidden[k] |= 1u << (4 * t + 2 * h + i);
+                }
               }
-            }
+          }
         }
       }
       float corr[NT][2];
@@ -350,7 +392,9 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float mx = fmaxf(sc[t][i], sc[t][2 + i]);
+          float mx = fmaxf(sc[0][t][i], sc[0][t][2 + i]);
+#pragma unroll
+          for (int k = 1; k < KT; ++k) mx = fmaxf(mx, fmaxf(sc[k][t][i], sc[k][t][2 + i]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
@@ -358,10 +402,16 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
           const float ref = m_new == -INFINITY ? 0.f : m_new;
           moved |= mx > m_run[t][i];
           corr[t][i] = ex2(m_run[t][i] - ref);
-          const float x0 = ex2(sc[t][i] - ref), x1 = ex2(sc[t][2 + i] - ref);
-          sc[t][i] = x0;
-          sc[t][2 + i] = x1;
-          l_run[t][i] = fmaf(l_run[t][i], corr[t][i], kFp8 ? fmaf(x0, inv_v[0], x1 * inv_v[1]) : x0 + x1);
+          float sum = 0.f;
+#pragma unroll
+          for (int k = 0; k < KT; ++k)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const float x = ex2(sc[k][t][2 * h + i] - ref);
+              sc[k][t][2 * h + i] = x;
+              sum = kFp8 ? fmaf(x, inv_v[k][h], sum) : sum + x;
+            }
+          l_run[t][i] = fmaf(l_run[t][i], corr[t][i], sum);
           m_run[t][i] = m_new;
         }
       if (__any_sync(0xffffffffu, moved)) {  // rarely after a row's first tiles; otherwise every factor is 1
@@ -374,69 +424,74 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
       }
       if (!odd_v) {
         // the weights are rounded to the type of the V operand: bf16, or half (2^-12) for e4m3
-        uint32_t pb[NT][2];
+        uint32_t pb[KT][NT][2];
 #pragma unroll
-        for (int t = 0; t < NT; ++t)
+        for (int k = 0; k < KT; ++k)
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
-            pb[t][h] = transpose8(kFp8 ? pack_half(sc[t][2 * h], sc[t][2 * h + 1]) : pack_bf16(sc[t][2 * h], sc[t][2 * h + 1]));
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              pb[k][t][h] = transpose8(kFp8 ? pack_half(sc[k][t][2 * h], sc[k][t][2 * h + 1])
+                                            : pack_bf16(sc[k][t][2 * h], sc[k][t][2 * h + 1]));
         if constexpr (kFp8) {
           // A transposed 8x8 of 16-bit elements gives a lane two tokens of a
           // pair of dims; a byte permutation pairs the tokens of each dim. Row
           // g of the MMA is dim 2 g of the 16-dim chunk, row g + 8 dim 2 g + 1.
 #pragma unroll
-          for (int cp = 0; cp < 4; ++cp) {
-            uint32_t b[4];
-            ldmatrix_x4_trans(swz_fp8(vb, tok0 + (lane & 7) + ((mi & 1) << 3), cp * 2 + (mi >> 1)), b[0], b[1], b[2],
-                              b[3]);
+          for (int cp = 0; cp < 4; ++cp)
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              uint32_t va[4];
-              e4m3x4_to_half(__byte_perm(b[2 * q], 0, 0x3120), va[0], va[1]);
-              e4m3x4_to_half(__byte_perm(b[2 * q + 1], 0, 0x3120), va[2], va[3]);
+            for (int k = 0; k < KT; ++k) {
+              uint32_t b[4];
+              ldmatrix_x4_trans(vb + voff[cp] + k * 2048, b[0], b[1], b[2], b[3]);
 #pragma unroll
-              for (int t = 0; t < NT; ++t) mma_f16_16816(o[t][2 * cp + q], va, pb[t][0], pb[t][1]);
+              for (int q = 0; q < 2; ++q) {
+                uint32_t va[4];
+                e4m3x4_to_half(__byte_perm(b[2 * q], 0, 0x3120), va[0], va[1]);
+                e4m3x4_to_half(__byte_perm(b[2 * q + 1], 0, 0x3120), va[2], va[3]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) mma_f16_16816(o[t][2 * cp + q], va, pb[k][t][0], pb[k][t][1]);
+              }
             }
-          }
         } else {
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             uint32_t va[4];
-            ldmatrix_x4_trans(swz_bf16(vb, tok0 + (lane & 7) + ((mi >> 1) << 3), 2 * c + (mi & 1)), va[0], va[1], va[2],
-                              va[3]);
+            ldmatrix_x4_trans(vb + voff[c & 3] + (c >> 2) * (64 * 128), va[0], va[1], va[2], va[3]);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) mma_bf16_16816(o[t][c], va, pb[t][0], pb[t][1]);
+            for (int t = 0; t < NT; ++t) mma_bf16_16816(o[t][c], va, pb[0][t][0], pb[0][t][1]);
           }
         }
       } else {
         // a drafted V row that is not finite: add only what each row sees, token
         // by token (rare, so it is written for size)
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
 #pragma unroll 1
-        for (int tk = 0; tk < 16; ++tk) {
-          const int src = (tk & 7) * 4 + j4, h = tk >> 3;
-          const uint32_t hid = __shfl_sync(0xffffffffu, hidden, src);
+          for (int tk = 0; tk < 16; ++tk) {
+            const int src = (tk & 7) * 4 + j4, h = tk >> 3, row = tok0 + 16 * k + tk;
+            const uint32_t hid = __shfl_sync(0xffffffffu, hidden[k], src);
 #pragma unroll
-          for (int t = 0; t < NT; ++t) {
-            const float p0t = __shfl_sync(0xffffffffu, h ? sc[t][2] : sc[t][0], src);
-            const float p1t = __shfl_sync(0xffffffffu, h ? sc[t][3] : sc[t][1], src);
-            const bool see0 = !((hid >> (4 * t + 2 * h)) & 1u), see1 = !((hid >> (4 * t + 2 * h + 1)) & 1u);
+            for (int t = 0; t < NT; ++t) {
+              const float p0t = __shfl_sync(0xffffffffu, h ? sc[k][t][2] : sc[k][t][0], src);
+              const float p1t = __shfl_sync(0xffffffffu, h ? sc[k][t][3] : sc[k][t][1], src);
+              const bool see0 = !((hid >> (4 * t + 2 * h)) & 1u), see1 = !((hid >> (4 * t + 2 * h + 1)) & 1u);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              float v0, v1;  // this lane's two dims of chunk c
-              if constexpr (kFp8) {
-                uint32_t h01, unused;
-                e4m3x4_to_half(lds16(swz_fp8(vb, tok0 + tk, c) + g * 2), h01, unused);
-                const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h01));
-                v0 = v.x, v1 = v.y;
-              } else {
-                v0 = __uint_as_float(lds16(swz_bf16(vb, tok0 + tk, 2 * c) + g * 2) << 16);
-                v1 = __uint_as_float(lds16(swz_bf16(vb, tok0 + tk, 2 * c + 1) + g * 2) << 16);
+              for (int c = 0; c < 8; ++c) {
+                float v0, v1;  // this lane's two dims of chunk c
+                if constexpr (kFp8) {
+                  uint32_t h01, unused;
+                  e4m3x4_to_half(lds16(swz<kFp8>(vb, row, c) + g * 2), h01, unused);
+                  const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&h01));
+                  v0 = v.x, v1 = v.y;
+                } else {
+                  v0 = __uint_as_float(lds16(swz<kFp8>(vb, row, 2 * c) + g * 2) << 16);
+                  v1 = __uint_as_float(lds16(swz<kFp8>(vb, row, 2 * c + 1) + g * 2) << 16);
+                }
+                if (see0) o[t][c][0] += p0t * v0, o[t][c][2] += p0t * v1;
+                if (see1) o[t][c][1] += p1t * v0, o[t][c][3] += p1t * v1;
               }
-              if (see0) o[t][c][0] += p0t * v0, o[t][c][2] += p0t * v1;
-              if (see1) o[t][c][1] += p1t * v0, o[t][c][3] += p1t * v1;
             }
           }
-        }
       }
       // order this warp's generic-proxy writes (tail zeroing) before the
       // producer's next async-proxy (TMA) write into the stage
@@ -585,25 +640,30 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __gr
   __shared__ Joined s_join[kMergeWarps][32];
   const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const tree::Seq s = tree::seq_of(a, b, false);
-  const int64_t rows = (int64_t)s.nodes * a.hq;
+  const int64_t rows = (int64_t)s.nodes * a.hq;  // fits 31 bits: the host checked total_q * hq
   const int64_t first = a.first[b], range = tree::range_of(a.first[a.batch], a.parts);
   for (int64_t i0 = (int64_t)blockIdx.x * rows_per_block; i0 < rows; i0 += (int64_t)gridDim.x * rows_per_block) {
     // where the parts of row i are
     int c0 = 0, n = 0, row = 0;
     bf16* op = nullptr;
     const auto locate = [&](int64_t i) {
-      const int nd = (int)(i / a.hq), head = (int)(i - (int64_t)nd * a.hq), h = head / a.group;
+      const int nd = (int)i / a.hq, head = (int)i - nd * a.hq, h = head / a.group;
       op = a.out + (int64_t)(s.q0 + nd) * a.o_st + (int64_t)head * a.o_sh + lane * 4;
       if (s.tiles == 0) {
         n = 0;
         return;
       }
-      const int64_t R = (int64_t)nd * a.group + head - h * a.group;
-      const int rb = (int)(R / a.rows);
-      row = (int)(R - (int64_t)rb * a.rows);
+      const int R = nd * a.group + head - h * a.group, rb = R / a.rows;
+      row = R - rb * a.rows;
       const int64_t lo = first + ((int64_t)h * s.blocks + rb) * s.tiles;
-      c0 = (int)(lo / range);
-      n = (int)((lo + s.tiles - 1) / range) - c0 + 1;
+      const int64_t hi = lo + s.tiles - 1;
+      if (hi <= UINT32_MAX) {  // nearly always: a 64-bit division takes ten times as long
+        c0 = (int)((uint32_t)lo / (uint32_t)range);
+        n = (int)((uint32_t)hi / (uint32_t)range) - c0 + 1;
+      } else {
+        c0 = (int)(lo / range);
+        n = (int)(hi / range) - c0 + 1;
+      }
     };
     const auto write = [&](const Joined& x) {
       const float inv = x.l == 0.f ? 0.f : 1.f / x.l;
@@ -618,6 +678,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __gr
       else if (n > 1 && n <= kFew)
         write(join_parts(a, c0, n, 0, 1, row, lane));
     }
+    if (!__syncthreads_or(n > kFew)) continue;
     for (int r = 0; r < mine; ++r) {
       locate(i0 + r);
       if (n <= kFew) continue;  // the same for the whole block
@@ -700,6 +761,7 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
     return set_error(kInvalid, "kvb_tree_attn: bad sizes");
   if (head_dim != kHD) return set_error(kUnsupported, "kvb_tree_attn: head_dim must be 128");
   if (block_size % 64) return set_error(kUnsupported, "kvb_tree_attn: block_size must be a multiple of 64");
+  if (total_q * num_q_heads > INT32_MAX) return set_error(kUnsupported, "kvb_tree_attn: more than 2^31 query rows");
   if (batch > 65535) return set_error(kUnsupported, "kvb_tree_attn: more than 65535 sequences");
   if ((int64_t)max_blocks_per_seq * block_size > INT32_MAX - 1024)
     return set_error(kUnsupported, "kvb_tree_attn: block tables of more than 2^31 tokens");
@@ -724,7 +786,8 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   Args a = {};
   const int group = num_q_heads / num_kv_heads;
   a.rows = (int64_t)group * max_seqlen_q <= 8 ? 8 : 16;
-  a.tile = kTile;
+  a.tile = fp8 ? Cfg<true, 1>::kTile : Cfg<false, 1>::kTile;
+  a.box = block_size % a.tile == 0 ? a.tile : 64;
   // what the SMs hold: one wave
   a.parts = device_sm_count() * (a.rows == 8 ? (fp8 ? Cfg<true, 1>::kCtas : Cfg<false, 1>::kCtas)
                                              : (fp8 ? Cfg<true, 2>::kCtas : Cfg<false, 2>::kCtas));
@@ -765,8 +828,8 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
 
   CUtensorMap km, vm;
   const int64_t bytes = block_stride * (fp8 ? 1 : 2);
-  int rc = encode_pages(&km, k_cache, fp8, num_blocks, bytes, block_size, num_kv_heads, a.tile);
-  if (!rc) rc = encode_pages(&vm, v_cache, fp8, num_blocks, bytes, block_size, num_kv_heads, a.tile);
+  int rc = encode_pages(&km, k_cache, fp8, num_blocks, bytes, block_size, num_kv_heads, a.box);
+  if (!rc) rc = encode_pages(&vm, v_cache, fp8, num_blocks, bytes, block_size, num_kv_heads, a.box);
   const cudaStream_t st = (cudaStream_t)stream;
   if (!rc)
     rc = a.rows == 8 ? (fp8 ? launch_warp<true, 1>(km, vm, a, st) : launch_warp<false, 1>(km, vm, a, st))

@@ -38,6 +38,7 @@ struct Args {
   int batch, hq, hkv, group;
   int num_blocks, block_size;
   int parts, rows, tile;  // CTAs of the attention grid, query rows of a unit, tokens of a tile
+  int box;                // tokens of a TMA box: a tile's, or a page's when that is smaller
   float* part_o;          // [parts][2][rows][128]
   float* part_m;          // [parts][2][rows]
   float* part_l;
