@@ -30,8 +30,9 @@ using tree::kHD;
 using tree::Walk;
 
 // ------------------------------------------------------------- warp-MMA kernel
-// 8 NT query rows (nodes x query heads of one kv head) per unit, tiles of 64 KT
-// tokens staged by TMA; each of four consumer warps takes 16 KT tokens of a tile. Tokens
+// 8 NT query rows (nodes x query heads) of each of HP kv heads per unit, tiles of
+// 64 KT / HP tokens staged by TMA; each of four consumer warps takes 16 KT tokens
+// of one head. Tokens
 // (then head dims) are the MMAs' 16-row side and query rows their 8-column side,
 // S^T = K Q^T and O^T = V^T P^T, so a decode step's 4 to 8 query heads fill the
 // instructions and K and V are converted once for all rows. e4m3 bytes become
@@ -41,19 +42,26 @@ constexpr int kWarps = 4;
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kScratchStride = kHD + 4;  // fp32 row of the warp merge, padded against bank conflicts
 
-template <bool kFp8, int NT>
+template <bool kFp8, int NT, int HP>
 struct Cfg {
   static constexpr int kRows = 8 * NT;
   // e4m3 tiles hold twice the tokens: as many bytes a stage, and two chains of
   // MMAs a warp, whose softmax steps overlap
   static constexpr int KT = kFp8 ? 2 : 1;
-  static constexpr int kTile = 64 * KT;
-  static constexpr int kKV = kTile * kHD * (kFp8 ? 1 : 2);  // bytes of a K (or V) tile
+  // A token's row of one e4m3 head is 128 bytes, num_kv_heads * 128 apart. One
+  // head a unit left HBM at 5.1 TB/s (256 x 1024 tokens, 8 heads, loads alone):
+  // the heads of the same tokens were fetched at other times. Neighbouring heads
+  // of a unit are fetched together.
+  static constexpr int kGroups = kWarps / HP;        // warps that share a head's tokens
+  static constexpr int kTile = 16 * KT * kGroups;
+  static constexpr int kHead = kTile * kHD * (kFp8 ? 1 : 2);  // bytes of a head's K (or V) tile
+  static constexpr int kKV = HP * kHead;
   static constexpr int kStage = 2 * kKV;
   // CTAs an SM holds, and stages that fit its shared memory then
   static constexpr int kCtas = kFp8 && NT == 1 ? 3 : 2;
-  static constexpr int kStages = kFp8 && NT == 1 ? 2 : 3;
-  static constexpr int kSmem = kStages * kStage + kRows * kScratchStride * 4 + 1024;
+  static constexpr int kStages = kFp8 && (NT == 1 || HP == 2) ? 2 : 3;
+  static constexpr int kScratch = kGroups > 1 ? HP * kRows * kScratchStride * 4 : 0;
+  static constexpr int kSmem = kStages * kStage + kScratch + 1024;
 };
 
 // 16-byte chunk of a token's row in a tile: e4m3 rows are 128 bytes; bf16 rows
@@ -109,17 +117,18 @@ __device__ __forceinline__ uint32_t lds16(uint32_t addr) {
   return v;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-template <bool kFp8, int NT>
-__global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
+template <bool kFp8, int NT, int HP>
+__global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
     tree_warp_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
                      const __grid_constant__ Args a) {
-  using C = Cfg<kFp8, NT>;
+  using C = Cfg<kFp8, NT, HP>;
+  static_assert(C::kCtas * (C::kSmem + 1408 + 1024) <= 228 * 1024, "the CTAs of an SM share its memory (with 1.4 KB of static, 1 KB reserved each)");
   constexpr int kRows = C::kRows, KT = C::KT, kTile = C::kTile;
   kernel_entry();
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t full_bar[C::kStages];
   __shared__ __align__(8) uint64_t empty_bar[C::kStages];
-  __shared__ __align__(16) uint8_t scales[C::kStages][2][kTile];
+  __shared__ __align__(16) uint8_t scales[C::kStages][2][HP * kTile];
   __shared__ float mw[kWarps][kRows], lw[kWarps][kRows];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* scratch = reinterpret_cast<float*>(smem + C::kStages * C::kStage);
@@ -173,23 +182,30 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
             const int off = at - col * a.block_size;
             if (kFp8 && bad) {  // a block outside the pool reads zeros, of scale 1
               for (int i = 0; i < 2; ++i)
-                for (int k = 0; k < a.box / 4; ++k) reinterpret_cast<uint32_t*>(&scales[s][i][x * a.box])[k] = 0x7f7f7f7fu;
+                for (int h = 0; h < HP; ++h)
+                  for (int k = 0; k < a.box / 4; ++k)
+                    reinterpret_cast<uint32_t*>(&scales[s][i][h * kTile + x * a.box])[k] = 0x7f7f7f7fu;
               asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before a later copy into the same bytes
             }
-            const uint32_t bytes = 2 * (C::kKV / boxes) + (kFp8 && !bad ? 2 * a.box : 0);
+            const uint32_t bytes = 2 * (C::kKV / boxes) + (kFp8 && !bad ? 2 * HP * a.box : 0);
             if (x + 1 < boxes)
               mbar_expect_tx(fb, bytes);
             else
               mbar_arrive_expect_tx(fb, bytes);
-            const uint32_t kd = st + x * a.box * 128, vd = kd + C::kKV;
-            tma_load_4d(kd, &kmap, 0, w.h, off, blk, fb, pol);
-            if constexpr (!kFp8) tma_load_4d(kd + C::kKV / 2, &kmap, 64, w.h, off, blk, fb, pol);
-            tma_load_4d(vd, &vmap, 0, w.h, off, blk, fb, pol);
-            if constexpr (!kFp8) tma_load_4d(vd + C::kKV / 2, &vmap, 64, w.h, off, blk, fb, pol);
+            for (int v = 0; v < 2; ++v)
+#pragma unroll
+              for (int h = 0; h < HP; ++h) {
+                const uint32_t dst = st + v * C::kKV + h * C::kHead + x * a.box * 128;
+                tma_load_4d(dst, v ? &vmap : &kmap, 0, w.h + h, off, blk, fb, pol);
+                if constexpr (!kFp8) tma_load_4d(dst + C::kHead / 2, v ? &vmap : &kmap, 64, w.h + h, off, blk, fb, pol);
+              }
             if (kFp8 && !bad) {
               const int64_t so = blk * a.scale_stride + (int64_t)w.h * a.block_size + off;
-              bulk_load(smem_u32(&scales[s][0][x * a.box]), a.ks + so, a.box, fb);
-              bulk_load(smem_u32(&scales[s][1][x * a.box]), a.vs + so, a.box, fb);
+#pragma unroll
+              for (int h = 0; h < HP; ++h) {
+                bulk_load(smem_u32(&scales[s][0][h * kTile + x * a.box]), a.ks + so + (int64_t)h * a.block_size, a.box, fb);
+                bulk_load(smem_u32(&scales[s][1][h * kTile + x * a.box]), a.vs + so + (int64_t)h * a.block_size, a.box, fb);
+              }
             }
           }
         }
@@ -205,7 +221,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
   // Lane (g, j4): tokens g and g + 8 of the warp's sixteen and query rows
   // 8 t + 2 j4, + 1 of S^T; the same rows and the dims of dim_of() of O^T.
   const int g = lane >> 2, j4 = lane & 3, mi = lane >> 3;
-  const int tok0 = warp * 16 * KT;
+  const int hw = warp % HP, turn_of = warp / HP;  // this warp's head of the unit and place among its warps
+  const int tok0 = turn_of * 16 * KT;
   // shared-memory offsets of this lane's rows in ldmatrix: 4 pairs of chunks;
   // chunks of a bf16 row's other half and the other tokens are constants apart
   uint32_t koff[4], voff[4];
@@ -226,7 +243,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
       const int R = w.rb * kRows + t * 8 + g, node = R / a.group;
       const bool in = node < w.s.nodes;
       const bf16* qp = a.q + (int64_t)(w.s.q0 + (in ? node : 0)) * a.q_st +
-                       (int64_t)(w.h * a.group + (in ? R - node * a.group : 0)) * a.q_sh;
+                       (int64_t)((w.h + hw) * a.group + (in ? R - node * a.group : 0)) * a.q_sh;
       if constexpr (kFp8) {
         // the row over a power of two as halves: exact to 2^-25 of its largest
         // finite value, which is brought to [1, 2)
@@ -278,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
         ok = false;
         break;
       }
-      const uint32_t kb = smem_u32(smem + s * C::kStage), vb = kb + C::kKV;
+      const uint32_t kb = smem_u32(smem + s * C::kStage) + hw * C::kHead, vb = kb + C::kKV;
       const int p0 = (w.t0 + jt) * kTile + tok0;  // position of this warp's first token
       bool odd_v = false;                          // a node's V row holds a value that is not finite
       const bool tail = p0 + 16 * KT > base;
@@ -346,7 +363,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           if constexpr (kFp8) {
-            const int tk = tok0 + k * 16 + g + 8 * h;
+            const int tk = hw * kTile + tok0 + k * 16 + g + 8 * h;
             const uint32_t kc = scales[s][0][tk], vc = scales[s][1][tk];
             const float ksc = __uint_as_float(kc << 23);
             const float ev = __uint_as_float(0x4b000000u | vc) - (8388608.f + 127.f);  // vc - 127
@@ -500,89 +517,124 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT>::kCtas))
       if (lane == 0) mbar_arrive(smem_u32(&empty_bar[s]));
     }
 
-    // ------------------------------------------- join the four warps' tokens
+    // ------------------------------------------- join the warps of a head
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) l_run[t][i] += __shfl_xor_sync(0xffffffffu, l_run[t][i], d);
-        if (g == 0) {
-          mw[warp][t * 8 + 2 * j4 + i] = m_run[t][i];
-          lw[warp][t * 8 + 2 * j4 + i] = l_run[t][i];
+    if constexpr (C::kGroups == 1) {
+      // one warp holds the head: its fragments go straight to memory
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = t * 8 + 2 * j4 + i, R = w.rb * kRows + row, nd = R / a.group;
+          const float M = ok ? m_run[t][i] : -INFINITY, L = ok ? l_run[t][i] : 0.f;
+          if (nd >= w.s.nodes) continue;
+          if (w.whole()) {
+            const float inv = L == 0.f ? 0.f : 1.f / L;  // nothing seen: 0
+            bf16* op = a.out + (int64_t)(w.s.q0 + nd) * a.o_st + (int64_t)((w.h + hw) * a.group + R - nd * a.group) * a.o_sh;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<uint32_t*>(op + c * 16 + 2 * g) = pack_bf16(o[t][c][i] * inv, o[t][c][2 + i] * inv);
+          } else {
+            const int64_t pr = (((int64_t)blockIdx.x * 2 + w.slot()) * HP + hw) * kRows + row;
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+              *reinterpret_cast<float2*>(a.part_o + pr * kHD + c * 16 + 2 * g) = make_float2(o[t][c][i], o[t][c][2 + i]);
+            if (g == 0) {
+              a.part_m[pr] = M;
+              a.part_l[pr] = L;
+            }
+          }
         }
-      }
-    named_bar_sync(1, kWarps * 32);
-    float f[NT][2];
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float M = -INFINITY;
-#pragma unroll
-        for (int v = 0; v < kWarps; ++v) M = fmaxf(M, mw[v][t * 8 + 2 * j4 + i]);
-        // a warp whose tokens were all masked contributes nothing (its rows are 0)
-        f[t][i] = m_run[t][i] == -INFINITY ? 0.f : ex2(m_run[t][i] - M);
-      }
-#pragma unroll 1
-    for (int turn = 0; turn < kWarps; ++turn) {
-      if (warp == turn) {
+    } else {
+      if (g == 0) {
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              float* at = scratch + (t * 8 + 2 * j4 + i) * kScratchStride + c * 16;
-              const float v0 = o[t][c][i] * f[t][i], v1 = o[t][c][2 + i] * f[t][i];
-              if constexpr (kFp8) {
-                float2* p2 = reinterpret_cast<float2*>(at + 2 * g);
-                const float2 old = turn > 0 ? *p2 : make_float2(0.f, 0.f);
-                *p2 = make_float2(old.x + v0, old.y + v1);
-              } else {
-                at[g] = (turn > 0 ? at[g] : 0.f) + v0;
-                at[8 + g] = (turn > 0 ? at[8 + g] : 0.f) + v1;
-              }
-            }
+          for (int i = 0; i < 2; ++i) {
+            mw[warp][t * 8 + 2 * j4 + i] = m_run[t][i];
+            lw[warp][t * 8 + 2 * j4 + i] = l_run[t][i];
+          }
       }
       named_bar_sync(1, kWarps * 32);
-    }
-    constexpr int kDims = kRows;  // dims of a thread: 128 threads share kRows x 128 values
-    const int row = threadIdx.x / (kHD / kDims), d0 = threadIdx.x % (kHD / kDims) * kDims;
-    const int R = w.rb * kRows + row;
-    const int nd = R / a.group;
-    float M = -INFINITY, L = 0.f;
+      float f[NT][2];
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v) M = fmaxf(M, mw[v][row]);
+      for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int v = 0; v < kWarps; ++v) L += mw[v][row] == -INFINITY ? 0.f : ex2(mw[v][row] - M) * lw[v][row];
-    if (!ok) M = -INFINITY, L = 0.f;
-    const float* sp = scratch + row * kScratchStride + d0;
-    if (nd < w.s.nodes) {
-      if (w.whole()) {
-        const float inv = L == 0.f ? 0.f : 1.f / L;  // nothing seen: 0
-        bf16* op = a.out + (int64_t)(w.s.q0 + nd) * a.o_st + (int64_t)(w.h * a.group + R - nd * a.group) * a.o_sh + d0;
+        for (int i = 0; i < 2; ++i) {
+          float M = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < kDims / 8; ++c) {
-          uint4 y;
-          y.x = pack_bf16(sp[8 * c] * inv, sp[8 * c + 1] * inv);
-          y.y = pack_bf16(sp[8 * c + 2] * inv, sp[8 * c + 3] * inv);
-          y.z = pack_bf16(sp[8 * c + 4] * inv, sp[8 * c + 5] * inv);
-          y.w = pack_bf16(sp[8 * c + 6] * inv, sp[8 * c + 7] * inv);
-          reinterpret_cast<uint4*>(op)[c] = y;
+          for (int v = 0; v < C::kGroups; ++v) M = fmaxf(M, mw[v * HP + hw][t * 8 + 2 * j4 + i]);
+          // a warp whose tokens were all masked contributes nothing (its rows are 0)
+          f[t][i] = m_run[t][i] == -INFINITY ? 0.f : ex2(m_run[t][i] - M);
         }
-      } else {
-        const int64_t pr = ((int64_t)blockIdx.x * 2 + w.slot()) * kRows + row;
-        float4* dst = reinterpret_cast<float4*>(a.part_o + pr * kHD + d0);
+#pragma unroll 1
+      for (int turn = 0; turn < C::kGroups; ++turn) {
+        if (turn_of == turn) {
 #pragma unroll
-        for (int c = 0; c < kDims / 4; ++c) dst[c] = make_float4(sp[4 * c], sp[4 * c + 1], sp[4 * c + 2], sp[4 * c + 3]);
-        if (d0 == 0) {
-          a.part_m[pr] = M;
-          a.part_l[pr] = L;
+          for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int c = 0; c < 8; ++c)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                float* at = scratch + (hw * kRows + t * 8 + 2 * j4 + i) * kScratchStride + c * 16;
+                const float v0 = o[t][c][i] * f[t][i], v1 = o[t][c][2 + i] * f[t][i];
+                if constexpr (kFp8) {
+                  float2* p2 = reinterpret_cast<float2*>(at + 2 * g);
+                  const float2 old = turn > 0 ? *p2 : make_float2(0.f, 0.f);
+                  *p2 = make_float2(old.x + v0, old.y + v1);
+                } else {
+                  at[g] = (turn > 0 ? at[g] : 0.f) + v0;
+                  at[8 + g] = (turn > 0 ? at[8 + g] : 0.f) + v1;
+                }
+              }
+        }
+        named_bar_sync(1, kWarps * 32);
+      }
+      constexpr int kDims = HP * kRows;  // dims of a thread: 128 threads share HP x kRows x 128 values
+      const int hrow = threadIdx.x / (kHD / kDims), d0 = threadIdx.x % (kHD / kDims) * kDims;
+      const int hh = hrow / kRows, row = hrow - hh * kRows;
+      const int R = w.rb * kRows + row;
+      const int nd = R / a.group;
+      float M = -INFINITY, L = 0.f;
+#pragma unroll
+      for (int v = 0; v < C::kGroups; ++v) M = fmaxf(M, mw[v * HP + hh][row]);
+#pragma unroll
+      for (int v = 0; v < C::kGroups; ++v)
+        L += mw[v * HP + hh][row] == -INFINITY ? 0.f : ex2(mw[v * HP + hh][row] - M) * lw[v * HP + hh][row];
+      if (!ok) M = -INFINITY, L = 0.f;
+      const float* sp = scratch + hrow * kScratchStride + d0;
+      if (nd < w.s.nodes) {
+        if (w.whole()) {
+          const float inv = L == 0.f ? 0.f : 1.f / L;  // nothing seen: 0
+          bf16* op =
+              a.out + (int64_t)(w.s.q0 + nd) * a.o_st + (int64_t)((w.h + hh) * a.group + R - nd * a.group) * a.o_sh + d0;
+#pragma unroll
+          for (int c = 0; c < kDims / 8; ++c) {
+            uint4 y;
+            y.x = pack_bf16(sp[8 * c] * inv, sp[8 * c + 1] * inv);
+            y.y = pack_bf16(sp[8 * c + 2] * inv, sp[8 * c + 3] * inv);
+            y.z = pack_bf16(sp[8 * c + 4] * inv, sp[8 * c + 5] * inv);
+            y.w = pack_bf16(sp[8 * c + 6] * inv, sp[8 * c + 7] * inv);
+            reinterpret_cast<uint4*>(op)[c] = y;
+          }
+        } else {
+          const int64_t pr = (((int64_t)blockIdx.x * 2 + w.slot()) * HP + hh) * kRows + row;
+          float4* dst = reinterpret_cast<float4*>(a.part_o + pr * kHD + d0);
+#pragma unroll
+          for (int c = 0; c < kDims / 4; ++c) dst[c] = make_float4(sp[4 * c], sp[4 * c + 1], sp[4 * c + 2], sp[4 * c + 3]);
+          if (d0 == 0) {
+            a.part_m[pr] = M;
+            a.part_l[pr] = L;
+          }
         }
       }
+      named_bar_sync(1, kWarps * 32);  // scratch and statistics are free again
     }
-    named_bar_sync(1, kWarps * 32);  // scratch and statistics are free again
   }
 }
 
@@ -623,7 +675,7 @@ __device__ __forceinline__ Joined join_parts(const Args& a, int c0, int n, int k
       o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (kk < n) {
         // the unit's first part holds its beginning (slot 1), the others follow on (slot 0)
-        const int64_t pr = ((int64_t)(c0 + kk) * 2 + (kk == 0)) * a.rows + row;
+        const int64_t pr = ((int64_t)(c0 + kk) * 2 + (kk == 0)) * a.heads * a.rows + row;
         m[u] = a.part_m[pr];
         l[u] = a.part_l[pr];
         o[u] = *reinterpret_cast<const float4*>(a.part_o + pr * kHD + lane * 4);
@@ -654,8 +706,9 @@ __global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __gr
         return;
       }
       const int R = nd * a.group + head - h * a.group, rb = R / a.rows;
-      row = R - rb * a.rows;
-      const int64_t lo = first + ((int64_t)h * s.blocks + rb) * s.tiles;
+      const int hg = h / a.heads;
+      row = (h - hg * a.heads) * a.rows + R - rb * a.rows;
+      const int64_t lo = first + ((int64_t)hg * s.blocks + rb) * s.tiles;
       const int64_t hi = lo + s.tiles - 1;
       if (hi <= UINT32_MAX) {  // nearly always: a 64-bit division takes ten times as long
         c0 = (int)((uint32_t)lo / (uint32_t)range);
@@ -714,22 +767,51 @@ int encode_pages(CUtensorMap* map, const void* base, bool fp8, int64_t num_block
   return kOk;
 }
 
-size_t workspace_bytes(int parts, int rows, int batch) {
-  return (size_t)parts * 2 * rows * (kHD + 2) * sizeof(float) + ((size_t)batch + 2) * sizeof(int64_t);
+// The kernel variant of a call, and what its launch needs.
+struct Variant {
+  int nt, heads, tile, box, parts;
+  size_t workspace;
+};
+
+template <bool kFp8, int NT, int HP>
+void fill(Variant* v) {
+  using C = Cfg<kFp8, NT, HP>;
+  v->nt = NT;
+  v->heads = HP;
+  v->tile = C::kTile;
+  v->parts = C::kCtas * device_sm_count();  // what the SMs hold: one wave
 }
 
-template <bool kFp8, int NT>
+Variant variant_for(bool fp8, int batch, int hq, int hkv, int max_nodes, int block_size) {
+  Variant v;
+  const bool few = (int64_t)(hq / hkv) * max_nodes <= 8;
+  const int hp = !fp8 ? 1 : hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;
+  if (!fp8)
+    few ? fill<false, 1, 1>(&v) : fill<false, 2, 1>(&v);
+  else if (hp == 4)
+    few ? fill<true, 1, 4>(&v) : fill<true, 2, 4>(&v);
+  else if (hp == 2)
+    few ? fill<true, 1, 2>(&v) : fill<true, 2, 2>(&v);
+  else
+    few ? fill<true, 1, 1>(&v) : fill<true, 2, 1>(&v);
+  v.box = block_size % v.tile == 0 ? v.tile : 64;
+  v.workspace = (size_t)v.parts * 2 * v.heads * v.nt * 8 * (kHD + 2) * sizeof(float) + ((size_t)batch + 2) * sizeof(int64_t);
+  return v;
+}
+
+template <bool kFp8, int NT, int HP>
 int launch_warp(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, cudaStream_t st) {
   static std::atomic<unsigned long long> done{0};
+  constexpr int kSmem = Cfg<kFp8, NT, HP>::kSmem;
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_status(e, "kvb_tree_attn: cudaGetDevice");
   if (dev >= 64 || !((done.load() >> dev) & 1ull)) {
-    e = cudaFuncSetAttribute(tree_warp_kernel<kFp8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (Cfg<kFp8, NT>::kSmem));
+    e = cudaFuncSetAttribute(tree_warp_kernel<kFp8, NT, HP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e != cudaSuccess) return cuda_status(e, "kvb_tree_attn: shared memory attribute");
     if (dev < 64) done.fetch_or(1ull << dev);
   }
-  e = launch_kernel(tree_warp_kernel<kFp8, NT>, dim3(a.parts), dim3(kThreads), (Cfg<kFp8, NT>::kSmem), st, km, vm, a);
+  e = launch_kernel(tree_warp_kernel<kFp8, NT, HP>, dim3(a.parts), dim3(kThreads), kSmem, st, km, vm, a);
   return cuda_status(e, "kvb_tree_attn launch");
 }
 
@@ -743,7 +825,10 @@ extern "C" int kvb_tree_attn_workspace_size(int batch, int num_q_heads, int num_
   if (!bytes) return set_error(kInvalid, "kvb_tree_attn_workspace_size: bytes is NULL");
   if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_seqlen_q < 0)
     return set_error(kInvalid, "kvb_tree_attn_workspace_size: bad sizes");
-  *bytes = workspace_bytes(4 * device_sm_count(), 16, batch);
+  // the larger of the two cache types' needs (the block size does not matter)
+  const size_t a = variant_for(false, batch, num_q_heads, num_kv_heads, max_seqlen_q, 256).workspace;
+  const size_t b = variant_for(true, batch, num_q_heads, num_kv_heads, max_seqlen_q, 256).workspace;
+  *bytes = a > b ? a : b;
   return kOk;
 }
 
@@ -784,14 +869,13 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   if (!(scale > 0.f) || scale > 1e30f) return set_error(kInvalid, "kvb_tree_attn: scale must be positive and finite");
 
   Args a = {};
-  const int group = num_q_heads / num_kv_heads;
-  a.rows = (int64_t)group * max_seqlen_q <= 8 ? 8 : 16;
-  a.tile = fp8 ? Cfg<true, 1>::kTile : Cfg<false, 1>::kTile;
-  a.box = block_size % a.tile == 0 ? a.tile : 64;
-  // what the SMs hold: one wave
-  a.parts = device_sm_count() * (a.rows == 8 ? (fp8 ? Cfg<true, 1>::kCtas : Cfg<false, 1>::kCtas)
-                                             : (fp8 ? Cfg<true, 2>::kCtas : Cfg<false, 2>::kCtas));
-  const size_t need = workspace_bytes(a.parts, a.rows, batch);
+  const Variant v = variant_for(fp8, batch, num_q_heads, num_kv_heads, max_seqlen_q, block_size);
+  a.rows = v.nt * 8;
+  a.heads = v.heads;
+  a.tile = v.tile;
+  a.box = v.box;
+  a.parts = v.parts;
+  const size_t need = v.workspace;
   if (!workspace || workspace_bytes_given < need)
     return set_error(kWorkspace, "kvb_tree_attn: workspace of %zu bytes needed, %zu given", need,
                      workspace ? workspace_bytes_given : (size_t)0);
@@ -817,13 +901,13 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   a.batch = batch;
   a.hq = num_q_heads;
   a.hkv = num_kv_heads;
-  a.group = group;
+  a.group = num_q_heads / num_kv_heads;
   a.num_blocks = (int)num_blocks;
   a.block_size = block_size;
   a.first = (int64_t*)workspace;
-  a.part_o = (float*)workspace + (((size_t)batch + 1) * 2 + 3) / 4 * 4;
-  a.part_m = a.part_o + (size_t)a.parts * 2 * a.rows * kHD;
-  a.part_l = a.part_m + (size_t)a.parts * 2 * a.rows;
+  a.part_o = (float*)workspace + (((size_t)batch + 1) * 2 + 3) / 4 * 4;  // 16-byte aligned behind the prefix sums
+  a.part_m = a.part_o + (size_t)a.parts * 2 * a.heads * a.rows * kHD;
+  a.part_l = a.part_m + (size_t)a.parts * 2 * a.heads * a.rows;
   a.scale_log2 = scale * 1.4426950408889634f;
 
   CUtensorMap km, vm;
@@ -831,9 +915,15 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   int rc = encode_pages(&km, k_cache, fp8, num_blocks, bytes, block_size, num_kv_heads, a.box);
   if (!rc) rc = encode_pages(&vm, v_cache, fp8, num_blocks, bytes, block_size, num_kv_heads, a.box);
   const cudaStream_t st = (cudaStream_t)stream;
-  if (!rc)
-    rc = a.rows == 8 ? (fp8 ? launch_warp<true, 1>(km, vm, a, st) : launch_warp<false, 1>(km, vm, a, st))
-                     : (fp8 ? launch_warp<true, 2>(km, vm, a, st) : launch_warp<false, 2>(km, vm, a, st));
+  if (rc) return rc;
+  if (!fp8)
+    rc = v.nt == 1 ? launch_warp<false, 1, 1>(km, vm, a, st) : launch_warp<false, 2, 1>(km, vm, a, st);
+  else if (v.heads == 4)
+    rc = v.nt == 1 ? launch_warp<true, 1, 4>(km, vm, a, st) : launch_warp<true, 2, 4>(km, vm, a, st);
+  else if (v.heads == 2)
+    rc = v.nt == 1 ? launch_warp<true, 1, 2>(km, vm, a, st) : launch_warp<true, 2, 2>(km, vm, a, st);
+  else
+    rc = v.nt == 1 ? launch_warp<true, 1, 1>(km, vm, a, st) : launch_warp<true, 2, 1>(km, vm, a, st);
   if (rc) return rc;
   // rows of many partials come with few rows in all: a block each then
   const int64_t mrows = (int64_t)max_seqlen_q * num_q_heads;

@@ -1,8 +1,8 @@
 // Work partition shared by the tree-attention kernels and their merge.
 //
-// A unit is one (sequence, kv head, block of query rows): it walks the
-// sequence's context in tiles of tokens. The tiles of all units, in the order
-// sequence > kv head > row block, form one line that is cut into ranges of
+// A unit is one (sequence, group of kv heads, block of query rows of each): it
+// walks the sequence's context in tiles of tokens. The tiles of all units, in the
+// order sequence > head group > row block, form one line that is cut into ranges of
 // equal length, one per CTA (at most `parts`): every CTA streams the same number
 // of K/V bytes whatever the lengths of the sequences are, and the host needs
 // none of the device's lengths. A unit cut between CTAs leaves fp32
@@ -37,10 +37,11 @@ struct Args {
   int64_t scale_stride;  // bytes between blocks of the scale arrays
   int batch, hq, hkv, group;
   int num_blocks, block_size;
-  int parts, rows, tile;  // CTAs of the attention grid, query rows of a unit, tokens of a tile
+  int heads;              // kv heads of a unit
+  int parts, rows, tile;  // CTAs of the attention grid, query rows of a unit and head, tokens of a tile
   int box;                // tokens of a TMA box: a tile's, or a page's when that is smaller
-  float* part_o;          // [parts][2][rows][128]
-  float* part_m;          // [parts][2][rows]
+  float* part_o;          // [parts][2][heads][rows][128]
+  float* part_m;          // [parts][2][heads][rows]
   float* part_l;
   int64_t* first;         // [batch + 1]: tiles before each sequence, written for the merge
   float scale_log2;
@@ -74,7 +75,7 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int b, bool report) {
   s.blocks = (int)(((int64_t)s.nodes * a.group + a.rows - 1) / a.rows);
   return s;
 }
-__device__ __forceinline__ int64_t cost_of(const Args& a, const Seq& s) { return (int64_t)s.tiles * s.blocks * a.hkv; }
+__device__ __forceinline__ int64_t cost_of(const Args& a, const Seq& s) { return (int64_t)s.tiles * s.blocks * (a.hkv / a.heads); }
 
 // Exclusive prefix of each thread's sum over the block, and the total.
 template <int kThreads>
@@ -139,7 +140,7 @@ struct Walk {
   int b;
   int64_t off, left;
   Seq s;
-  int h, rb, t0, n;  // kv head, row block, first tile, tiles
+  int h, rb, t0, n;  // first kv head, row block, first tile, tiles
 
   __device__ __forceinline__ Walk(const Args& a, const Start& st) : b(st.b), off(st.off), left(st.left) {
     if (left > 0) s = seq_of(a, b, false);
@@ -153,8 +154,9 @@ struct Walk {
     }
     const int64_t u = off / s.tiles;
     t0 = (int)(off - u * s.tiles);
-    h = (int)(u / s.blocks);
-    rb = (int)(u - (int64_t)h * s.blocks);
+    const int hg = (int)(u / s.blocks);
+    h = hg * a.heads;
+    rb = (int)(u - (int64_t)hg * s.blocks);
     const int64_t room = s.tiles - t0;
     n = (int)(left < room ? left : room);
     off += n;
