@@ -20,6 +20,7 @@
 
 KVB_DEFINE_ERROR_WORD(tree)
 
+#include "tcgen05.cuh"
 #include "tree_plan.cuh"
 
 namespace kvb {
@@ -76,6 +77,16 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar)
                : "memory");
+}
+
+// A load without the evict-first hint, for rows that are read again soon.
+__device__ __forceinline__ void tma_load_4d_keep(uint32_t dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                                 uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
+      "[%6];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(bar)
+      : "memory");
 }
 
 // Adds bytes to the transactions the barrier's current phase waits for.
@@ -605,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
       for (int v = 0; v < C::kGroups; ++v) M = fmaxf(M, mw[v * HP + hh][row]);
 #pragma unroll
       for (int v = 0; v < C::kGroups; ++v)
-        L += mw[v * HP + hh][row] == -INFINITY ? 0.f : ex2(mw[v * HP + hh][row] - M) * lw[v * HP + hh][row];
+        L += (mw[v * HP + hh][row] == -INFINITY ? 0.f : ex2(mw[v * HP + hh][row] - M)) * lw[v * HP + hh][row];  // keeps NaN
       if (!ok) M = -INFINITY, L = 0.f;
       const float* sp = scratch + hrow * kScratchStride + d0;
       if (nd < w.s.nodes) {
@@ -637,6 +648,14 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
     }
   }
 }
+
+}  // namespace
+}  // namespace kvb
+
+#include "tree_attn_tc.cuh"
+
+namespace kvb {
+namespace {
 
 // ------------------------------------------------------------------- merge
 // Joins the partials of units that were cut between CTAs, in an order that does
@@ -769,7 +788,8 @@ int encode_pages(CUtensorMap* map, const void* base, bool fp8, int64_t num_block
 
 // The kernel variant of a call, and what its launch needs.
 struct Variant {
-  int nt, heads, tile, box, parts;
+  int nt;  // eights of query rows a unit holds for the warp-MMA kernel; 0: the tcgen05 kernel
+  int rows, heads, tile, box, parts;
   size_t workspace;
 };
 
@@ -777,6 +797,7 @@ template <bool kFp8, int NT, int HP>
 void fill(Variant* v) {
   using C = Cfg<kFp8, NT, HP>;
   v->nt = NT;
+  v->rows = C::kRows;
   v->heads = HP;
   v->tile = C::kTile;
   v->parts = C::kCtas * device_sm_count();  // what the SMs hold: one wave
@@ -784,9 +805,16 @@ void fill(Variant* v) {
 
 Variant variant_for(bool fp8, int batch, int hq, int hkv, int max_nodes, int block_size) {
   Variant v;
-  const bool few = (int64_t)(hq / hkv) * max_nodes <= 8;
+  const int64_t rows = (int64_t)(hq / hkv) * max_nodes;
+  const bool few = rows <= 8;
   const int hp = !fp8 ? 1 : hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;
-  if (!fp8)
+  if (rows > 16) {
+    v.nt = 0;
+    v.rows = tcore::kRows;
+    v.heads = 1;
+    v.tile = tcore::kTile;
+    v.parts = device_sm_count();
+  } else if (!fp8)
     few ? fill<false, 1, 1>(&v) : fill<false, 2, 1>(&v);
   else if (hp == 4)
     few ? fill<true, 1, 4>(&v) : fill<true, 2, 4>(&v);
@@ -795,8 +823,24 @@ Variant variant_for(bool fp8, int batch, int hq, int hkv, int max_nodes, int blo
   else
     few ? fill<true, 1, 1>(&v) : fill<true, 2, 1>(&v);
   v.box = block_size % v.tile == 0 ? v.tile : 64;
-  v.workspace = (size_t)v.parts * 2 * v.heads * v.nt * 8 * (kHD + 2) * sizeof(float) + ((size_t)batch + 2) * sizeof(int64_t);
+  v.workspace = (size_t)v.parts * 2 * v.heads * v.rows * (kHD + 2) * sizeof(float) + ((size_t)batch + 2) * sizeof(int64_t);
   return v;
+}
+
+template <bool kFp8>
+int launch_tc(const CUtensorMap& km, const CUtensorMap& vm, const Args& a, cudaStream_t st) {
+  static std::atomic<unsigned long long> done{0};
+  constexpr int kSmem = tcore::Cfg<kFp8>::kSmem;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e, "kvb_tree_attn: cudaGetDevice");
+  if (dev >= 64 || !((done.load() >> dev) & 1ull)) {
+    e = cudaFuncSetAttribute(tcore::tree_tc_kernel<kFp8>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e != cudaSuccess) return cuda_status(e, "kvb_tree_attn: shared memory attribute");
+    if (dev < 64) done.fetch_or(1ull << dev);
+  }
+  e = launch_kernel(tcore::tree_tc_kernel<kFp8>, dim3(a.parts), dim3(tcore::kThreads), kSmem, st, km, vm, a);
+  return cuda_status(e, "kvb_tree_attn launch");
 }
 
 template <bool kFp8, int NT, int HP>
@@ -870,7 +914,7 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
 
   Args a = {};
   const Variant v = variant_for(fp8, batch, num_q_heads, num_kv_heads, max_seqlen_q, block_size);
-  a.rows = v.nt * 8;
+  a.rows = v.rows;
   a.heads = v.heads;
   a.tile = v.tile;
   a.box = v.box;
@@ -916,7 +960,9 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   if (!rc) rc = encode_pages(&vm, v_cache, fp8, num_blocks, bytes, block_size, num_kv_heads, a.box);
   const cudaStream_t st = (cudaStream_t)stream;
   if (rc) return rc;
-  if (!fp8)
+  if (v.nt == 0)
+    rc = fp8 ? launch_tc<true>(km, vm, a, st) : launch_tc<false>(km, vm, a, st);
+  else if (!fp8)
     rc = v.nt == 1 ? launch_warp<false, 1, 1>(km, vm, a, st) : launch_warp<false, 2, 1>(km, vm, a, st);
   else if (v.heads == 4)
     rc = v.nt == 1 ? launch_warp<true, 1, 4>(km, vm, a, st) : launch_warp<true, 2, 4>(km, vm, a, st);
