@@ -4,19 +4,22 @@
 // A CTA owns 128 query rows (nodes x query heads of one kv head) and walks the
 // context in 128-token tiles: S = Q K^T is a tcgen05.mma chain into TMEM, two
 // softmax warpgroups take the tiles in turn (one thread per query row, so no
-// reduction crosses threads), write the weights P to shared memory and fold
-// P V, a second tcgen05.mma chain, into their own fp32 rows. The two groups keep
-// separate maxima and sums, which are joined at the end of a segment, so one
-// group's exponentials overlap the other group's MMAs. One warp issues the TMA
-// loads, one thread the MMAs.
+// reduction crosses threads) and put the weights P back over S in TMEM, from where
+// a second chain adds P V to the group's output rows, also in TMEM. The two groups
+// keep separate references and sums, which are joined at the end of a segment, so
+// one group's exponentials overlap the other group's MMAs. A row's reference moves
+// only when its maximum has passed it by 2^8: weights of up to 2^8 cost nothing in
+// bf16 or half, and the output rows are rescaled once or twice in a context instead
+// of at every tile. One warp issues the TMA loads, one thread the MMAs.
 //
-// Over an e4m3 cache the operands stay e4m3: Q and P are split in two e4m3 parts,
-// x = hi + lo, hi = e4m3(x), lo = e4m3(x - hi). Two 4-bit significands with the
-// lower one signed hold a bf16 query exactly (its 8 bits) down to 2^-10 of the
-// row's maximum, scaled to [128, 256), and 2^-18 of that maximum below it; a weight
-// scaled by 2^8 likewise, so its error is at most 2^-9 of itself or 2^-18 of the
-// row's largest. Two e4m3 chains take as long as one bf16 chain, K and V are never
-// converted, and their tiles are half as large.
+// Over an e4m3 cache K stays e4m3: Q is split in two e4m3 parts, x = hi + lo, hi =
+// e4m3(x), lo = e4m3(x - hi), which hold a bf16 value (8 bits, two signed 4-bit
+// significands) exactly down to 2^-10 of its row's maximum, scaled to [128, 256),
+// and to 2^-18 of that maximum below it. Two e4m3 chains take as long as one
+// 16-bit chain and K is never converted. The weights need more range than e4m3
+// has (2^-18 of the largest would be lost, and 10^5 tokens can hold a fifth of
+// the sum below that), so they are halves, and two more warps turn V into
+// halves, exactly.
 #pragma once
 
 namespace kvb {
@@ -26,21 +29,22 @@ namespace tcore {
 constexpr int kRows = 128;
 constexpr int kTile = 128;
 constexpr int kGroups = 2;                                // softmax warpgroups
-constexpr int kThreads = 128 + kGroups * 128;             // warp 0 TMA, warp 1 MMA + TMEM, warps 2 and 3 idle
+constexpr int kThreads = 128 + kGroups * 128;             // warp 0 TMA, 1 MMA + TMEM, 2 and 3 convert V
 // Registers: 168 a thread at launch (384 threads); the control warps give theirs
 // up for the softmax threads' output rows: 128 (56 + 2 * 224) = 384 * 168.
 constexpr int kControlRegs = 56, kSoftmaxRegs = 224;
-constexpr uint32_t kCols = 512;                           // S0, S1, PV0, PV1 (128 columns each)
-constexpr int kOperand = kRows * kHD * 2;                 // Q or P: bf16, or two e4m3 parts
-constexpr int kPart = kOperand / 2;                       // an e4m3 part, or 64 columns of bf16
+constexpr uint32_t kCols = 512;                           // S0, S1 (then P0, P1), O0, O1: 128 columns each
+constexpr float kSlack = 8.f;                             // log2 of the largest weight
+constexpr int kHalf = kTile * 128;                        // 128 rows of 128 bytes
+constexpr int kOperand = 2 * kHalf;                       // 16-bit Q or V (two halves of 64 dims), or two e4m3 parts of Q
 template <bool kFp8>
 struct Cfg {
   static constexpr int kKV = kTile * kHD * (kFp8 ? 1 : 2);
-  static constexpr int kStage = 2 * kKV;
-  static constexpr int kStages = kFp8 ? 3 : 2;
-  static constexpr int kQ = 0, kP = kOperand, kRing = (1 + kGroups) * kOperand;
-  static constexpr int kSmem = kRing + kStages * kStage + 1024;
+  static constexpr int kStages = 3;
+  static constexpr int kQ = 0, kV16 = kOperand, kRing = kOperand + (kFp8 ? 2 * kOperand : 0);
+  static constexpr int kSmem = kRing + kStages * 2 * kKV + 1024;
 };
+
 // K-major operand rows of 128 bytes, 128-byte swizzle: 8-row groups 1024 B apart.
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr) {
   return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
@@ -66,6 +70,13 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
         "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
+// D (+)= P V with the 16-bit P in TMEM (two values a column, a row a lane).
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc));
+}
 __device__ __forceinline__ void commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
@@ -80,11 +91,82 @@ __device__ __forceinline__ bool any_of_barrier(int id, int threads, bool x) {
       : "memory");
   return r != 0;
 }
-__device__ __forceinline__ float tmem_ld1(uint32_t taddr) {
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
   uint32_t r;
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(r) : "r"(taddr));
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-  return __uint_as_float(r);
+  return r;
+}
+// 32 columns of this thread's lane into r[kAt..], without waiting; ready after landed().
+template <int kAt>
+__device__ __forceinline__ void tmem_get(uint32_t taddr, float (&v)[128]) {
+  float* r = v + kAt;
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(taddr));
+}
+template <int kAt>
+__device__ __forceinline__ void pin(float (&v)[128]) {  // no use of the registers moves before this
+  float* r = v + kAt;
+  asm volatile(""
+               : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
+                 "+f"(r[9]), "+f"(r[10]), "+f"(r[11]), "+f"(r[12]), "+f"(r[13]), "+f"(r[14]), "+f"(r[15]), "+f"(r[16]),
+                 "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]),
+                 "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31]));
+}
+// A row's 128 columns.
+__device__ __forceinline__ void tmem_row(uint32_t taddr, float (&v)[128]) {
+  tmem_get<0>(taddr, v);
+  tmem_get<32>(taddr + 32, v);
+  tmem_get<64>(taddr + 64, v);
+  tmem_get<96>(taddr + 96, v);
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+  pin<0>(v);
+  pin<32>(v);
+  pin<64>(v);
+  pin<96>(v);
+}
+__device__ __forceinline__ void tmem_put_row(uint32_t taddr, const float (&v)[128]) {
+#pragma unroll
+  for (int c = 0; c < 4; ++c) tc::tmem_st32(taddr + c * 32, v + c * 32);
+}
+// 16 columns of this thread's lane.
+__device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// Packed fp32 pairs.
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void un2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
@@ -142,11 +224,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<kFp8>;
   kernel_entry();
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full, kfull[C::kStages], vfull[C::kStages], kv_empty[C::kStages], s_full[2], s_empty[2],
-      p_full[2], pv_full[2], pv_empty[2];
+  __shared__ __align__(8) uint64_t q_full, kfull[C::kStages], vfull[C::kStages], k_empty[C::kStages], v_empty[C::kStages],
+      v16_full[2], v16_empty[2], s_full[2], p_full[2], pv_full[2], o_empty[2];
   __shared__ __align__(16) uint8_t scales[kFp8 ? C::kStages : 1][2][kTile];
-  // a tile's scales 2^a (K) and 2^b (V) as floats: 2^a, b and 2^-b
-  __shared__ __align__(16) float tok_k[kFp8 ? 2 : 1][kTile], tok_b[kFp8 ? 2 : 1][kTile], tok_i[kFp8 ? 2 : 1][kTile];
+  // scales 2^a (K) and 2^b (V) of a tile as floats: 2^a, b and 2^-b; two tiles of each group
+  __shared__ __align__(16) float tok_k[kFp8 ? 4 : 1][kTile], tok_b[kFp8 ? 4 : 1][kTile], tok_i[kFp8 ? 4 : 1][kTile];
   __shared__ float m_other[kRows], l_other[kRows];
   __shared__ uint32_t odd_bits[2][4];
   __shared__ uint32_t tmem_s;
@@ -159,14 +241,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(smem_u32(&kfull[i]), 1);
       mbar_init(smem_u32(&vfull[i]), 1);
-      mbar_init(smem_u32(&kv_empty[i]), 1);
+      mbar_init(smem_u32(&k_empty[i]), kFp8 ? 5 : 1);  // the MMAs; the four warps that read the tile's scales
+      mbar_init(smem_u32(&v_empty[i]), kFp8 ? 2 : 1);  // the converting warps, or the MMAs
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&v16_full[i]), 2);
+      mbar_init(smem_u32(&v16_empty[i]), 1);
       mbar_init(smem_u32(&s_full[i]), 1);
-      mbar_init(smem_u32(&s_empty[i]), 4);
       mbar_init(smem_u32(&p_full[i]), 4);
       mbar_init(smem_u32(&pv_full[i]), 1);
-      mbar_init(smem_u32(&pv_empty[i]), 4);
+      mbar_init(smem_u32(&o_empty[i]), 4);
     }
     fence_barrier_init();
   }
@@ -180,143 +264,193 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc::fence_after();
   const uint32_t tmem = tmem_s;
   Walk w(a, start);
+  // Tile i of the CTA: stage i % kStages of the rings (use i / kStages of it),
+  // V buffer i & 1 (use i / 2); tile j of a segment belongs to group j & 1.
+  const auto stage_of = [](uint32_t i) { return i % C::kStages; };
+  const auto phase_of = [](uint32_t i) { return (i / C::kStages) & 1; };
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
     if (warp == 0) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0) {
-      prefetch_tensormap(&kmap);
-      prefetch_tensormap(&vmap);
-      const uint64_t pol = l2_evict_first_policy();
-      uint32_t it = 0;
-      bool ok = true;
-      while (ok && w.next(a)) {
-        // several row blocks read the same rows: keep those in L2
-        const bool once = w.s.blocks == 1;
-        int col = -1, blk = 0;
-        bool bad = false;
-        for (int j = 0; j < w.n; ++j, ++it) {
-          const int st = it % C::kStages;
-          if (it >= C::kStages && !mbar_wait(smem_u32(&kv_empty[st]), (it / C::kStages - 1) & 1, &g_err_tree)) {
-            ok = false;
-            break;
-          }
-          const int t0 = (w.t0 + j) * kTile;
-          const uint32_t kd = sbase + C::kRing + st * C::kStage, vd = kd + C::kKV;
-          const uint32_t kb = smem_u32(&kfull[st]), vb = smem_u32(&vfull[st]);
-          const int boxes = kTile / a.box;
-          for (int x = 0; x < boxes; ++x) {
-            const int at = t0 + x * a.box;
-            if (at / a.block_size != col) {
-              col = at / a.block_size;
-              const bool past = at >= w.s.len;
-              blk = past ? -1 : a.tables[(int64_t)w.b * a.bt_stride + col];
-              bad = blk < 0 || blk >= a.num_blocks;
-              if (bad) {
-                if (!past) atomicOr(&g_err_tree, (unsigned)kErrBlockTable);
-                blk = a.num_blocks;  // out of the tensor map: TMA fills zeros
+      // ---------------------------------------------------------- TMA producer
+      if (lane == 0) {
+        prefetch_tensormap(&kmap);
+        prefetch_tensormap(&vmap);
+        const uint64_t pol = l2_evict_first_policy();
+        uint32_t it = 0;
+        bool ok = true;
+        while (ok && w.next(a)) {
+          const bool once = w.s.blocks == 1;  // else several row blocks read the same rows: keep those in L2
+          int col = -1, blk = 0;
+          bool bad = false;
+          for (int j = 0; j < w.n && ok; ++j, ++it) {
+            const uint32_t st = stage_of(it);
+            const int t0 = (w.t0 + j) * kTile, boxes = kTile / a.box;
+            const uint32_t kd = sbase + C::kRing + st * 2 * C::kKV, vd = kd + C::kKV;
+            const uint32_t kb = smem_u32(&kfull[st]), vb = smem_u32(&vfull[st]);
+            if (it >= C::kStages) ok = mbar_wait(smem_u32(&k_empty[st]), phase_of(it - C::kStages), &g_err_tree);
+            if (!ok) break;
+            int bcol[2], bblk[2];
+            for (int x = 0; x < boxes; ++x) {
+              const int at = t0 + x * a.box;
+              if (at / a.block_size != col) {
+                col = at / a.block_size;
+                const bool past = at >= w.s.len;
+                blk = past ? -1 : a.tables[(int64_t)w.b * a.bt_stride + col];
+                bad = blk < 0 || blk >= a.num_blocks;
+                if (bad) {
+                  if (!past) atomicOr(&g_err_tree, (unsigned)kErrBlockTable);
+                  blk = a.num_blocks;  // out of the tensor map: TMA fills zeros
+                }
               }
-            }
-            const int off = at - col * a.block_size;
-            if (kFp8 && bad) {  // a block outside the pool reads zeros, of scale 1
-              for (int i = 0; i < 2; ++i)
-                for (int k = 0; k < a.box / 4; ++k)
-                  reinterpret_cast<uint32_t*>(&scales[st][i][x * a.box])[k] = 0x7f7f7f7fu;
-              fence_async();  // before a later copy into the same bytes
-            }
-            const uint32_t bytes = C::kKV / boxes;
-            const uint32_t more = kFp8 && !bad ? 2 * a.box : 0;  // the scales come with K
-            if (x + 1 < boxes) {
-              mbar_expect_tx(kb, bytes + more);
-              mbar_expect_tx(vb, bytes);
-            } else {
-              mbar_arrive_expect_tx(kb, bytes + more);
-              mbar_arrive_expect_tx(vb, bytes);
-            }
-            if (kFp8 && !bad) {
-              const int64_t so = blk * a.scale_stride + (int64_t)w.h * a.block_size + off;
-              bulk_load(smem_u32(&scales[st][0][x * a.box]), a.ks + so, a.box, kb);
-              bulk_load(smem_u32(&scales[st][1][x * a.box]), a.vs + so, a.box, kb);
-            }
-#pragma unroll
-            for (int v = 0; v < 2; ++v)
+              bcol[x] = at - col * a.block_size;
+              bblk[x] = blk;
+              if (kFp8 && bad) {  // a block outside the pool reads zeros, of scale 1
+                for (int i = 0; i < 2; ++i)
+                  for (int k = 0; k < a.box / 4; ++k)
+                    reinterpret_cast<uint32_t*>(&scales[st][i][x * a.box])[k] = 0x7f7f7f7fu;
+                fence_async();  // before a later copy into the same bytes
+              }
+              const uint32_t bytes = C::kKV / boxes + (kFp8 && !bad ? 2 * a.box : 0);  // the scales come with K
+              if (x + 1 < boxes)
+                mbar_expect_tx(kb, bytes);
+              else
+                mbar_arrive_expect_tx(kb, bytes);
+              if (kFp8 && !bad) {
+                const int64_t so = blk * a.scale_stride + (int64_t)w.h * a.block_size + bcol[x];
+                bulk_load(smem_u32(&scales[st][0][x * a.box]), a.ks + so, a.box, kb);
+                bulk_load(smem_u32(&scales[st][1][x * a.box]), a.vs + so, a.box, kb);
+              }
 #pragma unroll
               for (int hf = 0; hf < (kFp8 ? 1 : 2); ++hf) {
-                const uint32_t dst = (v ? vd : kd) + hf * kPart + x * a.box * 128;
                 if (once)
-                  tma_load_4d(dst, v ? &vmap : &kmap, hf * 64, w.h, off, blk, v ? vb : kb, pol);
+                  tma_load_4d(kd + hf * kHalf + x * a.box * 128, &kmap, hf * 64, w.h, bcol[x], blk, kb, pol);
                 else
-                  tma_load_4d_keep(dst, v ? &vmap : &kmap, hf * 64, w.h, off, blk, v ? vb : kb);
+                  tma_load_4d_keep(kd + hf * kHalf + x * a.box * 128, &kmap, hf * 64, w.h, bcol[x], blk, kb);
+              }
+            }
+            if (it >= C::kStages) ok = mbar_wait(smem_u32(&v_empty[st]), phase_of(it - C::kStages), &g_err_tree);
+            if (!ok) {
+              mbar_wait(kb, phase_of(it), &g_err_tree);  // this tile's K copies
+              break;
+            }
+            mbar_arrive_expect_tx(vb, C::kKV);
+            for (int x = 0; x < boxes; ++x)
+#pragma unroll
+              for (int hf = 0; hf < (kFp8 ? 1 : 2); ++hf) {
+                if (once)
+                  tma_load_4d(vd + hf * kHalf + x * a.box * 128, &vmap, hf * 64, w.h, bcol[x], bblk[x], vb, pol);
+                else
+                  tma_load_4d_keep(vd + hf * kHalf + x * a.box * 128, &vmap, hf * 64, w.h, bcol[x], bblk[x], vb);
               }
           }
         }
-      }
-      // no copy may outlive the CTA: wait (bounded) for the last phase of every stage
-      for (uint32_t i = it < C::kStages ? 0 : it - C::kStages; i < it; ++i) {
-        mbar_wait(smem_u32(&kfull[i % C::kStages]), (i / C::kStages) & 1, &g_err_tree);
-        mbar_wait(smem_u32(&vfull[i % C::kStages]), (i / C::kStages) & 1, &g_err_tree);
-      }
-    }
-    } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer
-    if (lane == 0) {
-      // fp32 accumulation, M = N = 128, bf16 or e4m3 operands; V is read head-dim-major (bit 16)
-      constexpr uint32_t kIdesc = (1u << 4) | (kFp8 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)(kTile >> 3) << 17) |
-                                  ((uint32_t)(kRows >> 4) << 24);
-      constexpr int kParts = kFp8 ? 2 : 1, kSteps = kFp8 ? 4 : 8;  // MMAs of 32 or 16 along K
-      uint32_t it = 0, seg = 0, done[2] = {0, 0};                  // tiles, segments, tiles of each group so far
-      bool ok = true;
-      while (ok && w.next(a)) {
-        if (!mbar_wait(smem_u32(&q_full), seg & 1, &g_err_tree)) break;
-        ++seg;
-        const auto issue_s = [&](int j) -> bool {
-          const int gr = j & 1;
-          const uint32_t i = it + j, st = i % C::kStages, use = done[gr] + (j >> 1);
-          if (use >= 1 && !mbar_wait(smem_u32(&s_empty[gr]), (use - 1) & 1, &g_err_tree)) return false;
-          if (!mbar_wait(smem_u32(&kfull[st]), (i / C::kStages) & 1, &g_err_tree)) return false;
-          tc::fence_after();
-          const uint32_t q = sbase + C::kQ, k = sbase + C::kRing + st * C::kStage;
-#pragma unroll
-          for (int part = 0; part < kParts; ++part)
-#pragma unroll
-            for (int ks = 0; ks < kSteps; ++ks) {
-              const uint32_t off = (kFp8 ? 0 : (ks >> 2) * kPart) + (ks & 3) * 32;
-              mma<kFp8>(tmem + gr * 128, desc_k(q + part * kPart + off), desc_k(k + off), kIdesc, part > 0 || ks > 0);
-            }
-          commit(smem_u32(&s_full[gr]));
-          return true;
-        };
-        ok = issue_s(0);
-        for (int j = 0; j < w.n && ok; ++j) {
-          if (j + 1 < w.n && !issue_s(j + 1)) {
-            ok = false;
-            break;
-          }
-          const int gr = j & 1;
-          const uint32_t i = it + j, st = i % C::kStages, use = done[gr] + (j >> 1);
-          ok = mbar_wait(smem_u32(&p_full[gr]), use & 1, &g_err_tree) &&
-               mbar_wait(smem_u32(&vfull[st]), (i / C::kStages) & 1, &g_err_tree) &&
-               (use == 0 || mbar_wait(smem_u32(&pv_empty[gr]), (use - 1) & 1, &g_err_tree));
-          if (!ok) break;
-          tc::fence_after();
-          const uint32_t p = sbase + C::kP + gr * kOperand, v = sbase + C::kRing + st * C::kStage + C::kKV;
-#pragma unroll
-          for (int part = 0; part < kParts; ++part)
-#pragma unroll
-            for (int ks = 0; ks < kSteps; ++ks) {
-              const uint32_t off = (kFp8 ? 0 : (ks >> 2) * kPart) + (ks & 3) * 32;
-              mma<kFp8>(tmem + (2 + gr) * 128, desc_k(p + part * kPart + off), desc_mn(v + ks * (kFp8 ? 4096 : 2048), kPart),
-                        kIdesc | (1u << 16), part > 0 || ks > 0);
-            }
-          commit(smem_u32(&pv_full[gr]));
-          commit(smem_u32(&kv_empty[st]));
+        // no copy may outlive the CTA: wait (bounded) for the last phase of every stage
+        for (uint32_t i = it < C::kStages ? 0 : it - C::kStages; i < it; ++i) {
+          mbar_wait(smem_u32(&kfull[stage_of(i)]), phase_of(i), &g_err_tree);
+          mbar_wait(smem_u32(&vfull[stage_of(i)]), phase_of(i), &g_err_tree);
         }
-        it += w.n;
-        done[0] += (w.n + 1) >> 1;
-        done[1] += w.n >> 1;
       }
-    }
+    } else if (warp == 1) {
+      // ------------------------------------------------------------ MMA issuer
+      if (lane == 0) {
+        // fp32 accumulation, M = N = 128. Q K^T: bf16, or e4m3 parts of Q; P V: bf16
+        // or halves, V read head-dim-major (bit 16)
+        constexpr uint32_t kShape = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+        constexpr uint32_t kBf16 = kFp8 ? 0u : (1u << 7) | (1u << 10);
+        constexpr int kParts = kFp8 ? 2 : 1, kSteps = kFp8 ? 4 : 8;  // Q K^T: MMAs of 32 or 16 dims
+        uint32_t it = 0, seg = 0, done[2] = {0, 0}, outs[2] = {0, 0};  // tiles, segments; tiles and segments of each group
+        bool ok = true;
+        while (ok && w.next(a)) {
+          if (!mbar_wait(smem_u32(&q_full), seg & 1, &g_err_tree)) break;
+          ++seg;
+          // S of the group's next tile goes over P of its last: when that P V has ended
+          // (MMAs with different accumulators may run out of order)
+          const auto issue_s = [&](int j) -> bool {
+            const uint32_t i = it + j, st = stage_of(i), gr = j & 1, use = done[gr] + (j >> 1);
+            if (use > 0 && !mbar_wait(smem_u32(&pv_full[gr]), (use - 1) & 1, &g_err_tree)) return false;
+            if (!mbar_wait(smem_u32(&kfull[st]), phase_of(i), &g_err_tree)) return false;
+            tc::fence_after();
+            const uint32_t q = sbase + C::kQ, k = sbase + C::kRing + st * 2 * C::kKV;
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+#pragma unroll
+              for (int ks = 0; ks < kSteps; ++ks) {
+                const uint32_t off = (kFp8 ? 0 : (ks >> 2) * kHalf) + (ks & 3) * 32;
+                mma<kFp8>(tmem + gr * 128, desc_k(q + part * kHalf + off), desc_k(k + off), kShape | kBf16,
+                          part > 0 || ks > 0);
+              }
+            commit(smem_u32(&s_full[gr]));
+            commit(smem_u32(&k_empty[st]));
+            return true;
+          };
+          ok = issue_s(0);
+          for (int j = 0; j < w.n && ok; ++j) {
+            if (j + 1 < w.n && !issue_s(j + 1)) {
+              ok = false;
+              break;
+            }
+            const uint32_t i = it + j, st = stage_of(i), gr = j & 1, use = done[gr] + (j >> 1);
+            ok = mbar_wait(smem_u32(kFp8 ? &v16_full[i & 1] : &vfull[st]), kFp8 ? (i >> 1) & 1 : phase_of(i), &g_err_tree) &&
+                 // a segment's first P V overwrites the output rows of the segment before
+                 (j >= 2 || outs[gr] == 0 || mbar_wait(smem_u32(&o_empty[gr]), (outs[gr] - 1) & 1, &g_err_tree)) &&
+                 mbar_wait(smem_u32(&p_full[gr]), use & 1, &g_err_tree);
+            if (!ok) break;
+            tc::fence_after();
+            const uint32_t v = sbase + (kFp8 ? C::kV16 + (i & 1) * kOperand : C::kRing + st * 2 * C::kKV + C::kKV);
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              mma_ts(tmem + (2 + gr) * 128, tmem + gr * 128 + ks * 8, desc_mn(v + ks * 2048, kHalf),
+                     kShape | kBf16 | (1u << 16), j >= 2 || ks > 0);
+            commit(smem_u32(&pv_full[gr]));
+            commit(smem_u32(kFp8 ? &v16_empty[i & 1] : &v_empty[st]));
+          }
+          it += w.n;
+          done[0] += (w.n + 1) >> 1;
+          done[1] += w.n >> 1;
+          outs[0] += 1;
+          outs[1] += w.n > 1;
+        }
+      }
+    } else if (kFp8) {
+      // ------------------------------------------- V's e4m3 bytes to halves
+      uint32_t it = 0;
+      bool ok = true;
+      const int t2 = threadIdx.x - 64;
+      while (w.next(a)) {
+        for (int j = 0; j < w.n; ++j, ++it) {
+          const uint32_t st = stage_of(it), buf = it & 1;
+          ok = ok && mbar_wait(smem_u32(&vfull[st]), phase_of(it), &g_err_tree) &&
+               (it < 2 || mbar_wait(smem_u32(&v16_empty[buf]), ((it >> 1) - 1) & 1, &g_err_tree));
+          if (!ok) continue;
+          const uint32_t src = sbase + C::kRing + st * 2 * C::kKV + C::kKV, dst = sbase + C::kV16 + buf * kOperand;
+#pragma unroll 4
+          for (int i = 0; i < 16; ++i) {
+            // 16 dims (chunk c) of token t: two 8-dim chunks of its row's half c / 4
+            const int idx = i * 64 + t2, t = idx >> 3, c = idx & 7;
+            const uint4 x = lds128(src + t * 128 + ((c ^ (t & 7)) << 4));
+            uint32_t y[8];
+            e4m3x4_to_half(x.x, y[0], y[1]);
+            e4m3x4_to_half(x.y, y[2], y[3]);
+            e4m3x4_to_half(x.z, y[4], y[5]);
+            e4m3x4_to_half(x.w, y[6], y[7]);
+            const uint32_t row = dst + (c >> 2) * kHalf + t * 128;
+            const int first = (c & 3) * 2, odd = c >> 2;  // the halves' lanes start on different banks
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const bool up = (k ^ odd) != 0;
+              sts128(row + (((first + up) ^ (t & 7)) << 4), up ? y[4] : y[0], up ? y[5] : y[1], up ? y[6] : y[2],
+                     up ? y[7] : y[3]);
+            }
+          }
+          fence_async();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(smem_u32(&v16_full[buf]));
+            mbar_arrive(smem_u32(&v_empty[st]));
+          }
+        }
+      }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
@@ -328,8 +462,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = qd * 32 + lane;                    // query row of the unit = TMEM lane; token of a tile
     const int bar = 1 + gr;                          // the group's named barrier
     const uint32_t lane_base = tmem + ((uint32_t)(qd * 32) << 16);
-    const uint32_t srow = lane_base + gr * 128, pvrow = lane_base + (2 + gr) * 128;
-    const uint32_t pbase = sbase + C::kP + gr * kOperand;
+    const uint32_t srow = lane_base + gr * 128, orow = lane_base + (2 + gr) * 128;
     uint32_t it = 0, use = 0;
     bool ok = true;
     while (w.next(a)) {
@@ -346,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if constexpr (kFp8) {
           uint32_t mx = 0;
           bool finite = true;
-#pragma unroll 4
+#pragma unroll
           for (int c = 0; c < 16; ++c) {
             const uint4 x = in ? qp[c] : zero;
             const uint32_t wd[4] = {x.x & 0x7fff7fffu, x.y & 0x7fff7fffu, x.z & 0x7fff7fffu, x.w & 0x7fff7fffu};
@@ -380,13 +513,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             const uint32_t at = sbase + C::kQ + r * 128 + (((c >> 1) ^ (r & 7)) << 4);
             sts128(at, hi[0], hi[1], hi[2], hi[3]);
-            sts128(at + kPart, lo[0], lo[1], lo[2], lo[3]);
+            sts128(at + kHalf, lo[0], lo[1], lo[2], lo[3]);
           }
         } else {
 #pragma unroll
           for (int c = 0; c < 8; ++c) {
             const uint4 x = in ? qp[gr * 8 + c] : zero;
-            sts128(sbase + C::kQ + gr * kPart + r * 128 + ((c ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
+            sts128(sbase + C::kQ + gr * kHalf + r * 128 + ((c ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
           }
         }
       }
@@ -394,177 +527,160 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(smem_u32(&q_full));
 
-      float o[kHD];
-#pragma unroll
-      for (int i = 0; i < kHD; ++i) o[i] = 0.f;
-      float m_run = -INFINITY, l_run = 0.f;
-      float corr_prev = 1.f;  // factor of the tile whose P V is folded next
-      bool pending = false;
-      // O = O * corr + P V of this group's last tile
-      const auto fold = [&](float corr) {
+      float m_ref = -INFINITY, l_run = 0.f;
+      // the group's output rows, when the P V of its last tile has ended
+      const auto wait_o = [&]() {
         ok = ok && mbar_wait(smem_u32(&pv_full[gr]), (use - 1) & 1, &g_err_tree);
         tc::fence_after();
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tc::tmem_ld32(pvrow + c * 32, v);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[c * 32 + i] = o[c * 32 + i] * corr + v[i];
-        }
-        tc::fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&pv_empty[gr]));
       };
       for (int j = gr; j < w.n; j += 2) {
-        const uint32_t i0 = it + j, st = i0 % C::kStages, ph = (i0 / C::kStages) & 1;
+        const uint32_t i0 = it + j, st = stage_of(i0), tb = gr * 2 + (use & 1);
         const int p0 = (w.t0 + j) * kTile;
         const bool tail = p0 + kTile > base;
         if constexpr (kFp8) {
-          // the tile's scales as floats, a token a thread
-          ok = ok && mbar_wait(smem_u32(&kfull[st]), ph, &g_err_tree);
+          // the tile's scales as floats, a token a thread (the buffer's last
+          // readers have passed the barrier of the tile between)
+          ok = ok && mbar_wait(smem_u32(&kfull[st]), phase_of(i0), &g_err_tree);
           const uint32_t kc = scales[st][0][r], vc = scales[st][1][r];
           float inv = __uint_as_float((254u - vc) << 23);
           if (tail && !(inv >= 0.f && inv < INFINITY)) inv = 0.f;  // stale scale bytes
-          named_bar_sync(bar, 128);                                 // the tile before is done with them
-          tok_k[gr][r] = __uint_as_float(kc << 23);
-          tok_b[gr][r] = (float)((int)vc - 127);
-          tok_i[gr][r] = inv;
+          tok_k[tb][r] = __uint_as_float(kc << 23);
+          tok_b[tb][r] = (float)((int)vc - 127);
+          tok_i[tb][r] = inv;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&k_empty[st]));
           named_bar_sync(bar, 128);
         }
         ok = ok && mbar_wait(smem_u32(&s_full[gr]), use & 1, &g_err_tree);
         tc::fence_after();
-        // four scores of a row, from token t on, as powers of two
-        const auto scores4 = [&](float* s, int t) {
+        float v[128];  // the row's scores, as powers of two
+        tmem_row(srow, v);
+        const uint64_t rs2 = pk2(rscale, rscale);
+#pragma unroll
+        for (int i = 0; i < 128; i += 4) {
+          uint64_t x = mul2(pk2(v[i], v[i + 1]), rs2), y = mul2(pk2(v[i + 2], v[i + 3]), rs2);
           if constexpr (kFp8) {
-            const float4 k = *reinterpret_cast<const float4*>(&tok_k[gr][t]), b = *reinterpret_cast<const float4*>(&tok_b[gr][t]);
-            s[0] = fmaf(s[0] * rscale, k.x, b.x);
-            s[1] = fmaf(s[1] * rscale, k.y, b.y);
-            s[2] = fmaf(s[2] * rscale, k.z, b.z);
-            s[3] = fmaf(s[3] * rscale, k.w, b.w);
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] *= rscale;
+            const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&tok_k[tb][i]);
+            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&tok_b[tb][i]);
+            x = fma2(x, k.x, b.x);
+            y = fma2(y, k.y, b.y);
           }
-        };
-        float mx = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tc::tmem_ld32(srow + c * 32, v);
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) scores4(v + i, c * 32 + i);
-          if (tail) {
-            const uint32_t seen = in ? seen32(a, qrow, node, base, w.s.len, p0 + c * 32) : 0u;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = (seen >> i) & 1u ? v[i] : -INFINITY;
-          }
-#pragma unroll
-          for (int i = 0; i < 32; ++i) mx = fmaxf(mx, v[i]);
+          un2(x, v[i], v[i + 1]);
+          un2(y, v[i + 2], v[i + 3]);
         }
-        const float m_new = fmaxf(m_run, mx);
-        const float ref = m_new == -INFINITY ? 0.f : m_new;
-        const float corr = ex2(m_run - ref);
-        float psum = 0.f;
-        // this group's P was last read by P V of its tile before, folded below
-        if (pending) fold(corr_prev);
-        corr_prev = corr;
-        const float shift = kFp8 ? ref - 8.f : ref;  // e4m3 weights are scaled by 2^8
-#pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tc::tmem_ld32(srow + c * 32, v);
+        if (tail) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) scores4(v + i, c * 32 + i);
-          if (tail) {
+          for (int c = 0; c < 4; ++c) {
             const uint32_t seen = in ? seen32(a, qrow, node, base, w.s.len, p0 + c * 32) : 0u;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = (seen >> i) & 1u ? v[i] : -INFINITY;
+            for (int i = 0; i < 32; ++i) v[c * 32 + i] = (seen >> i) & 1u ? v[c * 32 + i] : -INFINITY;
           }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
+        for (int i = 0; i < 128; i += 8)
 #pragma unroll
-            for (int y = 0; y < 4; ++y) v[i + y] = ex2(v[i + y] - shift);
+          for (int y = 0; y < 4; ++y) mx[y] = fmaxf(mx[y], fmaxf(v[i + 2 * y], v[i + 2 * y + 1]));
+        const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const bool first = j < 2;
+        const bool move = first || m_tile > m_ref + kSlack;
+        if (__any_sync(0xffffffffu, move)) {
+          const float m_new = move ? fmaxf(m_ref, m_tile) : m_ref;
+          if (!first) {
+            const float corr = m_new == m_ref ? 1.f : ex2(m_ref - m_new);
+            wait_o();
+            // a few columns at a time: the scores stay in their registers
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+              float y[16];
+              tc::tmem_ld16(orow + c * 16, y);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) y[i] *= corr;
+              tc::tmem_st16(orow + c * 16, y);
+            }
+            l_run *= corr;
+          }
+          m_ref = m_new;
+        }
+        const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+        uint64_t sum[4] = {0, 0, 0, 0};
+        const uint64_t nref = pk2(-ref, -ref);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t p[16];
+#pragma unroll
+          for (int i = c * 32; i < c * 32 + 32; i += 4) {
+            un2(add2(pk2(v[i], v[i + 1]), nref), v[i], v[i + 1]);
+            un2(add2(pk2(v[i + 2], v[i + 3]), nref), v[i + 2], v[i + 3]);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) v[i + y] = ex2(v[i + y]);
+            const uint64_t x = pk2(v[i], v[i + 1]), y = pk2(v[i + 2], v[i + 3]);
+            const int sx = (i >> 1) & 2;
             if constexpr (kFp8) {
-              const float4 n = *reinterpret_cast<const float4*>(&tok_i[gr][c * 32 + i]);
-              psum = fmaf(v[i], n.x, psum);
-              psum = fmaf(v[i + 1], n.y, psum);
-              psum = fmaf(v[i + 2], n.z, psum);
-              psum = fmaf(v[i + 3], n.w, psum);
+              const ulonglong2 n = *reinterpret_cast<const ulonglong2*>(&tok_i[tb][i]);
+              sum[sx] = fma2(x, n.x, sum[sx]);
+              sum[sx + 1] = fma2(y, n.y, sum[sx + 1]);
             } else {
-              psum += (v[i] + v[i + 1]) + (v[i + 2] + v[i + 3]);
+              sum[sx] = add2(sum[sx], x);
+              sum[sx + 1] = add2(sum[sx + 1], y);
             }
+            p[(i & 31) / 2] = kFp8 ? pack_half(v[i], v[i + 1]) : pack_bf16(v[i], v[i + 1]);
+            p[(i & 31) / 2 + 1] = kFp8 ? pack_half(v[i + 2], v[i + 3]) : pack_bf16(v[i + 2], v[i + 3]);
           }
-          if constexpr (kFp8) {
-            uint32_t hi[8], lo[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) split4(v + 4 * i, hi[i], lo[i]);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const uint32_t at = pbase + r * 128 + (((c * 2 + k) ^ (r & 7)) << 4);
-              sts128(at, hi[4 * k], hi[4 * k + 1], hi[4 * k + 2], hi[4 * k + 3]);
-              sts128(at + kPart, lo[4 * k], lo[4 * k + 1], lo[4 * k + 2], lo[4 * k + 3]);
-            }
-          } else {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-              sts128(pbase + (c >> 1) * kPart + r * 128 + ((((c & 1) * 4 + k) ^ (r & 7)) << 4),
-                     pack_bf16(v[8 * k], v[8 * k + 1]), pack_bf16(v[8 * k + 2], v[8 * k + 3]),
-                     pack_bf16(v[8 * k + 4], v[8 * k + 5]), pack_bf16(v[8 * k + 6], v[8 * k + 7]));
-          }
+          tmem_put16(srow + c * 16, p);
         }
+        {
+          const uint64_t x = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
+          float s0, s1;
+          un2(x, s0, s1);
+          l_run += s0 + s1;
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        bool any_odd = false;
         if (tail) {
           // Rows of V past the context hold stale bytes (possibly NaN), and drafted
           // rows may be hidden from some query rows: a zero weight does not cancel
           // NaN or infinities. Zero the former; take drafted rows that are not
-          // finite out of the tile and add them here, row by row.
-          ok = ok && mbar_wait(smem_u32(&vfull[st]), ph, &g_err_tree);
-          const uint32_t vr = sbase + C::kRing + st * C::kStage + C::kKV + r * 128;
+          // finite out of the tile and add their share, summed here row by row, when
+          // the tile's P V has ended.
+          ok = ok && mbar_wait(smem_u32(kFp8 ? &v16_full[i0 & 1] : &vfull[st]), kFp8 ? (i0 >> 1) & 1 : phase_of(i0),
+                               &g_err_tree);
+          const uint32_t vt = sbase + (kFp8 ? C::kV16 + (i0 & 1) * kOperand : C::kRing + st * 2 * C::kKV + C::kKV);
+          const uint32_t vr = vt + r * 128;
           bool odd = false;
           if (p0 + r >= base && p0 + r < w.s.len) {
 #pragma unroll 1
-            for (int c = 0; c < (kFp8 ? 8 : 16); ++c) {
-              const uint4 x = lds128(vr + (c >> 3) * kPart + ((c & 7) << 4));  // any order: the whole row is looked at
-              const uint32_t wd[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                odd |= kFp8 ? __vcmpeq4(wd[i] & 0x7f7f7f7fu, 0x7f7f7f7fu) != 0
-                            : __vcmpeq2(wd[i] & 0x7f807f80u, 0x7f807f80u) != 0;
+            for (int c = 0; c < 16; ++c) {
+              const uint4 x = lds128(vr + (c >> 3) * kHalf + ((c & 7) << 4));  // any order: the whole row is looked at
+              const uint32_t ex = kFp8 ? 0x7c007c00u : 0x7f807f80u;
+              odd |= (__vcmpeq2(x.x & ex, ex) | __vcmpeq2(x.y & ex, ex) | __vcmpeq2(x.z & ex, ex) |
+                      __vcmpeq2(x.w & ex, ex)) != 0;
             }
           }
-          if (any_of_barrier(bar, 128, odd)) {
+          any_odd = any_of_barrier(bar, 128, odd);
+          if (any_odd) {
             const uint32_t bits = __ballot_sync(0xffffffffu, odd);
             if (lane == 0) odd_bits[gr][qd] = bits;
             named_bar_sync(bar, 128);
 #pragma unroll
-            for (int i = 0; i < kHD; ++i) o[i] *= corr;
-            corr_prev = 1.f;
+            for (int i = 0; i < kHD; ++i) v[i] = 0.f;
 #pragma unroll 1
             for (int t = 0; t < kTile; ++t) {
               if (!((odd_bits[gr][t >> 5] >> (t & 31)) & 1u)) continue;  // the same for the whole group
               const uint32_t seen = in ? seen32(a, qrow, node, base, w.s.len, p0 + (t & ~31)) : 0u;
-              float x = tmem_ld1(srow + t) * rscale;
-              if (kFp8) x = fmaf(x, tok_k[gr][t], tok_b[gr][t]);
+              const uint32_t two = tmem_ld1(srow + (t >> 1)) >> (t & 1 ? 16 : 0);
               if ((seen >> (t & 31)) & 1u) {
-                const float p = ex2(x - shift);
-                const uint32_t row = sbase + C::kRing + st * C::kStage + C::kKV + t * 128;
+                const float p = kFp8 ? __half2float(__ushort_as_half((unsigned short)two)) : __uint_as_float(two << 16);
 #pragma unroll
-                for (int c = 0; c < (kFp8 ? 8 : 16); ++c) {
-                  const uint4 y = lds128(row + (c >> 3) * kPart + (((c & 7) ^ (t & 7)) << 4));
+                for (int c = 0; c < 16; ++c) {
+                  const uint4 y = lds128(vt + t * 128 + (c >> 3) * kHalf + (((c & 7) ^ (t & 7)) << 4));
                   const uint32_t wd[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                   for (int i = 0; i < 4; ++i) {
-                    if constexpr (kFp8) {
-                      uint32_t h0, h1;
-                      e4m3x4_to_half(wd[i], h0, h1);
-                      const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0));
-                      const float2 f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                      float* at = o + c * 16 + i * 4;
-                      at[0] += p * f0.x, at[1] += p * f0.y, at[2] += p * f1.x, at[3] += p * f1.y;
-                    } else {
-                      float* at = o + c * 8 + i * 2;
-                      at[0] += p * __uint_as_float(wd[i] << 16);
-                      at[1] += p * __uint_as_float(wd[i] & 0xffff0000u);
-                    }
+                    const float2 f = kFp8 ? __half22float2(*reinterpret_cast<const __half2*>(&wd[i]))
+                                          : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wd[i]));
+                    v[c * 8 + i * 2] += p * f.x;
+                    v[c * 8 + i * 2 + 1] += p * f.y;
                   }
                 }
               }
@@ -574,73 +690,93 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (odd || p0 + r >= w.s.len) {
 #pragma unroll
-            for (int c = 0; c < (kFp8 ? 8 : 16); ++c) sts128(vr + (c >> 3) * kPart + ((c & 7) << 4), 0u, 0u, 0u, 0u);
+            for (int c = 0; c < 16; ++c) sts128(vr + (c >> 3) * kHalf + ((c & 7) << 4), 0u, 0u, 0u, 0u);
           }
+          fence_async();
         }
         tc::fence_before();
-        fence_async();
         __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(smem_u32(&s_empty[gr]));
-          mbar_arrive(smem_u32(&p_full[gr]));
-        }
-        l_run = fmaf(l_run, corr, psum);
-        m_run = m_new;
-        pending = true;
+        if (lane == 0) mbar_arrive(smem_u32(&p_full[gr]));
         ++use;
+        if (any_odd) {
+          wait_o();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float y[16];
+            tc::tmem_ld16(orow + c * 16, y);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] += v[c * 16 + i];
+            tc::tmem_st16(orow + c * 16, y);
+          }
+          tc::fence_before();
+        }
       }
-      if (pending) fold(corr_prev);
       it += w.n;
+      const bool any = gr < w.n;
+      if (any) wait_o();
+      float o[128];  // the group's output rows (read in any case, so that no path leaves them without a value)
+      tmem_row(orow, o);
+      tc::fence_before();
+      __syncwarp();
+      if (any && lane == 0) mbar_arrive(smem_u32(&o_empty[gr]));
 
       // ---------------------------------------------- join the two groups' tiles
-      if (!ok) m_run = -INFINITY, l_run = 0.f;
-      const uint32_t scratch = sbase + C::kP + r * 512;  // both P buffers: no MMA reads them any more
-      named_bar_sync(3, kGroups * 128);                  // both groups' MMAs are over (Q is free as well)
+      if (!ok) m_ref = -INFINITY, l_run = 0.f;
+      named_bar_sync(3, kGroups * 128);  // both groups' MMAs are over: Q's memory is free
+      float f0 = 1.f, f1 = 0.f;
       if (w.n > 1) {
-        if (gr == 1) {
-          m_other[r] = m_run;
-          l_other[r] = l_run;
+        // group 1 hands its rows over, 64 dims at a time
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            sts128(scratch + ((c ^ lane) << 4), __float_as_uint(o[4 * c]), __float_as_uint(o[4 * c + 1]),
-                   __float_as_uint(o[4 * c + 2]), __float_as_uint(o[4 * c + 3]));
-        }
-        named_bar_sync(3, kGroups * 128);
-      }
-      if (gr == 0) {
-        float f0 = 1.f;
-        if (w.n > 1) {
-          const float m1 = m_other[r], M = fmaxf(m_run, m1);
-          f0 = m_run == -INFINITY ? 0.f : ex2(m_run - M);
-          const float f1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
-          l_run = l_run * f0 + l_other[r] * f1;
-          m_run = M;
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t row = sbase + C::kQ + r * 256;
+          if (gr == 1) {
+            if (half == 0) m_other[r] = m_ref, l_other[r] = l_run;
 #pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            const uint4 x = lds128(scratch + ((c ^ lane) << 4));
-            o[4 * c] = o[4 * c] * f0 + __uint_as_float(x.x) * f1;
-            o[4 * c + 1] = o[4 * c + 1] * f0 + __uint_as_float(x.y) * f1;
-            o[4 * c + 2] = o[4 * c + 2] * f0 + __uint_as_float(x.z) * f1;
-            o[4 * c + 3] = o[4 * c + 3] * f0 + __uint_as_float(x.w) * f1;
+            for (int c = 0; c < 16; ++c) {
+              const float* x = o + half * 64 + 4 * c;
+              sts128(row + ((c ^ (r & 15)) << 4), __float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
+                     __float_as_uint(x[3]));
+            }
           }
+          named_bar_sync(3, kGroups * 128);
+          if (gr == 0) {
+            if (half == 0) {
+              const float m1 = m_other[r], M = fmaxf(m_ref, m1);
+              f0 = m_ref == -INFINITY ? 0.f : ex2(m_ref - M);
+              f1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
+              l_run = l_run * f0 + l_other[r] * f1;
+              m_ref = M;
+            }
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              float* x = o + half * 64 + 4 * c;
+              const uint4 y = lds128(row + ((c ^ (r & 15)) << 4));
+              x[0] = x[0] * f0 + __uint_as_float(y.x) * f1;
+              x[1] = x[1] * f0 + __uint_as_float(y.y) * f1;
+              x[2] = x[2] * f0 + __uint_as_float(y.z) * f1;
+              x[3] = x[3] * f0 + __uint_as_float(y.w) * f1;
+            }
+          }
+          named_bar_sync(3, kGroups * 128);
         }
-        if (in && w.whole()) {
+      }
+      if (gr == 0 && in) {
+        if (w.whole()) {
           const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // nothing seen: 0
           uint4* op = reinterpret_cast<uint4*>(a.out + (int64_t)qrow * a.o_st + (int64_t)head * a.o_sh);
 #pragma unroll
           for (int c = 0; c < 16; ++c)
             op[c] = make_uint4(pack_bf16(o[8 * c] * inv, o[8 * c + 1] * inv), pack_bf16(o[8 * c + 2] * inv, o[8 * c + 3] * inv),
                                pack_bf16(o[8 * c + 4] * inv, o[8 * c + 5] * inv), pack_bf16(o[8 * c + 6] * inv, o[8 * c + 7] * inv));
-        } else if (in) {
+        } else {
           const int64_t pr = ((int64_t)blockIdx.x * 2 + w.slot()) * kRows + r;
           float4* dst = reinterpret_cast<float4*>(a.part_o + pr * kHD);
 #pragma unroll
           for (int c = 0; c < 32; ++c) dst[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-          a.part_m[pr] = m_run;
+          a.part_m[pr] = m_ref;
           a.part_l[pr] = l_run;
         }
       }
-      named_bar_sync(3, kGroups * 128);  // the P buffers are free again
     }
   }
   tc::fence_before();
