@@ -164,33 +164,23 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
       uint32_t it = 0;
       bool ok = true;
       while (ok && w.next(a)) {
-        int col = -1, blk = 0;
-        bool bad = false;
+        const int boxes = kTile / a.box;
+        tree::Pages pg;
+        pg.start(a, w, w.t0 * kTile);
         for (int j = 0; j < w.n; ++j, ++it) {
           const int s = it % C::kStages;
           if (it >= C::kStages && !mbar_wait(smem_u32(&empty_bar[s]), (it / C::kStages - 1) & 1, &g_err_tree)) {
             ok = false;
             break;
           }
-          const int tok = (w.t0 + j) * kTile;
           const uint32_t st = smem_u32(smem + s * C::kStage);
           const uint32_t fb = smem_u32(&full_bar[s]);
           // a tile is one box, or two when the pages hold 64 tokens (their second
           // half may lie past the sequence: it is read as zeros then)
-          const int boxes = kTile / a.box;
           for (int x = 0; x < boxes; ++x) {
-            const int at = tok + x * a.box;
-            if (at / a.block_size != col) {
-              col = at / a.block_size;
-              const bool past = at >= w.s.len;
-              blk = past ? -1 : a.tables[(int64_t)w.b * a.bt_stride + col];  // len is cut to the table
-              bad = blk < 0 || blk >= a.num_blocks;
-              if (bad) {
-                if (!past) atomicOr(&g_err_tree, (unsigned)kErrBlockTable);
-                blk = a.num_blocks;  // out of the tensor map: TMA fills zeros
-              }
-            }
-            const int off = at - col * a.block_size;
+            const bool bad = pg.absent(a, w);
+            const int blk = bad ? a.num_blocks : pg.blk;  // out of the tensor map: TMA fills zeros
+            const int off = pg.off;
             if (kFp8 && bad) {  // a block outside the pool reads zeros, of scale 1
               for (int i = 0; i < 2; ++i)
                 for (int h = 0; h < HP; ++h)
@@ -218,6 +208,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
                 bulk_load(smem_u32(&scales[s][1][h * kTile + x * a.box]), a.vs + so + (int64_t)h * a.block_size, a.box, fb);
               }
             }
+            pg.advance(a, w, a.box);
           }
         }
       }

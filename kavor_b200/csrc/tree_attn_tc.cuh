@@ -4,13 +4,14 @@
 // A CTA owns 128 query rows (nodes x query heads of one kv head) and walks the
 // context in 128-token tiles: S = Q K^T is a tcgen05.mma chain into TMEM, two
 // softmax warpgroups take the tiles in turn (one thread per query row, so no
-// reduction crosses threads) and put the weights P back over S in TMEM, from where
-// a second chain adds P V to the group's output rows, also in TMEM. The two groups
-// keep separate references and sums, which are joined at the end of a segment, so
-// one group's exponentials overlap the other group's MMAs. A row's reference moves
-// only when its maximum has passed it by 2^8: weights of up to 2^8 cost nothing in
-// bf16 or half, and the output rows are rescaled once or twice in a context instead
-// of at every tile. One warp issues the TMA loads, one thread the MMAs.
+// reduction crosses threads), walk S twice in loops of 64 columns (straight-line
+// code for a row missed the instruction cache) and put the weights P in TMEM, from
+// where a second chain adds P V to the output rows, also in TMEM. One group's exponentials overlap the
+// other group's and the MMAs. Both groups weigh a row against the same reference,
+// settled tile by tile (a barrier hands it from group to group); it moves only when
+// a tile's maximum passes it by 2^15: weights of up to 2^15 cost nothing in bf16 or
+// half, and the output rows are rescaled once or twice in a context instead of at
+// every tile. One warp issues the TMA loads, one thread the MMAs.
 //
 // Over an e4m3 cache K stays e4m3: Q is split in two e4m3 parts, x = hi + lo, hi =
 // e4m3(x), lo = e4m3(x - hi), which hold a bf16 value (8 bits, two signed 4-bit
@@ -33,8 +34,9 @@ constexpr int kThreads = 128 + kGroups * 128;             // warp 0 TMA, 1 MMA +
 // Registers: 168 a thread at launch (384 threads); the control warps give theirs
 // up for the softmax threads' output rows: 128 (56 + 2 * 224) = 384 * 168.
 constexpr int kControlRegs = 56, kSoftmaxRegs = 224;
-constexpr uint32_t kCols = 512;                           // S0, S1 (then P0, P1), O0, O1: 128 columns each
-constexpr float kSlack = 8.f;                             // log2 of the largest weight
+constexpr uint32_t kCols = 512;                           // S0, S1, O: 128 columns each; P0, P1: 64
+constexpr uint32_t kColO = 256, kColP = 384;
+constexpr float kSlack = 15.f;                            // log2 of the largest weight: below the largest half
 constexpr int kHalf = kTile * 128;                        // 128 rows of 128 bytes
 constexpr int kOperand = 2 * kHalf;                       // 16-bit Q or V (two halves of 64 dims), or two e4m3 parts of Q
 template <bool kFp8>
@@ -57,28 +59,41 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t addr, uint32_t apart) {
   return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(apart >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
+// The MMAs and commits are written for a whole warp: the instruction itself elects
+// its one thread. A warp without a branch keeps the descriptors in uniform
+// registers; from one thread's branch each MMA waited 93 cycles for its descriptors'
+// way there (an MMA itself takes 64).
 template <bool kFp8>
 __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   if constexpr (kFp8)
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc));
   else
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
         "l"(a), "l"(b), "r"(idesc), "r"(acc));
 }
 // D (+)= P V with the 16-bit P in TMEM (two values a column, a row a lane).
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "{\n\t.reg .pred p, e;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"(acc));
 }
 __device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  asm volatile(
+      "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar)
+      : "memory");
+}
+// The same value in every lane, known as such to the compiler.
+__device__ __forceinline__ uint32_t uniform(uint32_t x) { return __shfl_sync(0xffffffffu, x, 0); }
+// The arriving half of a named barrier whose other half waits.
+__device__ __forceinline__ void named_bar_arrive(int id, int nthreads) {
+  asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ bool any_of_barrier(int id, int threads, bool x) {
@@ -98,8 +113,8 @@ __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
   return r;
 }
 // 32 columns of this thread's lane into r[kAt..], without waiting; ready after landed().
-template <int kAt>
-__device__ __forceinline__ void tmem_get(uint32_t taddr, float (&v)[128]) {
+template <int kAt, int kN>
+__device__ __forceinline__ void tmem_get(uint32_t taddr, float (&v)[kN]) {
   float* r = v + kAt;
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
@@ -110,8 +125,8 @@ __device__ __forceinline__ void tmem_get(uint32_t taddr, float (&v)[128]) {
         "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
       : "r"(taddr));
 }
-template <int kAt>
-__device__ __forceinline__ void pin(float (&v)[128]) {  // no use of the registers moves before this
+template <int kAt, int kN>
+__device__ __forceinline__ void pin(float (&v)[kN]) {  // no use of the registers moves before this
   float* r = v + kAt;
   asm volatile(""
                : "+f"(r[0]), "+f"(r[1]), "+f"(r[2]), "+f"(r[3]), "+f"(r[4]), "+f"(r[5]), "+f"(r[6]), "+f"(r[7]), "+f"(r[8]),
@@ -119,21 +134,13 @@ __device__ __forceinline__ void pin(float (&v)[128]) {  // no use of the registe
                  "+f"(r[17]), "+f"(r[18]), "+f"(r[19]), "+f"(r[20]), "+f"(r[21]), "+f"(r[22]), "+f"(r[23]), "+f"(r[24]),
                  "+f"(r[25]), "+f"(r[26]), "+f"(r[27]), "+f"(r[28]), "+f"(r[29]), "+f"(r[30]), "+f"(r[31]));
 }
-// A row's 128 columns.
-__device__ __forceinline__ void tmem_row(uint32_t taddr, float (&v)[128]) {
+// 64 columns of a row.
+__device__ __forceinline__ void tmem_row64(uint32_t taddr, float (&v)[64]) {
   tmem_get<0>(taddr, v);
   tmem_get<32>(taddr + 32, v);
-  tmem_get<64>(taddr + 64, v);
-  tmem_get<96>(taddr + 96, v);
   asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
   pin<0>(v);
   pin<32>(v);
-  pin<64>(v);
-  pin<96>(v);
-}
-__device__ __forceinline__ void tmem_put_row(uint32_t taddr, const float (&v)[128]) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c) tc::tmem_st32(taddr + c * 32, v + c * 32);
 }
 // 16 columns of this thread's lane.
 __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t (&r)[16]) {
@@ -225,11 +232,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   kernel_entry();
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t q_full, kfull[C::kStages], vfull[C::kStages], k_empty[C::kStages], v_empty[C::kStages],
-      v16_full[2], v16_empty[2], s_full[2], p_full[2], pv_full[2], o_empty[2];
+      v16_full[2], v16_empty[2], s_full[2], s_empty[2], p_full[2], pv_full[2], o_empty;
   __shared__ __align__(16) uint8_t scales[kFp8 ? C::kStages : 1][2][kTile];
-  // scales 2^a (K) and 2^b (V) of a tile as floats: 2^a, b and 2^-b; two tiles of each group
-  __shared__ __align__(16) float tok_k[kFp8 ? 4 : 1][kTile], tok_b[kFp8 ? 4 : 1][kTile], tok_i[kFp8 ? 4 : 1][kTile];
-  __shared__ float m_other[kRows], l_other[kRows];
+  // scales 2^a (K) and 2^b (V) of a tile: 2^a, b and 2^-b, exact in bf16; two tiles of each group
+  __shared__ __align__(16) bf16 tok_k[kFp8 ? 4 : 1][kTile], tok_b[kFp8 ? 4 : 1][kTile], tok_i[kFp8 ? 4 : 1][kTile];
+  __shared__ float ref_s[kRows], l_s[2][kRows];
+  __shared__ uint32_t o_started;  // the output rows hold something before a segment's first P V
   __shared__ uint32_t odd_bits[2][4];
   __shared__ uint32_t tmem_s;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -248,10 +256,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(smem_u32(&v16_full[i]), 2);
       mbar_init(smem_u32(&v16_empty[i]), 1);
       mbar_init(smem_u32(&s_full[i]), 1);
+      mbar_init(smem_u32(&s_empty[i]), 4);
       mbar_init(smem_u32(&p_full[i]), 4);
       mbar_init(smem_u32(&pv_full[i]), 1);
-      mbar_init(smem_u32(&o_empty[i]), 4);
     }
+    mbar_init(smem_u32(&o_empty), kGroups * 4);
+    o_started = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
@@ -271,145 +281,132 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
-    if (warp == 0) {
-      // ---------------------------------------------------------- TMA producer
+    if (warp == 0 || (!kFp8 && warp == 2)) {
+      // --------------------------------------------------------- TMA producers
+      // Warp 0 loads K and the e4m3 rows of V; bf16 rows of V, whose buffers are
+      // held until their P V has ended, have warp 2 for themselves.
+      const bool do_k = warp == 0, do_v = kFp8 || warp == 2;
       if (lane == 0) {
-        prefetch_tensormap(&kmap);
-        prefetch_tensormap(&vmap);
+        prefetch_tensormap(do_k ? &kmap : &vmap);
         const uint64_t pol = l2_evict_first_policy();
+        const int boxes = kTile / a.box;
         uint32_t it = 0;
         bool ok = true;
         while (ok && w.next(a)) {
           const bool once = w.s.blocks == 1;  // else several row blocks read the same rows: keep those in L2
-          int col = -1, blk = 0;
-          bool bad = false;
-          for (int j = 0; j < w.n && ok; ++j, ++it) {
-            const uint32_t st = stage_of(it);
-            const int t0 = (w.t0 + j) * kTile, boxes = kTile / a.box;
-            const uint32_t kd = sbase + C::kRing + st * 2 * C::kKV, vd = kd + C::kKV;
-            const uint32_t kb = smem_u32(&kfull[st]), vb = smem_u32(&vfull[st]);
-            if (it >= C::kStages) ok = mbar_wait(smem_u32(&k_empty[st]), phase_of(it - C::kStages), &g_err_tree);
-            if (!ok) break;
-            int bcol[2], bblk[2];
-            for (int x = 0; x < boxes; ++x) {
-              const int at = t0 + x * a.box;
-              if (at / a.block_size != col) {
-                col = at / a.block_size;
-                const bool past = at >= w.s.len;
-                blk = past ? -1 : a.tables[(int64_t)w.b * a.bt_stride + col];
-                bad = blk < 0 || blk >= a.num_blocks;
-                if (bad) {
-                  if (!past) atomicOr(&g_err_tree, (unsigned)kErrBlockTable);
-                  blk = a.num_blocks;  // out of the tensor map: TMA fills zeros
-                }
-              }
-              bcol[x] = at - col * a.block_size;
-              bblk[x] = blk;
-              if (kFp8 && bad) {  // a block outside the pool reads zeros, of scale 1
-                for (int i = 0; i < 2; ++i)
-                  for (int k = 0; k < a.box / 4; ++k)
-                    reinterpret_cast<uint32_t*>(&scales[st][i][x * a.box])[k] = 0x7f7f7f7fu;
-                fence_async();  // before a later copy into the same bytes
-              }
-              const uint32_t bytes = C::kKV / boxes + (kFp8 && !bad ? 2 * a.box : 0);  // the scales come with K
-              if (x + 1 < boxes)
-                mbar_expect_tx(kb, bytes);
+          const auto load = [&](const CUtensorMap* map, uint32_t dst, int off, int blk, uint32_t bar) {
+#pragma unroll
+            for (int hf = 0; hf < (kFp8 ? 1 : 2); ++hf) {
+              if (once)
+                tma_load_4d(dst + hf * kHalf, map, hf * 64, w.h, off, blk, bar, pol);
               else
-                mbar_arrive_expect_tx(kb, bytes);
-              if (kFp8 && !bad) {
-                const int64_t so = blk * a.scale_stride + (int64_t)w.h * a.block_size + bcol[x];
-                bulk_load(smem_u32(&scales[st][0][x * a.box]), a.ks + so, a.box, kb);
-                bulk_load(smem_u32(&scales[st][1][x * a.box]), a.vs + so, a.box, kb);
-              }
-#pragma unroll
-              for (int hf = 0; hf < (kFp8 ? 1 : 2); ++hf) {
-                if (once)
-                  tma_load_4d(kd + hf * kHalf + x * a.box * 128, &kmap, hf * 64, w.h, bcol[x], blk, kb, pol);
-                else
-                  tma_load_4d_keep(kd + hf * kHalf + x * a.box * 128, &kmap, hf * 64, w.h, bcol[x], blk, kb);
-              }
+                tma_load_4d_keep(dst + hf * kHalf, map, hf * 64, w.h, off, blk, bar);
             }
-            if (it >= C::kStages) ok = mbar_wait(smem_u32(&v_empty[st]), phase_of(it - C::kStages), &g_err_tree);
-            if (!ok) {
-              mbar_wait(kb, phase_of(it), &g_err_tree);  // this tile's K copies
-              break;
+          };
+          tree::Pages pg;
+          pg.start(a, w, w.t0 * kTile);
+          for (int j = 0; j < w.n && ok; ++j, ++it) {
+            const uint32_t st = stage_of(it), kd = sbase + C::kRing + st * 2 * C::kKV, vd = kd + C::kKV;
+            const uint32_t kb = smem_u32(&kfull[st]), vb = smem_u32(&vfull[st]);
+            if (it >= C::kStages) {
+              if (do_k) ok = mbar_wait(smem_u32(&k_empty[st]), phase_of(it - C::kStages), &g_err_tree);
+              if (do_v) ok = ok && mbar_wait(smem_u32(&v_empty[st]), phase_of(it - C::kStages), &g_err_tree);
+              if (!ok) break;
             }
-            mbar_arrive_expect_tx(vb, C::kKV);
-            for (int x = 0; x < boxes; ++x)
-#pragma unroll
-              for (int hf = 0; hf < (kFp8 ? 1 : 2); ++hf) {
-                if (once)
-                  tma_load_4d(vd + hf * kHalf + x * a.box * 128, &vmap, hf * 64, w.h, bcol[x], bblk[x], vb, pol);
+            for (int x = 0; x < boxes; ++x) {
+              const bool none = pg.absent(a, w);
+              const int blk = none ? a.num_blocks : pg.blk;  // out of the tensor map: TMA fills zeros
+              if (do_k) {
+                const uint32_t bytes = C::kKV / boxes + (kFp8 && !none ? 2 * a.box : 0);  // the scales come with K
+                if (kFp8 && none) {  // zeros, of scale 1
+                  for (int i = 0; i < 2; ++i)
+                    for (int k = 0; k < a.box / 4; ++k)
+                      reinterpret_cast<uint32_t*>(&scales[st][i][x * a.box])[k] = 0x7f7f7f7fu;
+                  fence_async();  // before a later copy into the same bytes
+                }
+                if (x + 1 < boxes)
+                  mbar_expect_tx(kb, bytes);
                 else
-                  tma_load_4d_keep(vd + hf * kHalf + x * a.box * 128, &vmap, hf * 64, w.h, bcol[x], bblk[x], vb);
+                  mbar_arrive_expect_tx(kb, bytes);
+                if (kFp8 && !none) {
+                  const int64_t so = blk * a.scale_stride + (int64_t)w.h * a.block_size + pg.off;
+                  bulk_load(smem_u32(&scales[st][0][x * a.box]), a.ks + so, a.box, kb);
+                  bulk_load(smem_u32(&scales[st][1][x * a.box]), a.vs + so, a.box, kb);
+                }
+                load(&kmap, kd + x * a.box * 128, pg.off, blk, kb);
               }
+              if (do_v) {
+                if (x == 0) mbar_arrive_expect_tx(vb, C::kKV);
+                load(&vmap, vd + x * a.box * 128, pg.off, blk, vb);
+              }
+              pg.advance(a, w, a.box);
+            }
           }
         }
         // no copy may outlive the CTA: wait (bounded) for the last phase of every stage
         for (uint32_t i = it < C::kStages ? 0 : it - C::kStages; i < it; ++i) {
-          mbar_wait(smem_u32(&kfull[stage_of(i)]), phase_of(i), &g_err_tree);
-          mbar_wait(smem_u32(&vfull[stage_of(i)]), phase_of(i), &g_err_tree);
+          if (do_k) mbar_wait(smem_u32(&kfull[stage_of(i)]), phase_of(i), &g_err_tree);
+          if (do_v) mbar_wait(smem_u32(&vfull[stage_of(i)]), phase_of(i), &g_err_tree);
         }
       }
     } else if (warp == 1) {
       // ------------------------------------------------------------ MMA issuer
-      if (lane == 0) {
+      {
         // fp32 accumulation, M = N = 128. Q K^T: bf16, or e4m3 parts of Q; P V: bf16
         // or halves, V read head-dim-major (bit 16)
         constexpr uint32_t kShape = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
         constexpr uint32_t kBf16 = kFp8 ? 0u : (1u << 7) | (1u << 10);
         constexpr int kParts = kFp8 ? 2 : 1, kSteps = kFp8 ? 4 : 8;  // Q K^T: MMAs of 32 or 16 dims
-        uint32_t it = 0, seg = 0, done[2] = {0, 0}, outs[2] = {0, 0};  // tiles, segments; tiles and segments of each group
+        uint32_t it = 0, seg = 0, done[2] = {0, 0};                  // tiles, segments, tiles of each group so far
         bool ok = true;
         while (ok && w.next(a)) {
-          if (!mbar_wait(smem_u32(&q_full), seg & 1, &g_err_tree)) break;
-          ++seg;
-          // S of the group's next tile goes over P of its last: when that P V has ended
-          // (MMAs with different accumulators may run out of order)
-          const auto issue_s = [&](int j) -> bool {
-            const uint32_t i = it + j, st = stage_of(i), gr = j & 1, use = done[gr] + (j >> 1);
-            if (use > 0 && !mbar_wait(smem_u32(&pv_full[gr]), (use - 1) & 1, &g_err_tree)) return false;
-            if (!mbar_wait(smem_u32(&kfull[st]), phase_of(i), &g_err_tree)) return false;
-            tc::fence_after();
-            const uint32_t q = sbase + C::kQ, k = sbase + C::kRing + st * 2 * C::kKV;
+          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), seg & 1, &g_err_tree))) break;
+          // step j: S of tile j (its buffer: tile j - 2 has been weighed), then P V of tile j - 2
+          for (int j = 0; j < w.n + 2 && ok; ++j) {
+            if (j < w.n) {
+              const uint32_t i = it + j, st = stage_of(i), gr = j & 1, use = done[gr] + (j >> 1);
+              ok = (use == 0 || mbar_wait(smem_u32(&s_empty[gr]), (use - 1) & 1, &g_err_tree)) &&
+                   mbar_wait(smem_u32(&kfull[st]), phase_of(i), &g_err_tree);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tc::fence_after();
+              const uint64_t q = desc_k(sbase + C::kQ), k = desc_k(uniform(sbase + C::kRing + st * 2 * C::kKV));
+              const uint32_t d = uniform(tmem + gr * 128);
 #pragma unroll
-            for (int part = 0; part < kParts; ++part)
+              for (int part = 0; part < kParts; ++part)
 #pragma unroll
-              for (int ks = 0; ks < kSteps; ++ks) {
-                const uint32_t off = (kFp8 ? 0 : (ks >> 2) * kHalf) + (ks & 3) * 32;
-                mma<kFp8>(tmem + gr * 128, desc_k(q + part * kHalf + off), desc_k(k + off), kShape | kBf16,
-                          part > 0 || ks > 0);
-              }
-            commit(smem_u32(&s_full[gr]));
-            commit(smem_u32(&k_empty[st]));
-            return true;
-          };
-          ok = issue_s(0);
-          for (int j = 0; j < w.n && ok; ++j) {
-            if (j + 1 < w.n && !issue_s(j + 1)) {
-              ok = false;
-              break;
+                for (int ks = 0; ks < kSteps; ++ks) {
+                  // descriptors count 16 bytes
+                  const uint32_t off = ((kFp8 ? 0 : (ks >> 2) * kHalf) + (ks & 3) * 32) >> 4;
+                  mma<kFp8>(d, q + (part * kHalf >> 4) + off, k + off, kShape | kBf16, part > 0 || ks > 0);
+                }
+              commit(smem_u32(&s_full[gr]));
+              commit(smem_u32(&k_empty[st]));
             }
-            const uint32_t i = it + j, st = stage_of(i), gr = j & 1, use = done[gr] + (j >> 1);
-            ok = mbar_wait(smem_u32(kFp8 ? &v16_full[i & 1] : &vfull[st]), kFp8 ? (i >> 1) & 1 : phase_of(i), &g_err_tree) &&
-                 // a segment's first P V overwrites the output rows of the segment before
-                 (j >= 2 || outs[gr] == 0 || mbar_wait(smem_u32(&o_empty[gr]), (outs[gr] - 1) & 1, &g_err_tree)) &&
-                 mbar_wait(smem_u32(&p_full[gr]), use & 1, &g_err_tree);
-            if (!ok) break;
-            tc::fence_after();
-            const uint32_t v = sbase + (kFp8 ? C::kV16 + (i & 1) * kOperand : C::kRing + st * 2 * C::kKV + C::kKV);
+            if (j >= 2) {
+              const uint32_t i = it + j - 2, st = stage_of(i), gr = j & 1, use = done[gr] + (j >> 1) - 1;
+              ok = mbar_wait(smem_u32(kFp8 ? &v16_full[i & 1] : &vfull[st]), kFp8 ? (i >> 1) & 1 : phase_of(i), &g_err_tree) &&
+                   // a segment's first P V overwrites the output rows of the segment before
+                   (j > 2 || seg == 0 || mbar_wait(smem_u32(&o_empty), (seg - 1) & 1, &g_err_tree)) &&
+                   mbar_wait(smem_u32(&p_full[gr]), use & 1, &g_err_tree);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              tc::fence_after();
+              const uint64_t v =
+                  desc_mn(uniform(sbase + (kFp8 ? C::kV16 + (i & 1) * kOperand : C::kRing + st * 2 * C::kKV + C::kKV)), kHalf);
+              const uint32_t more = uniform(j > 2 || *reinterpret_cast<volatile uint32_t*>(&o_started));
+              const uint32_t d = uniform(tmem + kColO), p = uniform(tmem + kColP + gr * 64);
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-              mma_ts(tmem + (2 + gr) * 128, tmem + gr * 128 + ks * 8, desc_mn(v + ks * 2048, kHalf),
-                     kShape | kBf16 | (1u << 16), j >= 2 || ks > 0);
-            commit(smem_u32(&pv_full[gr]));
-            commit(smem_u32(kFp8 ? &v16_empty[i & 1] : &v_empty[st]));
+              for (int ks = 0; ks < 8; ++ks)
+                mma_ts(d, p + ks * 8, v + ks * (2048 >> 4), kShape | kBf16 | (1u << 16), ks > 0 ? 1u : more);
+              commit(smem_u32(&pv_full[gr]));
+              commit(smem_u32(kFp8 ? &v16_empty[i & 1] : &v_empty[st]));
+            }
           }
           it += w.n;
+          ++seg;
           done[0] += (w.n + 1) >> 1;
           done[1] += w.n >> 1;
-          outs[0] += 1;
-          outs[1] += w.n > 1;
         }
       }
     } else if (kFp8) {
@@ -462,8 +459,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int r = qd * 32 + lane;                    // query row of the unit = TMEM lane; token of a tile
     const int bar = 1 + gr;                          // the group's named barrier
     const uint32_t lane_base = tmem + ((uint32_t)(qd * 32) << 16);
-    const uint32_t srow = lane_base + gr * 128, orow = lane_base + (2 + gr) * 128;
-    uint32_t it = 0, use = 0;
+    const uint32_t srow = lane_base + gr * 128, orow = lane_base + kColO, prow = lane_base + kColP + gr * 64;
+    uint32_t it = 0, use = 0, other = 0;  // tiles of the CTA, of this group, of the other group in the segments before
     bool ok = true;
     while (w.next(a)) {
       const int base = w.s.len - w.s.nodes;
@@ -528,11 +525,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) mbar_arrive(smem_u32(&q_full));
 
       float m_ref = -INFINITY, l_run = 0.f;
-      // the group's output rows, when the P V of its last tile has ended
-      const auto wait_o = [&]() {
-        ok = ok && mbar_wait(smem_u32(&pv_full[gr]), (use - 1) & 1, &g_err_tree);
+      // until P V of this group's tile k, or the other group's, has ended
+      const auto wait_pv = [&](uint32_t k) {
+        ok = ok && mbar_wait(smem_u32(&pv_full[gr]), k & 1, &g_err_tree);
         tc::fence_after();
       };
+      const auto wait_pv_other = [&](uint32_t k) {
+        ok = ok && mbar_wait(smem_u32(&pv_full[gr ^ 1]), k & 1, &g_err_tree);
+        tc::fence_after();
+      };
+      const uint32_t use0 = use;
       for (int j = gr; j < w.n; j += 2) {
         const uint32_t i0 = it + j, st = stage_of(i0), tb = gr * 2 + (use & 1);
         const int p0 = (w.t0 + j) * kTile;
@@ -544,52 +546,72 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t kc = scales[st][0][r], vc = scales[st][1][r];
           float inv = __uint_as_float((254u - vc) << 23);
           if (tail && !(inv >= 0.f && inv < INFINITY)) inv = 0.f;  // stale scale bytes
-          tok_k[tb][r] = __uint_as_float(kc << 23);
-          tok_b[tb][r] = (float)((int)vc - 127);
-          tok_i[tb][r] = inv;
+          tok_k[tb][r] = __ushort_as_bfloat16((unsigned short)(kc << 7));
+          tok_b[tb][r] = __float2bfloat16_rn((float)((int)vc - 127));
+          tok_i[tb][r] = __float2bfloat16_rn(inv);
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&k_empty[st]));
           named_bar_sync(bar, 128);
         }
         ok = ok && mbar_wait(smem_u32(&s_full[gr]), use & 1, &g_err_tree);
         tc::fence_after();
-        float v[128];  // the row's scores, as powers of two
-        tmem_row(srow, v);
+        // first walk: the tile's scores, as powers of two (bf16: times the row's
+        // scale in the second walk), back to S where that saves the second walk
+        // something, and their maximum
         const uint64_t rs2 = pk2(rscale, rscale);
-#pragma unroll
-        for (int i = 0; i < 128; i += 4) {
-          uint64_t x = mul2(pk2(v[i], v[i + 1]), rs2), y = mul2(pk2(v[i + 2], v[i + 3]), rs2);
-          if constexpr (kFp8) {
-            const ulonglong2 k = *reinterpret_cast<const ulonglong2*>(&tok_k[tb][i]);
-            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&tok_b[tb][i]);
-            x = fma2(x, k.x, b.x);
-            y = fma2(y, k.y, b.y);
-          }
-          un2(x, v[i], v[i + 1]);
-          un2(y, v[i + 2], v[i + 3]);
-        }
-        if (tail) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t seen = in ? seen32(a, qrow, node, base, w.s.len, p0 + c * 32) : 0u;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[c * 32 + i] = (seen >> i) & 1u ? v[c * 32 + i] : -INFINITY;
-          }
-        }
+        const auto pair_of = [](uint32_t two) { return pk2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u)); };
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 64) {
+          float v[64];
+          tmem_row64(srow + c, v);
+          if constexpr (kFp8) {
 #pragma unroll
-        for (int i = 0; i < 128; i += 8)
+            for (int i = 0; i < 64; i += 8) {
+              const uint4 k = *reinterpret_cast<const uint4*>(&tok_k[tb][c + i]);
+              const uint4 b = *reinterpret_cast<const uint4*>(&tok_b[tb][c + i]);
+              const uint32_t kw[4] = {k.x, k.y, k.z, k.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-          for (int y = 0; y < 4; ++y) mx[y] = fmaxf(mx[y], fmaxf(v[i + 2 * y], v[i + 2 * y + 1]));
-        const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        const bool first = j < 2;
-        const bool move = first || m_tile > m_ref + kSlack;
+              for (int y = 0; y < 4; ++y) {
+                const uint64_t x = mul2(pk2(v[i + 2 * y], v[i + 2 * y + 1]), rs2);
+                un2(fma2(x, pair_of(kw[y]), pair_of(bw[y])), v[i + 2 * y], v[i + 2 * y + 1]);
+              }
+            }
+          }
+          if (tail) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t seen = in ? seen32(a, qrow, node, base, w.s.len, p0 + c + h * 32) : 0u;
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[h * 32 + i] = (seen >> i) & 1u ? v[h * 32 + i] : -INFINITY;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 64; i += 8)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) mx[y] = fmaxf(mx[y], fmaxf(v[i + 2 * y], v[i + 2 * y + 1]));
+          if (kFp8 || tail) {
+            tc::tmem_st32(srow + c, v);
+            tc::tmem_st32(srow + c + 32, v + 32);
+          }
+        }
+        float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        if (!kFp8) m_tile *= rscale;
+        // the row's reference, as the tile before left it
+        if (j > 0) {
+          named_bar_sync(4 + (gr ^ 1), kGroups * 128);
+          const float left = ref_s[r];
+          if (left != m_ref) {
+            l_run *= m_ref == -INFINITY ? 0.f : ex2(m_ref - left);  // keeps NaN
+            m_ref = left;
+          }
+        }
+        const bool move = j == 0 || m_tile > m_ref + kSlack;
         if (__any_sync(0xffffffffu, move)) {
           const float m_new = move ? fmaxf(m_ref, m_tile) : m_ref;
-          if (!first) {
+          if (j > 0) {
             const float corr = m_new == m_ref ? 1.f : ex2(m_ref - m_new);
-            wait_o();
-            // a few columns at a time: the scores stay in their registers
+            wait_pv_other(other + ((j + 1) >> 1) - 1);  // the tile before: P V run in order
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
               float y[16];
@@ -602,33 +624,52 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           m_ref = m_new;
         }
+        if (j + 1 < w.n) {
+          ref_s[r] = m_ref;
+          named_bar_arrive(4 + gr, kGroups * 128);
+        }
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+        if (use > use0) wait_pv(use - 1);  // this group's P was read by P V of its tile before
         uint64_t sum[4] = {0, 0, 0, 0};
         const uint64_t nref = pk2(-ref, -ref);
+        // second walk: the weights
+#pragma unroll 1
+        for (int c = 0; c < 128; c += 64) {
+          float v[64];
+          tmem_row64(srow + c, v);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t p[16];
+          for (int h = 0; h < 2; ++h) {
+            uint32_t p[16];
 #pragma unroll
-          for (int i = c * 32; i < c * 32 + 32; i += 4) {
-            un2(add2(pk2(v[i], v[i + 1]), nref), v[i], v[i + 1]);
-            un2(add2(pk2(v[i + 2], v[i + 3]), nref), v[i + 2], v[i + 3]);
+            for (int i = h * 32; i < h * 32 + 32; i += 8) {
+              uint64_t e[4];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) v[i + y] = ex2(v[i + y]);
-            const uint64_t x = pk2(v[i], v[i + 1]), y = pk2(v[i + 2], v[i + 3]);
-            const int sx = (i >> 1) & 2;
-            if constexpr (kFp8) {
-              const ulonglong2 n = *reinterpret_cast<const ulonglong2*>(&tok_i[tb][i]);
-              sum[sx] = fma2(x, n.x, sum[sx]);
-              sum[sx + 1] = fma2(y, n.y, sum[sx + 1]);
-            } else {
-              sum[sx] = add2(sum[sx], x);
-              sum[sx + 1] = add2(sum[sx + 1], y);
+              for (int y = 0; y < 4; ++y) {
+                const uint64_t s2 = pk2(v[i + 2 * y], v[i + 2 * y + 1]);
+                float x0, x1;
+                un2(kFp8 ? add2(s2, nref) : fma2(s2, rs2, nref), x0, x1);
+                x0 = ex2(x0);
+                x1 = ex2(x1);
+                p[(i & 31) / 2 + y] = kFp8 ? pack_half(x0, x1) : pack_bf16(x0, x1);
+                e[y] = pk2(x0, x1);
+              }
+              if constexpr (kFp8) {
+                const uint4 n = *reinterpret_cast<const uint4*>(&tok_i[tb][c + i]);
+                sum[0] = fma2(e[0], pair_of(n.x), sum[0]);
+                sum[1] = fma2(e[1], pair_of(n.y), sum[1]);
+                sum[2] = fma2(e[2], pair_of(n.z), sum[2]);
+                sum[3] = fma2(e[3], pair_of(n.w), sum[3]);
+              } else {
+#pragma unroll
+                for (int y = 0; y < 4; ++y) sum[y] = add2(sum[y], e[y]);
+              }
             }
-            p[(i & 31) / 2] = kFp8 ? pack_half(v[i], v[i + 1]) : pack_bf16(v[i], v[i + 1]);
-            p[(i & 31) / 2 + 1] = kFp8 ? pack_half(v[i + 2], v[i + 3]) : pack_bf16(v[i + 2], v[i + 3]);
+            tmem_put16(prow + c / 2 + h * 16, p);
           }
-          tmem_put16(srow + c * 16, p);
         }
+        tc::fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&s_empty[gr]));
         {
           const uint64_t x = add2(add2(sum[0], sum[1]), add2(sum[2], sum[3]));
           float s0, s1;
@@ -636,13 +677,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           l_run += s0 + s1;
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        bool any_odd = false;
         if (tail) {
           // Rows of V past the context hold stale bytes (possibly NaN), and drafted
           // rows may be hidden from some query rows: a zero weight does not cancel
           // NaN or infinities. Zero the former; take drafted rows that are not
-          // finite out of the tile and add their share, summed here row by row, when
-          // the tile's P V has ended.
+          // finite out of the tile and add their share, summed here row by row, to the
+          // output rows, before the tile's own P V.
           ok = ok && mbar_wait(smem_u32(kFp8 ? &v16_full[i0 & 1] : &vfull[st]), kFp8 ? (i0 >> 1) & 1 : phase_of(i0),
                                &g_err_tree);
           const uint32_t vt = sbase + (kFp8 ? C::kV16 + (i0 & 1) * kOperand : C::kRing + st * 2 * C::kKV + C::kKV);
@@ -657,18 +697,18 @@ __global__ void __launch_bounds__(kThreads, 1)
                       __vcmpeq2(x.w & ex, ex)) != 0;
             }
           }
-          any_odd = any_of_barrier(bar, 128, odd);
-          if (any_odd) {
+          if (any_of_barrier(bar, 128, odd)) {
             const uint32_t bits = __ballot_sync(0xffffffffu, odd);
             if (lane == 0) odd_bits[gr][qd] = bits;
             named_bar_sync(bar, 128);
+            float v[128];
 #pragma unroll
             for (int i = 0; i < kHD; ++i) v[i] = 0.f;
 #pragma unroll 1
             for (int t = 0; t < kTile; ++t) {
               if (!((odd_bits[gr][t >> 5] >> (t & 31)) & 1u)) continue;  // the same for the whole group
               const uint32_t seen = in ? seen32(a, qrow, node, base, w.s.len, p0 + (t & ~31)) : 0u;
-              const uint32_t two = tmem_ld1(srow + (t >> 1)) >> (t & 1 ? 16 : 0);
+              const uint32_t two = tmem_ld1(prow + (t >> 1)) >> (t & 1 ? 16 : 0);
               if ((seen >> (t & 31)) & 1u) {
                 const float p = kFp8 ? __half2float(__ushort_as_half((unsigned short)two)) : __uint_as_float(two << 16);
 #pragma unroll
@@ -686,6 +726,16 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
               __syncwarp();
             }
+            if (j > 0) wait_pv_other(other + ((j + 1) >> 1) - 1);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              float y[16];
+              if (j > 0) tc::tmem_ld16(orow + c * 16, y);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) y[i] = (j > 0 ? y[i] : 0.f) + v[c * 16 + i];
+              tc::tmem_st16(orow + c * 16, y);
+            }
+            if (j == 0 && r == 0) o_started = 1;
             named_bar_sync(bar, 128);
           }
           if (odd || p0 + r >= w.s.len) {
@@ -698,83 +748,54 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&p_full[gr]));
         ++use;
-        if (any_odd) {
-          wait_o();
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float y[16];
-            tc::tmem_ld16(orow + c * 16, y);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) y[i] += v[c * 16 + i];
-            tc::tmem_st16(orow + c * 16, y);
-          }
-          tc::fence_before();
-        }
+      }
+
+      // ------------------------------- the segment's rows: 64 dims for each group
+      const bool had_last = ((w.n - 1) & 1) == gr;
+      if (had_last) {
+        wait_pv(use - 1);
+        ref_s[r] = m_ref;
+      } else {
+        wait_pv_other(other + (gr == 0 ? w.n >> 1 : (w.n + 1) >> 1) - 1);
       }
       it += w.n;
-      const bool any = gr < w.n;
-      if (any) wait_o();
-      float o[128];  // the group's output rows (read in any case, so that no path leaves them without a value)
-      tmem_row(orow, o);
-      tc::fence_before();
-      __syncwarp();
-      if (any && lane == 0) mbar_arrive(smem_u32(&o_empty[gr]));
-
-      // ---------------------------------------------- join the two groups' tiles
-      if (!ok) m_ref = -INFINITY, l_run = 0.f;
-      named_bar_sync(3, kGroups * 128);  // both groups' MMAs are over: Q's memory is free
-      float f0 = 1.f, f1 = 0.f;
-      if (w.n > 1) {
-        // group 1 hands its rows over, 64 dims at a time
+      other += gr == 0 ? w.n >> 1 : (w.n + 1) >> 1;
+      named_bar_sync(3, kGroups * 128);  // every tile of both groups is done: Q's memory is free
+      const float m_end = ref_s[r];
+      l_s[gr][r] = l_run * (m_ref == -INFINITY ? 0.f : ex2(m_ref - m_end));  // keeps NaN
+      if (threadIdx.x == 128) o_started = 0;
+      float o[64];
+      {
+        float y[32];
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t row = sbase + C::kQ + r * 256;
-          if (gr == 1) {
-            if (half == 0) m_other[r] = m_ref, l_other[r] = l_run;
+        for (int c = 0; c < 2; ++c) {
+          tc::tmem_ld32(orow + gr * 64 + c * 32, y);
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              const float* x = o + half * 64 + 4 * c;
-              sts128(row + ((c ^ (r & 15)) << 4), __float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]),
-                     __float_as_uint(x[3]));
-            }
-          }
-          named_bar_sync(3, kGroups * 128);
-          if (gr == 0) {
-            if (half == 0) {
-              const float m1 = m_other[r], M = fmaxf(m_ref, m1);
-              f0 = m_ref == -INFINITY ? 0.f : ex2(m_ref - M);
-              f1 = m1 == -INFINITY ? 0.f : ex2(m1 - M);
-              l_run = l_run * f0 + l_other[r] * f1;
-              m_ref = M;
-            }
-#pragma unroll
-            for (int c = 0; c < 16; ++c) {
-              float* x = o + half * 64 + 4 * c;
-              const uint4 y = lds128(row + ((c ^ (r & 15)) << 4));
-              x[0] = x[0] * f0 + __uint_as_float(y.x) * f1;
-              x[1] = x[1] * f0 + __uint_as_float(y.y) * f1;
-              x[2] = x[2] * f0 + __uint_as_float(y.z) * f1;
-              x[3] = x[3] * f0 + __uint_as_float(y.w) * f1;
-            }
-          }
-          named_bar_sync(3, kGroups * 128);
+          for (int i = 0; i < 32; ++i) o[c * 32 + i] = y[i];
         }
       }
-      if (gr == 0 && in) {
+      tc::fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&o_empty));
+      named_bar_sync(3, kGroups * 128);
+      const float l_end = ok ? l_s[0][r] + l_s[1][r] : 0.f;
+      if (in) {
         if (w.whole()) {
-          const float inv = l_run == 0.f ? 0.f : 1.f / l_run;  // nothing seen: 0
-          uint4* op = reinterpret_cast<uint4*>(a.out + (int64_t)qrow * a.o_st + (int64_t)head * a.o_sh);
+          const float inv = l_end == 0.f ? 0.f : 1.f / l_end;  // nothing seen: 0
+          uint4* op = reinterpret_cast<uint4*>(a.out + (int64_t)qrow * a.o_st + (int64_t)head * a.o_sh + gr * 64);
 #pragma unroll
-          for (int c = 0; c < 16; ++c)
+          for (int c = 0; c < 8; ++c)
             op[c] = make_uint4(pack_bf16(o[8 * c] * inv, o[8 * c + 1] * inv), pack_bf16(o[8 * c + 2] * inv, o[8 * c + 3] * inv),
                                pack_bf16(o[8 * c + 4] * inv, o[8 * c + 5] * inv), pack_bf16(o[8 * c + 6] * inv, o[8 * c + 7] * inv));
         } else {
           const int64_t pr = ((int64_t)blockIdx.x * 2 + w.slot()) * kRows + r;
-          float4* dst = reinterpret_cast<float4*>(a.part_o + pr * kHD);
+          float4* dst = reinterpret_cast<float4*>(a.part_o + pr * kHD + gr * 64);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) dst[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
-          a.part_m[pr] = m_ref;
-          a.part_l[pr] = l_run;
+          for (int c = 0; c < 16; ++c) dst[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+          if (gr == 0) {
+            a.part_m[pr] = ok ? m_end : -INFINITY;
+            a.part_l[pr] = l_end;
+          }
         }
       }
     }

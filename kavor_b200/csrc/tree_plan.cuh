@@ -168,6 +168,38 @@ struct Walk {
   __device__ __forceinline__ int slot() const { return t0 > 0 ? 0 : 1; }
 };
 
+// A sequence's pages in order: the page of the current tokens and, loaded ahead,
+// the next one (a table entry takes hundreds of cycles to arrive).
+struct Pages {
+  int col, off;   // page and token in it
+  int blk, next;  // block ids; -1 past the context
+
+  __device__ __forceinline__ static int entry(const Args& a, const Walk& w, int col) {
+    return (int64_t)col * a.block_size < w.s.len ? a.tables[(int64_t)w.b * a.bt_stride + col] : -1;
+  }
+  __device__ __forceinline__ void start(const Args& a, const Walk& w, int token) {
+    col = token / a.block_size;
+    off = token - col * a.block_size;
+    blk = entry(a, w, col);
+    next = entry(a, w, col + 1);
+  }
+  __device__ __forceinline__ void advance(const Args& a, const Walk& w, int tokens) {  // tokens divide a page
+    off += tokens;
+    if (off >= a.block_size) {
+      off = 0;
+      ++col;
+      blk = next;
+      next = entry(a, w, col + 1);
+    }
+  }
+  // Nothing to read: past the context, or a block id outside the pool, which raises the error bit.
+  __device__ __forceinline__ bool absent(const Args& a, const Walk& w) const {
+    if (blk >= 0 && blk < a.num_blocks) return false;
+    if ((int64_t)col * a.block_size < w.s.len) atomicOr(&g_err_tree, (unsigned)kErrBlockTable);
+    return true;
+  }
+};
+
 // Does node i of a sequence see node j?
 __device__ __forceinline__ bool sees(const Args& a, int row, int i, int j) {
   if (!a.mask) return j <= i;
