@@ -212,6 +212,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
           }
         }
       }
+      w.leave(a);
       // no copy may outlive the CTA: wait (bounded) for the last phase of every stage
       for (uint32_t i = it < C::kStages ? 0 : it - C::kStages; i < it; ++i)
         mbar_wait(smem_u32(&full_bar[i % C::kStages]), (i / C::kStages) & 1, &g_err_tree);
@@ -649,11 +650,11 @@ namespace kvb {
 namespace {
 
 // ------------------------------------------------------------------- merge
-// Joins the partials of units that were cut between CTAs, in an order that does
+// Joins the pieces of units that were cut between CTAs, in an order that does
 // not depend on timing, and writes zeros for sequences with an empty context.
-// Rows whose unit was whole have been written already. A warp takes a row of a
-// few partials; the eight warps of a block share a row of many.
+// Rows whose unit was whole have been written already.
 constexpr int kMergeWarps = 8;
+constexpr int kMergeCtas = 5;  // blocks an SM holds
 constexpr int kFew = 16;
 
 struct Joined {
@@ -671,8 +672,8 @@ __device__ __forceinline__ void join(Joined& x, float m, float l, const float4& 
   x.o.w = x.o.w * f0 + o.w * f1;
   x.m = m_new;
 }
-// Parts c0 + k, k = k0, k0 + step, .. < n of a row; loads of four parts in flight.
-__device__ __forceinline__ Joined join_parts(const Args& a, int c0, int n, int k0, int step, int row, int lane) {
+// Pieces k0, k0 + step, .. < n of four dims of a row, from part p on; loads of four in flight.
+__device__ __forceinline__ Joined join_parts(const Args& a, int p, int n, int k0, int step, int row, int chunk) {
   Joined x = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
   for (int k = k0; k < n; k += 4 * step) {
     float m[4], l[4];
@@ -685,10 +686,10 @@ __device__ __forceinline__ Joined join_parts(const Args& a, int c0, int n, int k
       o[u] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (kk < n) {
         // the unit's first part holds its beginning (slot 1), the others follow on (slot 0)
-        const int64_t pr = ((int64_t)(c0 + kk) * 2 + (kk == 0)) * a.heads * a.rows + row;
+        const int64_t first = ((int64_t)(p + kk) * 2 + (kk == 0)) * a.heads * a.rows, pr = first + row;
         m[u] = a.part_m[pr];
         l[u] = a.part_l[pr];
-        o[u] = *reinterpret_cast<const float4*>(a.part_o + pr * kHD + lane * 4);
+        o[u] = reinterpret_cast<const float4*>(a.part_o)[a.by_dims ? first * 32 + (int64_t)chunk * a.rows + row : pr * 32 + chunk];
       }
     }
 #pragma unroll
@@ -697,62 +698,54 @@ __device__ __forceinline__ Joined join_parts(const Args& a, int c0, int n, int k
   return x;
 }
 
-__global__ void __launch_bounds__(kMergeWarps * 32) tree_merge_kernel(const __grid_constant__ Args a, int rows_per_block) {
+// Only the cut units are looked at, at most one a part: a block has some parts
+// (blockIdx.x, at most 32) and takes eight rows of each unit (blockIdx.y), or, when
+// it has many pieces, its warps share a warp's part of those rows (a row's four
+// dims a thread). A warp for every query row of the batch,
+// finding its pieces from prefix sums, took 40 us for 64 x 1024 rows of which a
+// fifth was cut; this takes 12.
+__global__ void __launch_bounds__(kMergeWarps * 32, kMergeCtas) tree_merge_kernel(const __grid_constant__ Args a) {
   kernel_entry();
   __shared__ Joined s_join[kMergeWarps][32];
-  const int b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const tree::Seq s = tree::seq_of(a, b, false);
-  const int64_t rows = (int64_t)s.nodes * a.hq;  // fits 31 bits: the host checked total_q * hq
-  const int64_t first = a.first[b], range = tree::range_of(a.first[a.batch], a.parts);
-  for (int64_t i0 = (int64_t)blockIdx.x * rows_per_block; i0 < rows; i0 += (int64_t)gridDim.x * rows_per_block) {
-    // where the parts of row i are
-    int c0 = 0, n = 0, row = 0;
-    bf16* op = nullptr;
-    const auto locate = [&](int64_t i) {
-      const int nd = (int)i / a.hq, head = (int)i - nd * a.hq, h = head / a.group;
-      op = a.out + (int64_t)(s.q0 + nd) * a.o_st + (int64_t)head * a.o_sh + lane * 4;
-      if (s.tiles == 0) {
-        n = 0;
-        return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int mine = blockIdx.x + lane * gridDim.x;
+  uint32_t cut = __ballot_sync(0xffffffffu, mine < a.parts && a.cuts[mine].n != 0);
+  for (; cut; cut &= cut - 1) {
+    const int part = blockIdx.x + (__ffs(cut) - 1) * gridDim.x;
+    const tree::Cut c = a.cuts[part];
+    const bool many = c.n > kFew;
+    const int items = ((a.heads * c.rows + 7) >> 3) * (many ? 8 : 1);
+    for (int item = blockIdx.y; item < items; item += gridDim.y) {
+      const int group = many ? item >> 3 : item, eighth = many ? item & 7 : warp;
+      const int f = group * 8 + (a.by_dims ? lane & 7 : eighth);  // row of the unit, its heads one after another
+      const int head = f / c.rows, r = f - head * c.rows;
+      const int chunk = a.by_dims ? eighth * 4 + (lane >> 3) : lane;
+      const int n = head < a.heads ? c.n : 0;
+      Joined x = join_parts(a, part, n, many ? warp : 0, many ? kMergeWarps : 1, head * a.rows + r, chunk);
+      if (many) {
+        s_join[warp][lane] = x;
+        __syncthreads();
       }
-      const int R = nd * a.group + head - h * a.group, rb = R / a.rows;
-      const int hg = h / a.heads;
-      row = (h - hg * a.heads) * a.rows + R - rb * a.rows;
-      const int64_t lo = first + ((int64_t)hg * s.blocks + rb) * s.tiles;
-      const int64_t hi = lo + s.tiles - 1;
-      if (hi <= UINT32_MAX) {  // nearly always: a 64-bit division takes ten times as long
-        c0 = (int)((uint32_t)lo / (uint32_t)range);
-        n = (int)((uint32_t)hi / (uint32_t)range) - c0 + 1;
-      } else {
-        c0 = (int)(lo / range);
-        n = (int)(hi / range) - c0 + 1;
-      }
-    };
-    const auto write = [&](const Joined& x) {
-      const float inv = x.l == 0.f ? 0.f : 1.f / x.l;
-      *reinterpret_cast<uint2*>(op) =
-          make_uint2(pack_bf16(x.o.x * inv, x.o.y * inv), pack_bf16(x.o.z * inv, x.o.w * inv));
-    };
-    const int mine = min((int64_t)rows_per_block, rows - i0);
-    if (warp < mine) {
-      locate(i0 + warp);
-      if (n == 0)
-        *reinterpret_cast<uint2*>(op) = make_uint2(0u, 0u);
-      else if (n > 1 && n <= kFew)
-        write(join_parts(a, c0, n, 0, 1, row, lane));
-    }
-    if (!__syncthreads_or(n > kFew)) continue;
-    for (int r = 0; r < mine; ++r) {
-      locate(i0 + r);
-      if (n <= kFew) continue;  // the same for the whole block
-      s_join[warp][lane] = join_parts(a, c0, n, warp, kMergeWarps, row, lane);
-      __syncthreads();
-      if (warp == 0) {
-        Joined x = s_join[0][lane];
+      if (many && warp == 0)
         for (int w = 1; w < kMergeWarps; ++w) join(x, s_join[w][lane].m, s_join[w][lane].l, s_join[w][lane].o);
-        write(x);
+      if (n > 0 && (!many || warp == 0)) {
+        const float inv = x.l == 0.f ? 0.f : 1.f / x.l;
+        const int R = c.row0 + r, nd = R / a.group;
+        *reinterpret_cast<uint2*>(a.out + (int64_t)(c.q0 + nd) * a.o_st +
+                                  (int64_t)((c.h + head) * a.group + R - nd * a.group) * a.o_sh + chunk * 4) =
+            make_uint2(pack_bf16(x.o.x * inv, x.o.y * inv), pack_bf16(x.o.z * inv, x.o.w * inv));
       }
-      __syncthreads();
+      if (many) __syncthreads();  // before the next item's s_join
+    }
+  }
+  for (int b = blockIdx.y * gridDim.x + blockIdx.x; b < a.batch; b += gridDim.x * gridDim.y) {
+    const tree::Seq s = tree::seq_of(a, b, false);
+    if (s.tiles) continue;
+    const int64_t chunks = (int64_t)s.nodes * a.hq * 32;
+    for (int64_t i = threadIdx.x; i < chunks; i += kMergeWarps * 32) {
+      const int row = (int)(i >> 5), nd = row / a.hq;
+      *reinterpret_cast<uint2*>(a.out + (int64_t)(s.q0 + nd) * a.o_st + (int64_t)(row - nd * a.hq) * a.o_sh + (i & 31) * 4) =
+          make_uint2(0u, 0u);
     }
   }
 }
@@ -794,7 +787,7 @@ void fill(Variant* v) {
   v->parts = C::kCtas * device_sm_count();  // what the SMs hold: one wave
 }
 
-Variant variant_for(bool fp8, int batch, int hq, int hkv, int max_nodes, int block_size) {
+Variant variant_for(bool fp8, int hq, int hkv, int max_nodes, int block_size) {
   Variant v;
   const int64_t rows = (int64_t)(hq / hkv) * max_nodes;
   const bool few = rows <= 8;
@@ -814,7 +807,7 @@ Variant variant_for(bool fp8, int batch, int hq, int hkv, int max_nodes, int blo
   else
     few ? fill<true, 1, 1>(&v) : fill<true, 2, 1>(&v);
   v.box = block_size % v.tile == 0 ? v.tile : 64;
-  v.workspace = (size_t)v.parts * 2 * v.heads * v.rows * (kHD + 2) * sizeof(float) + ((size_t)batch + 2) * sizeof(int64_t);
+  v.workspace = (size_t)v.parts * 2 * v.heads * v.rows * (kHD + 2) * sizeof(float) + (size_t)v.parts * sizeof(tree::Cut);
   return v;
 }
 
@@ -861,8 +854,8 @@ extern "C" int kvb_tree_attn_workspace_size(int batch, int num_q_heads, int num_
   if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_seqlen_q < 0)
     return set_error(kInvalid, "kvb_tree_attn_workspace_size: bad sizes");
   // the larger of the two cache types' needs (the block size does not matter)
-  const size_t a = variant_for(false, batch, num_q_heads, num_kv_heads, max_seqlen_q, 256).workspace;
-  const size_t b = variant_for(true, batch, num_q_heads, num_kv_heads, max_seqlen_q, 256).workspace;
+  const size_t a = variant_for(false, num_q_heads, num_kv_heads, max_seqlen_q, 256).workspace;
+  const size_t b = variant_for(true, num_q_heads, num_kv_heads, max_seqlen_q, 256).workspace;
   *bytes = a > b ? a : b;
   return kOk;
 }
@@ -904,8 +897,9 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   if (!(scale > 0.f) || scale > 1e30f) return set_error(kInvalid, "kvb_tree_attn: scale must be positive and finite");
 
   Args a = {};
-  const Variant v = variant_for(fp8, batch, num_q_heads, num_kv_heads, max_seqlen_q, block_size);
+  const Variant v = variant_for(fp8, num_q_heads, num_kv_heads, max_seqlen_q, block_size);
   a.rows = v.rows;
+  a.by_dims = v.nt == 0;
   a.heads = v.heads;
   a.tile = v.tile;
   a.box = v.box;
@@ -939,8 +933,8 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   a.group = num_q_heads / num_kv_heads;
   a.num_blocks = (int)num_blocks;
   a.block_size = block_size;
-  a.first = (int64_t*)workspace;
-  a.part_o = (float*)workspace + (((size_t)batch + 1) * 2 + 3) / 4 * 4;  // 16-byte aligned behind the prefix sums
+  a.cuts = (tree::Cut*)workspace;
+  a.part_o = (float*)(a.cuts + a.parts);
   a.part_m = a.part_o + (size_t)a.parts * 2 * a.heads * a.rows * kHD;
   a.part_l = a.part_m + (size_t)a.parts * 2 * a.heads * a.rows;
   a.scale_log2 = scale * 1.4426950408889634f;
@@ -962,11 +956,15 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   else
     rc = v.nt == 1 ? launch_warp<true, 1, 1>(km, vm, a, st) : launch_warp<true, 2, 1>(km, vm, a, st);
   if (rc) return rc;
-  // rows of many partials come with few rows in all: a block each then
-  const int64_t mrows = (int64_t)max_seqlen_q * num_q_heads;
-  const int rpb = mrows * batch <= 8 * device_sm_count() ? 1 : kMergeWarps;
-  const int64_t mblocks = (mrows + rpb - 1) / rpb;
-  return cuda_status(launch_kernel(tree_merge_kernel, dim3((unsigned)(mblocks < 8192 ? mblocks : 8192), (unsigned)batch),
-                                   dim3(kMergeWarps * 32), 0, st, a, rpb),
+  // a block for each eight rows of a part's cut unit; where units are few and so cut in many pieces, a block for
+  // each eighth of that and fewer parts a block, to have one wave
+  const int64_t unit_rows = (int64_t)a.group * max_seqlen_q, blocks = (unit_rows + v.rows - 1) / v.rows;
+  const int64_t units = (int64_t)batch * (num_kv_heads / v.heads) * blocks;
+  const int eights = (int)((v.heads * (unit_rows < v.rows ? unit_rows : v.rows) + 7) / 8);
+  const bool few = units * kFew <= v.parts;
+  const int y = few ? eights * 8 : eights;
+  const int wave = kMergeCtas * device_sm_count() / y, least = (v.parts + 31) / 32;
+  const int x = !few || wave >= v.parts ? v.parts : wave > least ? wave : least;
+  return cuda_status(launch_kernel(tree_merge_kernel, dim3((unsigned)x, (unsigned)y), dim3(kMergeWarps * 32), 0, st, a),
                      "kvb_tree_attn merge launch");
 }

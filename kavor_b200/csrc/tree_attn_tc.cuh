@@ -30,15 +30,17 @@ namespace tcore {
 constexpr int kRows = 128;
 constexpr int kTile = 128;
 constexpr int kGroups = 2;                                // softmax warpgroups
-constexpr int kThreads = 128 + kGroups * 128;             // warp 0 TMA, 1 MMA + TMEM, 2 and 3 convert V
-// Registers: 168 a thread at launch (384 threads); the control warps give theirs
-// up for the softmax threads' output rows: 128 (56 + 2 * 224) = 384 * 168.
-constexpr int kControlRegs = 56, kSoftmaxRegs = 224;
 constexpr uint32_t kCols = 512;                           // S0, S1, O: 128 columns each; P0, P1: 64
 constexpr uint32_t kColO = 256, kColP = 384;
 constexpr float kSlack = 15.f;                            // log2 of the largest weight: below the largest half
 constexpr int kHalf = kTile * 128;                        // 128 rows of 128 bytes
 constexpr int kOperand = 2 * kHalf;                       // 16-bit Q or V (two halves of 64 dims), or two e4m3 parts of Q
+// Warps 0 and 2 load K and V, 1 issues Q K^T, 3 issues P V, 4 to 7 load Q and
+// convert V of an e4m3 cache; then the softmax groups.
+constexpr int kFirst = 8, kThreads = kFirst * 32 + kGroups * 128;
+// Registers: 128 a thread at launch; the other warps give theirs up for the
+// softmax threads: 128 (2 * 48 + 2 * 208) = 512 * 128.
+constexpr int kOtherRegs = 48, kSoftmaxRegs = 208;
 template <bool kFp8>
 struct Cfg {
   static constexpr int kKV = kTile * kHD * (kFp8 ? 1 : 2);
@@ -151,6 +153,11 @@ __device__ __forceinline__ void tmem_put16(uint32_t taddr, const uint32_t (&r)[1
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
+// 16 bytes to shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // Packed fp32 pairs.
 __device__ __forceinline__ uint64_t pk2(float a, float b) {
   uint64_t r;
@@ -231,12 +238,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   using C = Cfg<kFp8>;
   kernel_entry();
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t q_full, kfull[C::kStages], vfull[C::kStages], k_empty[C::kStages], v_empty[C::kStages],
+  __shared__ __align__(8) uint64_t q_full, q_empty, kfull[C::kStages], vfull[C::kStages], k_empty[C::kStages], v_empty[C::kStages],
       v16_full[2], v16_empty[2], s_full[2], s_empty[2], p_full[2], pv_full[2], o_empty;
   __shared__ __align__(16) uint8_t scales[kFp8 ? C::kStages : 1][2][kTile];
   // scales 2^a (K) and 2^b (V) of a tile: 2^a, b and 2^-b, exact in bf16; two tiles of each group
   __shared__ __align__(16) bf16 tok_k[kFp8 ? 4 : 1][kTile], tok_b[kFp8 ? 4 : 1][kTile], tok_i[kFp8 ? 4 : 1][kTile];
   __shared__ float ref_s[kRows], l_s[2][kRows];
+  __shared__ float qs_s[kFp8 ? 4 : 1][kRows];  // scale of a query row's e4m3 parts, of four segments
   __shared__ uint32_t o_started;  // the output rows hold something before a segment's first P V
   __shared__ uint32_t odd_bits[2][4];
   __shared__ uint32_t tmem_s;
@@ -245,15 +253,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
   if (threadIdx.x == 0) {
-    mbar_init(smem_u32(&q_full), kGroups * 4);
+    mbar_init(smem_u32(&q_full), 4);
+    mbar_init(smem_u32(&q_empty), 1);
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(smem_u32(&kfull[i]), 1);
       mbar_init(smem_u32(&vfull[i]), 1);
       mbar_init(smem_u32(&k_empty[i]), kFp8 ? 5 : 1);  // the MMAs; the four warps that read the tile's scales
-      mbar_init(smem_u32(&v_empty[i]), kFp8 ? 2 : 1);  // the converting warps, or the MMAs
+      mbar_init(smem_u32(&v_empty[i]), kFp8 ? 4 : 1);  // the converting warps, or the MMAs
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&v16_full[i]), 2);
+      mbar_init(smem_u32(&v16_full[i]), 4);
       mbar_init(smem_u32(&v16_empty[i]), 1);
       mbar_init(smem_u32(&s_full[i]), 1);
       mbar_init(smem_u32(&s_empty[i]), 4);
@@ -279,13 +288,13 @@ __global__ void __launch_bounds__(kThreads, 1)
   const auto stage_of = [](uint32_t i) { return i % C::kStages; };
   const auto phase_of = [](uint32_t i) { return (i / C::kStages) & 1; };
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kControlRegs));
-    if (warp == 0 || (!kFp8 && warp == 2)) {
-      // --------------------------------------------------------- TMA producers
-      // Warp 0 loads K and the e4m3 rows of V; bf16 rows of V, whose buffers are
-      // held until their P V has ended, have warp 2 for themselves.
-      const bool do_k = warp == 0, do_v = kFp8 || warp == 2;
+  if (warp < kFirst) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 0 || warp == 2) {
+      // ------------------------------------------------- TMA producers, K and V
+      // (in one thread, K waited behind V's buffers, which are held until P V has
+      // ended: 16 x 64 nodes over bf16 took 367 us, apart 337)
+      const bool do_k = warp == 0, do_v = warp == 2;
       if (lane == 0) {
         prefetch_tensormap(do_k ? &kmap : &vmap);
         const uint64_t pol = l2_evict_first_policy();
@@ -343,88 +352,150 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
+        if (do_k) w.leave(a);
         // no copy may outlive the CTA: wait (bounded) for the last phase of every stage
         for (uint32_t i = it < C::kStages ? 0 : it - C::kStages; i < it; ++i) {
           if (do_k) mbar_wait(smem_u32(&kfull[stage_of(i)]), phase_of(i), &g_err_tree);
           if (do_v) mbar_wait(smem_u32(&vfull[stage_of(i)]), phase_of(i), &g_err_tree);
         }
       }
-    } else if (warp == 1) {
-      // ------------------------------------------------------------ MMA issuer
-      {
-        // fp32 accumulation, M = N = 128. Q K^T: bf16, or e4m3 parts of Q; P V: bf16
-        // or halves, V read head-dim-major (bit 16)
-        constexpr uint32_t kShape = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-        constexpr uint32_t kBf16 = kFp8 ? 0u : (1u << 7) | (1u << 10);
-        constexpr int kParts = kFp8 ? 2 : 1, kSteps = kFp8 ? 4 : 8;  // Q K^T: MMAs of 32 or 16 dims
-        uint32_t it = 0, seg = 0, done[2] = {0, 0};                  // tiles, segments, tiles of each group so far
-        bool ok = true;
-        while (ok && w.next(a)) {
-          if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), seg & 1, &g_err_tree))) break;
-          // step j: S of tile j (its buffer: tile j - 2 has been weighed), then P V of tile j - 2
-          for (int j = 0; j < w.n + 2 && ok; ++j) {
-            if (j < w.n) {
-              const uint32_t i = it + j, st = stage_of(i), gr = j & 1, use = done[gr] + (j >> 1);
-              ok = (use == 0 || mbar_wait(smem_u32(&s_empty[gr]), (use - 1) & 1, &g_err_tree)) &&
-                   mbar_wait(smem_u32(&kfull[st]), phase_of(i), &g_err_tree);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              tc::fence_after();
-              const uint64_t q = desc_k(sbase + C::kQ), k = desc_k(uniform(sbase + C::kRing + st * 2 * C::kKV));
-              const uint32_t d = uniform(tmem + gr * 128);
+    } else if (warp == 1 || warp == 3) {
+      // ----------------------------------------------------------- MMA issuers
+      // fp32 accumulation, M = N = 128. Q K^T: bf16, or e4m3 parts of Q; P V: bf16
+      // or halves, V read head-dim-major (bit 16). A warp for each, so that neither
+      // waits behind what the other waits for.
+      constexpr uint32_t kShape = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+      constexpr uint32_t kBf16 = kFp8 ? 0u : (1u << 7) | (1u << 10);
+      constexpr int kParts = kFp8 ? 2 : 1, kSteps = kFp8 ? 4 : 8;  // Q K^T: MMAs of 32 or 16 dims
+      uint32_t it = 0, seg = 0, done[2] = {0, 0};                  // tiles, segments, tiles of each group so far
+      bool ok = true;
+      while (ok && w.next(a)) {
+        if (warp == 1 && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), seg & 1, &g_err_tree))) break;
+        for (int j = 0; j < w.n; ++j) {
+          const uint32_t i = it + j, st = stage_of(i), gr = j & 1, use = done[gr] + (j >> 1);
+          if (warp == 1) {  // S, once the tile before in its buffer has been weighed
+            ok = (use == 0 || mbar_wait(smem_u32(&s_empty[gr]), (use - 1) & 1, &g_err_tree)) &&
+                 mbar_wait(smem_u32(&kfull[st]), phase_of(i), &g_err_tree);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc::fence_after();
+            const uint64_t q = desc_k(sbase + C::kQ), k = desc_k(uniform(sbase + C::kRing + st * 2 * C::kKV));
+            const uint32_t d = uniform(tmem + gr * 128);
 #pragma unroll
-              for (int part = 0; part < kParts; ++part)
+            for (int part = 0; part < kParts; ++part)
 #pragma unroll
-                for (int ks = 0; ks < kSteps; ++ks) {
-                  // descriptors count 16 bytes
-                  const uint32_t off = ((kFp8 ? 0 : (ks >> 2) * kHalf) + (ks & 3) * 32) >> 4;
-                  mma<kFp8>(d, q + (part * kHalf >> 4) + off, k + off, kShape | kBf16, part > 0 || ks > 0);
-                }
-              commit(smem_u32(&s_full[gr]));
-              commit(smem_u32(&k_empty[st]));
-            }
-            if (j >= 2) {
-              const uint32_t i = it + j - 2, st = stage_of(i), gr = j & 1, use = done[gr] + (j >> 1) - 1;
-              ok = mbar_wait(smem_u32(kFp8 ? &v16_full[i & 1] : &vfull[st]), kFp8 ? (i >> 1) & 1 : phase_of(i), &g_err_tree) &&
-                   // a segment's first P V overwrites the output rows of the segment before
-                   (j > 2 || seg == 0 || mbar_wait(smem_u32(&o_empty), (seg - 1) & 1, &g_err_tree)) &&
-                   mbar_wait(smem_u32(&p_full[gr]), use & 1, &g_err_tree);
-              ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
-              tc::fence_after();
-              const uint64_t v =
-                  desc_mn(uniform(sbase + (kFp8 ? C::kV16 + (i & 1) * kOperand : C::kRing + st * 2 * C::kKV + C::kKV)), kHalf);
-              const uint32_t more = uniform(j > 2 || *reinterpret_cast<volatile uint32_t*>(&o_started));
-              const uint32_t d = uniform(tmem + kColO), p = uniform(tmem + kColP + gr * 64);
+              for (int ks = 0; ks < kSteps; ++ks) {
+                // descriptors count 16 bytes
+                const uint32_t off = ((kFp8 ? 0 : (ks >> 2) * kHalf) + (ks & 3) * 32) >> 4;
+                mma<kFp8>(d, q + (part * kHalf >> 4) + off, k + off, kShape | kBf16, part > 0 || ks > 0);
+              }
+            commit(smem_u32(&k_empty[st]));
+            if (j == w.n - 1) commit(smem_u32(&q_empty));
+            commit(smem_u32(&s_full[gr]));
+          } else {
+            ok = mbar_wait(smem_u32(kFp8 ? &v16_full[i & 1] : &vfull[st]), kFp8 ? (i >> 1) & 1 : phase_of(i), &g_err_tree) &&
+                 // a segment's first P V overwrites the output rows of the segment before
+                 (j > 0 || seg == 0 || mbar_wait(smem_u32(&o_empty), (seg - 1) & 1, &g_err_tree)) &&
+                 mbar_wait(smem_u32(&p_full[gr]), use & 1, &g_err_tree);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            tc::fence_after();
+            const uint64_t v =
+                desc_mn(uniform(sbase + (kFp8 ? C::kV16 + (i & 1) * kOperand : C::kRing + st * 2 * C::kKV + C::kKV)), kHalf);
+            const uint32_t more = uniform(j > 0 || *reinterpret_cast<volatile uint32_t*>(&o_started));
+            const uint32_t d = uniform(tmem + kColO), p = uniform(tmem + kColP + gr * 64);
 #pragma unroll
-              for (int ks = 0; ks < 8; ++ks)
-                mma_ts(d, p + ks * 8, v + ks * (2048 >> 4), kShape | kBf16 | (1u << 16), ks > 0 ? 1u : more);
-              commit(smem_u32(&pv_full[gr]));
-              commit(smem_u32(kFp8 ? &v16_empty[i & 1] : &v_empty[st]));
-            }
+            for (int ks = 0; ks < 8; ++ks)
+              mma_ts(d, p + ks * 8, v + ks * (2048 >> 4), kShape | kBf16 | (1u << 16), ks > 0 ? 1u : more);
+            commit(smem_u32(kFp8 ? &v16_empty[i & 1] : &v_empty[st]));
+            commit(smem_u32(&pv_full[gr]));
           }
-          it += w.n;
-          ++seg;
-          done[0] += (w.n + 1) >> 1;
-          done[1] += w.n >> 1;
         }
+        it += w.n;
+        ++seg;
+        done[0] += (w.n + 1) >> 1;
+        done[1] += w.n >> 1;
       }
-    } else if (kFp8) {
-      // ------------------------------------------- V's e4m3 bytes to halves
+    } else {
+      // ------------------------------------- query rows; V's e4m3 bytes to halves
       uint32_t it = 0;
       bool ok = true;
-      const int t2 = threadIdx.x - 64;
-      while (w.next(a)) {
-        for (int j = 0; j < w.n; ++j, ++it) {
+      const int t2 = threadIdx.x - 128;
+      for (uint32_t seg = 0; w.next(a); ++seg) {
+        // half a warp a row, rows 8 apart, once the last segment's Q K^T has read
+        // the rows before. (Read by the softmax threads, each its row, a segment
+        // began 20,000 to 27,000 cycles after the last tile of the one before.)
+        ok = ok && (seg == 0 || mbar_wait(smem_u32(&q_empty), (seg - 1) & 1, &g_err_tree));
+        const int c = t2 & 15;
+#pragma unroll 1
+        for (int r0 = t2 >> 4; r0 < kRows; r0 += 32) {
+          uint4 x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint32_t R = w.rb * kRows + r0 + i * 8, node = R / (uint32_t)a.group;
+            const int head = w.h * a.group + (int)(R - node * a.group);
+            const bool in = node < (uint32_t)w.s.nodes;
+            const bf16* src = a.q + (int64_t)(w.s.q0 + (in ? node : 0)) * a.q_st + (int64_t)head * a.q_sh + c * 8;
+            if constexpr (kFp8) {
+              x[i] = make_uint4(0u, 0u, 0u, 0u);
+              if (in) x[i] = *reinterpret_cast<const uint4*>(src);
+            } else {
+              const int row = r0 + i * 8;
+              copy16(sbase + C::kQ + (c >> 3) * kHalf + row * 128 + (((c & 7) ^ (row & 7)) << 4), src, in);
+            }
+          }
+          if constexpr (kFp8) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = r0 + i * 8;
+              const uint32_t wd[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+              uint32_t mx = 0, inf = 0;
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const uint32_t z = wd[y] & 0x7fff7fffu, big = __vcmpgtu2(z, 0x7f7f7f7fu);
+                inf |= big;
+                mx = __vmaxu2(mx, z & ~big);
+              }
+              mx = max(mx & 0xffffu, mx >> 16);
+#pragma unroll
+              for (int o = 1; o < 16; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+              const bool odd = (__ballot_sync(0xffffffffu, inf != 0) >> (lane & 16) & 0xffffu) != 0;
+              const int e = min(max((int)(mx >> 7) - 127 - 7, -100), 100);  // the largest to [128, 256)
+              const float inv = pow2(-e);
+              float f[8];
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wd[y]));
+                f[2 * y] = v.x * inv;
+                f[2 * y + 1] = v.y * inv;
+              }
+              uint2 hi, lo;
+              split4(f, hi.x, lo.x);
+              split4(f + 4, hi.y, lo.y);
+              uint8_t* at = smem + C::kQ + row * 128 + (((c >> 1) ^ (row & 7)) << 4) + (c & 1) * 8;
+              *reinterpret_cast<uint2*>(at) = hi;
+              *reinterpret_cast<uint2*>(at + kHalf) = lo;
+              // A row with NaN or an infinity gives NaN. The softmax threads have this by S,
+              // those of segment seg - 4 are done: the Q K^T of seg - 1 that ended waited for
+              // a tile of seg - 2, weighed after the barrier at the end of seg - 3
+              if (c == 0) qs_s[seg & 3][row] = odd ? NAN : a.scale_log2 * pow2(e);
+            }
+          }
+        }
+        if constexpr (!kFp8) copies_done();
+        fence_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&q_full));
+        for (int j = 0; kFp8 && j < w.n; ++j, ++it) {
           const uint32_t st = stage_of(it), buf = it & 1;
           ok = ok && mbar_wait(smem_u32(&vfull[st]), phase_of(it), &g_err_tree) &&
                (it < 2 || mbar_wait(smem_u32(&v16_empty[buf]), ((it >> 1) - 1) & 1, &g_err_tree));
           if (!ok) continue;
           const uint32_t src = sbase + C::kRing + st * 2 * C::kKV + C::kKV, dst = sbase + C::kV16 + buf * kOperand;
 #pragma unroll 4
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 8; ++i) {
             // 16 dims (chunk c) of token t: two 8-dim chunks of its row's half c / 4
-            const int idx = i * 64 + t2, t = idx >> 3, c = idx & 7;
+            const int idx = i * 128 + t2, t = idx >> 3, c = idx & 7;
             const uint4 x = lds128(src + t * 128 + ((c ^ (t & 7)) << 4));
             uint32_t y[8];
             e4m3x4_to_half(x.x, y[0], y[1]);
@@ -454,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------ softmax groups
     // A wait that gave up (its error bit is set) is not followed by others, and the
     // group goes on with what is there: its barriers stay matched, its rows are dropped.
-    const int gr = (warp - 4) >> 2;                  // group: tiles of its parity
+    const int gr = (warp - kFirst) >> 2;                  // group: tiles of its parity
     const int qd = warp & 3;                         // TMEM lane quarter of this warp
     const int r = qd * 32 + lane;                    // query row of the unit = TMEM lane; token of a tile
     const int bar = 1 + gr;                          // the group's named barrier
@@ -462,67 +533,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t srow = lane_base + gr * 128, orow = lane_base + kColO, prow = lane_base + kColP + gr * 64;
     uint32_t it = 0, use = 0, other = 0;  // tiles of the CTA, of this group, of the other group in the segments before
     bool ok = true;
-    while (w.next(a)) {
+    uint32_t seg = 0;
+    for (; w.next(a); ++seg) {
       const int base = w.s.len - w.s.nodes;
       const int R = w.rb * kRows + r, node = R / a.group;
       const bool in = node < w.s.nodes;
       const int qrow = w.s.q0 + (in ? node : 0);
       const int head = w.h * a.group + (in ? R - node * a.group : 0);
-      // -------- this thread's query row to shared memory: its half of the dims
       float rscale = a.scale_log2;
-      {
-        const uint4* qp = reinterpret_cast<const uint4*>(a.q + (int64_t)qrow * a.q_st + (int64_t)head * a.q_sh);
-        const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (kFp8) {
-          uint32_t mx = 0;
-          bool finite = true;
-#pragma unroll
-          for (int c = 0; c < 16; ++c) {
-            const uint4 x = in ? qp[c] : zero;
-            const uint32_t wd[4] = {x.x & 0x7fff7fffu, x.y & 0x7fff7fffu, x.z & 0x7fff7fffu, x.w & 0x7fff7fffu};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const uint32_t inf = __vcmpgtu2(wd[i], 0x7f7f7f7fu);
-              finite &= inf == 0;
-              mx = __vmaxu2(mx, wd[i] & ~inf);
-            }
-          }
-          mx = max(mx & 0xffffu, mx >> 16);
-          const int e = min(max((int)(mx >> 7) - 127 - 7, -100), 100);  // the largest to [128, 256)
-          const float inv = pow2(-e);
-          rscale = finite ? a.scale_log2 * pow2(e) : NAN;  // a row with NaN or an infinity gives NaN
-#pragma unroll 1
-          for (int c = gr * 8; c < gr * 8 + 8; c += 2) {
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-              const uint4 x = in ? qp[c + y] : zero;
-              const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x);
-              float f[8];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const float2 v = __bfloat1622float2(h[i]);
-                f[2 * i] = v.x * inv;
-                f[2 * i + 1] = v.y * inv;
-              }
-              split4(f, hi[2 * y], lo[2 * y]);
-              split4(f + 4, hi[2 * y + 1], lo[2 * y + 1]);
-            }
-            const uint32_t at = sbase + C::kQ + r * 128 + (((c >> 1) ^ (r & 7)) << 4);
-            sts128(at, hi[0], hi[1], hi[2], hi[3]);
-            sts128(at + kHalf, lo[0], lo[1], lo[2], lo[3]);
-          }
-        } else {
-#pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            const uint4 x = in ? qp[gr * 8 + c] : zero;
-            sts128(sbase + C::kQ + gr * kHalf + r * 128 + ((c ^ (r & 7)) << 4), x.x, x.y, x.z, x.w);
-          }
-        }
-      }
-      fence_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&q_full));
 
       float m_ref = -INFINITY, l_run = 0.f;
       // until P V of this group's tile k, or the other group's, has ended
@@ -555,6 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         ok = ok && mbar_wait(smem_u32(&s_full[gr]), use & 1, &g_err_tree);
         tc::fence_after();
+        if constexpr (kFp8) rscale = qs_s[seg & 3][r];
         // first walk: the tile's scores, as powers of two (bf16: times the row's
         // scale in the second walk), back to S where that saves the second walk
         // something, and their maximum
@@ -752,18 +771,18 @@ __global__ void __launch_bounds__(kThreads, 1)
 
       // ------------------------------- the segment's rows: 64 dims for each group
       const bool had_last = ((w.n - 1) & 1) == gr;
+      other += gr == 0 ? w.n >> 1 : (w.n + 1) >> 1;
       if (had_last) {
         wait_pv(use - 1);
         ref_s[r] = m_ref;
       } else {
-        wait_pv_other(other + (gr == 0 ? w.n >> 1 : (w.n + 1) >> 1) - 1);
+        wait_pv_other(other - 1);
       }
       it += w.n;
-      other += gr == 0 ? w.n >> 1 : (w.n + 1) >> 1;
-      named_bar_sync(3, kGroups * 128);  // every tile of both groups is done: Q's memory is free
+      named_bar_sync(3, kGroups * 128);  // every tile of both groups is done
       const float m_end = ref_s[r];
       l_s[gr][r] = l_run * (m_ref == -INFINITY ? 0.f : ex2(m_ref - m_end));  // keeps NaN
-      if (threadIdx.x == 128) o_started = 0;
+      if (threadIdx.x == kFirst * 32) o_started = 0;
       float o[64];
       {
         float y[32];
@@ -789,9 +808,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                                pack_bf16(o[8 * c + 4] * inv, o[8 * c + 5] * inv), pack_bf16(o[8 * c + 6] * inv, o[8 * c + 7] * inv));
         } else {
           const int64_t pr = ((int64_t)blockIdx.x * 2 + w.slot()) * kRows + r;
-          float4* dst = reinterpret_cast<float4*>(a.part_o + pr * kHD + gr * 64);
+          // four dims of 128 rows together: a warp's stores fill whole lines
+          float4* dst = reinterpret_cast<float4*>(a.part_o + (pr - r) * kHD) + gr * 16 * kRows + r;
 #pragma unroll
-          for (int c = 0; c < 16; ++c) dst[c] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
+          for (int c = 0; c < 16; ++c)
+            dst[c * kRows] = make_float4(o[4 * c], o[4 * c + 1], o[4 * c + 2], o[4 * c + 3]);
           if (gr == 0) {
             a.part_m[pr] = ok ? m_end : -INFINITY;
             a.part_l[pr] = l_end;

@@ -40,11 +40,20 @@ struct Args {
   int heads;              // kv heads of a unit
   int parts, rows, tile;  // CTAs of the attention grid, query rows of a unit and head, tokens of a tile
   int box;                // tokens of a TMA box: a tile's, or a page's when that is smaller
+  int by_dims;            // partials by dims: [parts][2][32][rows][4] (heads = 1)
   float* part_o;          // [parts][2][heads][rows][128]
   float* part_m;          // [parts][2][heads][rows]
   float* part_l;
-  int64_t* first;         // [batch + 1]: tiles before each sequence, written for the merge
+  struct Cut* cuts;       // [parts]: the unit each part leaves unfinished, written for the merge
   float scale_log2;
+};
+
+// A unit that begins in a part and goes on in the next ones.
+struct alignas(16) Cut {
+  int n;         // parts that hold a piece of it; 0: no such unit
+  int rows;      // its query rows for each head
+  int q0, row0;  // first query row of the sequence, the unit's first row (nodes x heads of a kv head)
+  int h, pad[3];
 };
 
 struct Seq {
@@ -104,8 +113,7 @@ __device__ __forceinline__ int64_t block_prefix(int64_t mine, int64_t* total) {
 __device__ __forceinline__ int64_t range_of(int64_t total, int parts) { return (total + parts - 1) / parts; }
 
 // Where this CTA's range starts: the sequence, the offset in its tiles, and
-// how many tiles the range has. Every thread of the block calls it; block 0
-// leaves the line's prefix sums for the merge.
+// how many tiles the range has. Every thread of the block calls it.
 struct Start {
   int b;
   int64_t off, left;
@@ -122,14 +130,12 @@ __device__ __forceinline__ Start find_start(const Args& a, int part) {
   const int64_t range = range_of(total, a.parts), lo = range * part, hi = min(lo + range, total);
   if (threadIdx.x == 0) s_start = Start{0, 0, 0};
   __syncthreads();
-  if (part == 0 || (lo < hi && at <= lo && lo < at + mine)) {
+  if (lo < hi && at <= lo && lo < at + mine) {
     for (int b = b0; b < b1; ++b) {
       const int64_t c = cost_of(a, seq_of(a, b, false));
-      if (part == 0) a.first[b] = at;
-      if (at <= lo && lo < min(at + c, hi)) s_start = Start{b, lo - at, hi - lo};
+      if (at <= lo && lo < at + c) s_start = Start{b, lo - at, hi - lo};
       at += c;
     }
-    if (part == 0 && threadIdx.x == 0) a.first[a.batch] = total;
   }
   __syncthreads();
   return s_start;
@@ -138,11 +144,11 @@ __device__ __forceinline__ Start find_start(const Args& a, int part) {
 // Walks a range segment by segment; a segment is the part of one unit inside it.
 struct Walk {
   int b;
-  int64_t off, left;
+  int64_t off, left, range;
   Seq s;
   int h, rb, t0, n;  // first kv head, row block, first tile, tiles
 
-  __device__ __forceinline__ Walk(const Args& a, const Start& st) : b(st.b), off(st.off), left(st.left) {
+  __device__ __forceinline__ Walk(const Args& a, const Start& st) : b(st.b), off(st.off), left(st.left), range(st.left), t0(1) {
     if (left > 0) s = seq_of(a, b, false);
   }
   __device__ __forceinline__ bool next(const Args& a) {
@@ -152,9 +158,16 @@ struct Walk {
       if (++b >= a.batch) return false;
       s = seq_of(a, b, false);
     }
-    const int64_t u = off / s.tiles;
+    int64_t u;
+    int hg;
+    if (off <= UINT32_MAX) {  // nearly always: a 64-bit division takes ten times as long
+      u = (uint32_t)off / (uint32_t)s.tiles;
+      hg = (int)((uint32_t)u / (uint32_t)s.blocks);
+    } else {
+      u = off / s.tiles;
+      hg = (int)(u / s.blocks);
+    }
     t0 = (int)(off - u * s.tiles);
-    const int hg = (int)(u / s.blocks);
     h = hg * a.heads;
     rb = (int)(u - (int64_t)hg * s.blocks);
     const int64_t room = s.tiles - t0;
@@ -164,6 +177,18 @@ struct Walk {
     return true;
   }
   __device__ __forceinline__ bool whole() const { return t0 == 0 && n == s.tiles; }
+  // After the last segment, by one thread of the part.
+  __device__ __forceinline__ void leave(const Args& a) const {
+    Cut c = {};
+    if (t0 == 0 && n < s.tiles) {  // a range that ends inside a unit is a full one
+      c.n = 1 + (int)((s.tiles - n + range - 1) / range);
+      c.row0 = rb * a.rows;
+      c.rows = min(a.rows, s.nodes * a.group - c.row0);
+      c.q0 = s.q0;
+      c.h = h;
+    }
+    a.cuts[blockIdx.x] = c;
+  }
   // partial slot of a cut segment: 0 when the unit began in an earlier CTA
   __device__ __forceinline__ int slot() const { return t0 > 0 ? 0 : 1; }
 };
