@@ -39,8 +39,8 @@ constexpr int kOperand = 2 * kHalf;                       // 16-bit Q or V (two 
 // convert V of an e4m3 cache; then the softmax groups.
 constexpr int kFirst = 8, kThreads = kFirst * 32 + kGroups * 128;
 // Registers: 128 a thread at launch; the other warps give theirs up for the
-// softmax threads: 128 (2 * 48 + 2 * 208) = 512 * 128.
-constexpr int kOtherRegs = 48, kSoftmaxRegs = 208;
+// softmax threads: 128 (2 * 64 + 2 * 192) = 512 * 128.
+constexpr int kOtherRegs = 64, kSoftmaxRegs = 192;
 template <bool kFp8>
 struct Cfg {
   static constexpr int kKV = kTile * kHD * (kFp8 ? 1 : 2);
@@ -571,6 +571,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (lane == 0) mbar_arrive(smem_u32(&k_empty[st]));
           named_bar_sync(bar, 128);
         }
+        uint32_t seen[4];
+        if (tail)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) seen[i] = in ? seen32(a, qrow, node, base, w.s.len, p0 + i * 32) : 0u;
         ok = ok && mbar_wait(smem_u32(&s_full[gr]), use & 1, &g_err_tree);
         tc::fence_after();
         if constexpr (kFp8) rscale = qs_s[seg & 3][r];
@@ -600,9 +604,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (tail) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t seen = in ? seen32(a, qrow, node, base, w.s.len, p0 + c + h * 32) : 0u;
+              const uint32_t bits = c == 0 ? seen[h] : seen[2 + h];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[h * 32 + i] = (seen >> i) & 1u ? v[h * 32 + i] : -INFINITY;
+              for (int i = 0; i < 32; ++i) v[h * 32 + i] = (bits >> i) & 1u ? v[h * 32 + i] : -INFINITY;
             }
           }
 #pragma unroll
@@ -708,9 +712,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t vr = vt + r * 128;
           bool odd = false;
           if (p0 + r >= base && p0 + r < w.s.len) {
-#pragma unroll 1
+#pragma unroll 4
             for (int c = 0; c < 16; ++c) {
-              const uint4 x = lds128(vr + (c >> 3) * kHalf + ((c & 7) << 4));  // any order: the whole row is looked at
+              // the whole row is looked at, so any order will do: one that starts each lane on other banks
+              const int k = (c + r) & 15;
+              const uint4 x = lds128(vr + (k >> 3) * kHalf + ((k & 7) << 4));
               const uint32_t ex = kFp8 ? 0x7c007c00u : 0x7f807f80u;
               odd |= (__vcmpeq2(x.x & ex, ex) | __vcmpeq2(x.y & ex, ex) | __vcmpeq2(x.z & ex, ex) |
                       __vcmpeq2(x.w & ex, ex)) != 0;
@@ -726,9 +732,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll 1
             for (int t = 0; t < kTile; ++t) {
               if (!((odd_bits[gr][t >> 5] >> (t & 31)) & 1u)) continue;  // the same for the whole group
-              const uint32_t seen = in ? seen32(a, qrow, node, base, w.s.len, p0 + (t & ~31)) : 0u;
+              const uint32_t bits = t < 64 ? t < 32 ? seen[0] : seen[1] : t < 96 ? seen[2] : seen[3];
               const uint32_t two = tmem_ld1(prow + (t >> 1)) >> (t & 1 ? 16 : 0);
-              if ((seen >> (t & 31)) & 1u) {
+              if ((bits >> (t & 31)) & 1u) {
                 const float p = kFp8 ? __half2float(__ushort_as_half((unsigned short)two)) : __uint_as_float(two << 16);
 #pragma unroll
                 for (int c = 0; c < 16; ++c) {
@@ -758,8 +764,11 @@ __global__ void __launch_bounds__(kThreads, 1)
             named_bar_sync(bar, 128);
           }
           if (odd || p0 + r >= w.s.len) {
-#pragma unroll
-            for (int c = 0; c < 16; ++c) sts128(vr + (c >> 3) * kHalf + ((c & 7) << 4), 0u, 0u, 0u, 0u);
+#pragma unroll 4
+            for (int c = 0; c < 16; ++c) {
+              const int k = (c + r) & 15;
+              sts128(vr + (k >> 3) * kHalf + ((k & 7) << 4), 0u, 0u, 0u, 0u);
+            }
           }
           fence_async();
         }
