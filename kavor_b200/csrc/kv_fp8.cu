@@ -29,6 +29,10 @@ constexpr int kHD = 128;
 constexpr int kThreads = 256;
 constexpr int kRowLanes = 16;
 constexpr int kRowsPerBlock = kThreads / kRowLanes;
+// The write gives a lane two 16-byte pieces of a row, 64 values apart: what is done
+// once a row and lane is most of its instructions (16 lanes a row: 21.7 us, this 18.5
+// for 16384 tokens of 8 heads).
+constexpr int kStoreLanes = 8, kStoreRows = kThreads / kStoreLanes;
 
 struct CacheRef {
   uint8_t* k;
@@ -39,6 +43,30 @@ struct CacheRef {
   int block_size, hkv;
 };
 
+// n / d for 0 <= n < 2^31 by one multiplication: with 2^(s-1) < d <= 2^s and mul =
+// ceil(2^(31+s) / d), n mul / 2^(31+s) exceeds n / d by less than n / 2^(31+s) <
+// 2^-s <= 1 / d, so the whole parts agree. (The rows' and slots' divisions were a
+// third of the write's instructions.)
+struct Divisor {
+  uint32_t mul;
+  int shift;
+  explicit Divisor(int d) {
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    shift = 31 + s;
+    mul = (uint32_t)(((1ull << shift) + (uint64_t)d - 1) / (uint64_t)d);
+  }
+  __device__ __forceinline__ int divide(int n) const { return (int)((uint64_t)(uint32_t)n * mul >> shift); }
+};
+
+// Largest magnitudes of 8 bf16 values of k (low half) and of v, infinities and NaN
+// included: the largest finite ones where no infinity or NaN is among them.
+__device__ __forceinline__ uint32_t max8_of_two(const uint4& k, const uint4& v) {
+  constexpr uint32_t m = 0x7fff7fffu;
+  const uint32_t a = __vmaxu2(__vmaxu2(k.x & m, k.y & m), __vmaxu2(k.z & m, k.w & m));
+  const uint32_t b = __vmaxu2(__vmaxu2(v.x & m, v.y & m), __vmaxu2(v.z & m, v.w & m));
+  return __vmaxu2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+}
 // Largest finite magnitude of 8 bf16 values, as bf16 bits: for positive
 // floats the order of the bits is the order of the values.
 __device__ __forceinline__ uint32_t finite_max8(const uint4& r) {
@@ -58,46 +86,54 @@ __device__ __forceinline__ int scale_exponent(uint32_t bits) {
   return max(e, -100);
 }
 
+// bf16 pairs times 2^-e to four e4m3 bytes.
+__device__ __forceinline__ uint32_t quantise4(uint32_t lo, uint32_t hi, float inv) {
+  const float2 a = make_float2(__uint_as_float(lo << 16) * inv, __uint_as_float(lo & 0xffff0000u) * inv);
+  const float2 b = make_float2(__uint_as_float(hi << 16) * inv, __uint_as_float(hi & 0xffff0000u) * inv);
+  return __byte_perm(__nv_cvt_float2_to_fp8x2(a, __NV_SATFINITE, __NV_E4M3),
+                     __nv_cvt_float2_to_fp8x2(b, __NV_SATFINITE, __NV_E4M3), 0x5410);
+}
 __device__ __forceinline__ uint2 quantise8(const uint4& r, int e) {
   const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
-  uint32_t q[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float2 f = __bfloat1622float2(h[i]);
-    f.x *= inv;
-    f.y *= inv;
-    q[i] = __nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
-  }
-  return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+  return make_uint2(quantise4(r.x, r.y, inv), quantise4(r.z, r.w, inv));
 }
 
 __global__ void __launch_bounds__(kThreads)
     store_kv_fp8_kernel(const bf16* __restrict__ key, int64_t k_st, int64_t k_sh, const bf16* __restrict__ value,
-                        int64_t v_st, int64_t v_sh, CacheRef c, const int32_t* __restrict__ slots, int64_t rows) {
+                        int64_t v_st, int64_t v_sh, CacheRef c, Divisor by_heads, Divisor by_block,
+                        const int32_t* __restrict__ slots, int rows) {
   kernel_entry();
-  const int64_t row = (int64_t)blockIdx.x * kRowsPerBlock + threadIdx.x / kRowLanes;
-  const int lane = threadIdx.x % kRowLanes;
-  const int64_t rr = row < rows ? row : rows - 1;  // every lane takes part in the shuffles
-  const int64_t t = rr / c.hkv;
-  const int h = (int)(rr - t * c.hkv);
+  const int64_t row = (int64_t)blockIdx.x * kStoreRows + threadIdx.x / kStoreLanes;
+  const int lane = threadIdx.x % kStoreLanes;
+  const int rr = row < rows ? (int)row : rows - 1;  // every lane takes part in the shuffles
+  const int t = by_heads.divide(rr), h = rr - t * c.hkv;
   const int32_t slot = slots[t];
-  const uint4 kr = *reinterpret_cast<const uint4*>(key + t * k_st + h * k_sh + lane * 8);
-  const uint4 vr = *reinterpret_cast<const uint4*>(value + t * v_st + h * v_sh + lane * 8);
-  uint32_t mx = finite_max8(kr) | finite_max8(vr) << 16;
+  const uint4* kp = reinterpret_cast<const uint4*>(key + t * k_st + h * k_sh) + lane;
+  const uint4* vp = reinterpret_cast<const uint4*>(value + t * v_st + h * v_sh) + lane;
+  const uint4 k0 = kp[0], k1 = kp[kStoreLanes], v0 = vp[0], v1 = vp[kStoreLanes];
+  uint32_t mx = __vmaxu2(max8_of_two(k0, v0), max8_of_two(k1, v1));
 #pragma unroll
-  for (int o = kRowLanes / 2; o > 0; o >>= 1) mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  for (int o = kStoreLanes / 2; o > 0; o >>= 1) mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  if (__any_sync(0xffffffffu, (mx & 0xffffu) > 0x7f7fu || mx > 0x7f7fffffu)) {  // rare: an infinity or NaN in the warp's rows
+    mx = max(finite_max8(k0), finite_max8(k1)) | max(finite_max8(v0), finite_max8(v1)) << 16;
+#pragma unroll
+    for (int o = kStoreLanes / 2; o > 0; o >>= 1) mx = __vmaxu2(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  }
   if (row >= rows || slot == -1) return;
   if (slot < 0 || slot >= c.num_blocks * c.block_size) {
     if (lane == 0) atomicOr(&g_err_kv_fp8, (unsigned)kErrSlot);
     return;
   }
-  const int64_t blk = slot / c.block_size;
-  const int off = slot - (int)(blk * c.block_size);
+  const int64_t blk = by_block.divide(slot);
+  const int off = slot - (int)blk * c.block_size;
   const int ek = scale_exponent(mx & 0xffffu), ev = scale_exponent(mx >> 16);
-  const int64_t at = blk * c.block_stride + ((int64_t)off * c.hkv + h) * kHD + lane * 8;
-  *reinterpret_cast<uint2*>(c.k + at) = quantise8(kr, ek);
-  *reinterpret_cast<uint2*>(c.v + at) = quantise8(vr, ev);
+  const int64_t at = blk * c.block_stride + ((int64_t)off * c.hkv + h) * kHD;
+  uint2* kd = reinterpret_cast<uint2*>(c.k + at) + lane;
+  uint2* vd = reinterpret_cast<uint2*>(c.v + at) + lane;
+  kd[0] = quantise8(k0, ek);
+  kd[kStoreLanes] = quantise8(k1, ek);
+  vd[0] = quantise8(v0, ev);
+  vd[kStoreLanes] = quantise8(v1, ev);
   if (lane < 2) {
     const int64_t sat = blk * c.scale_stride + (int64_t)h * c.block_size + off;
     (lane == 0 ? c.ks : c.vs)[sat] = (uint8_t)((lane == 0 ? ek : ev) + 127);
@@ -210,11 +246,11 @@ extern "C" int kvb_store_kv_fp8(const void* key, int64_t key_stride_t, int64_t k
       value_stride_h % 8)
     return set_error(kInvalid, "kvb_store_kv_fp8: key/value rows must be 16-byte aligned");
   const int64_t rows = (int64_t)num_tokens * num_kv_heads;
-  const int64_t grid = (rows + kRowsPerBlock - 1) / kRowsPerBlock;
-  if (grid > INT32_MAX) return set_error(kUnsupported, "kvb_store_kv_fp8: too many rows");
+  if (rows > INT32_MAX) return set_error(kUnsupported, "kvb_store_kv_fp8: more than 2^31 rows");
+  const int64_t grid = (rows + kStoreRows - 1) / kStoreRows;
   return cuda_status(launch_kernel(store_kv_fp8_kernel, dim3((unsigned)grid), dim3(kThreads), 0, (cudaStream_t)stream,
                                    (const bf16*)key, key_stride_t, key_stride_h, (const bf16*)value, value_stride_t,
-                                   value_stride_h, c, slot_mapping, rows),
+                                   value_stride_h, c, Divisor(num_kv_heads), Divisor(block_size), slot_mapping, (int)rows),
                      "kvb_store_kv_fp8 launch");
 }
 
