@@ -49,13 +49,16 @@ struct Vec<float> {
   static __device__ __forceinline__ uint32_t floor_word(uint32_t w) {
     return __float_as_uint(fmaxf(__uint_as_float(w), kFloor));
   }
-  static __device__ __forceinline__ float max(const uint4& r) {
-    float a, b;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(__uint_as_float(r.x)), "f"(__uint_as_float(r.y)));
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(b) : "f"(__uint_as_float(r.z)), "f"(__uint_as_float(r.w)));
-    asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(b));
-    return a;
+  // the largest entry, NaN if there is one
+  static __device__ __forceinline__ uint32_t larger(uint32_t x, uint32_t y) {
+    float a;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(a) : "f"(__uint_as_float(x)), "f"(__uint_as_float(y)));
+    return __float_as_uint(a);
   }
+  static __device__ __forceinline__ float value(uint32_t x) { return __uint_as_float(x); }
+  // a bound, and whether an entry reaches it (NaN does)
+  static __device__ __forceinline__ uint32_t bound(float x) { return __float_as_uint(x); }
+  static __device__ __forceinline__ bool reaches(uint32_t x, uint32_t b) { return !(value(x) < value(b)); }
   static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
     v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
   }
@@ -86,14 +89,25 @@ struct Vec<bf16> {
     asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xfe96fe96u));
     return r;
   }
-  static __device__ __forceinline__ float max(const uint4& r) {
-    uint32_t a, b;
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(r.x), "r"(r.y));
-    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(b) : "r"(r.z), "r"(r.w));
-    asm("max.NaN.bf16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
-    float hi = __uint_as_float(a & 0xffff0000u), lo = __uint_as_float(a << 16);
+  // of two entries each, the larger ones in their halves; NaN if there is one
+  static __device__ __forceinline__ uint32_t larger(uint32_t x, uint32_t y) {
+    uint32_t a;
+    asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(a) : "r"(x), "r"(y));
+    return a;
+  }
+  static __device__ __forceinline__ float value(uint32_t x) {
+    float hi = __uint_as_float(x & 0xffff0000u), lo = __uint_as_float(x << 16);
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(lo));
     return hi;
+  }
+  static __device__ __forceinline__ uint32_t bound(float x) {  // never above x
+    const uint32_t h = __bfloat16_as_ushort(__float2bfloat16_rd(x));
+    return h | h << 16;
+  }
+  static __device__ __forceinline__ bool reaches(uint32_t x, uint32_t b) {
+    uint32_t r;
+    asm("{\n\t.reg .pred p, q;\n\tsetp.geu.bf16x2 p|q, %1, %2;\n\tor.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : "r"(x), "r"(b));
+    return r != 0;
   }
   static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -122,14 +136,25 @@ struct Vec<__half> {
     asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(w), "r"(0xfbfffbffu));
     return r;
   }
-  static __device__ __forceinline__ float max(const uint4& r) {
-    uint32_t a, b;
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(r.x), "r"(r.y));
-    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(b) : "r"(r.z), "r"(r.w));
-    asm("max.NaN.f16x2 %0, %0, %1;" : "+r"(a) : "r"(b));
-    float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a));
+  // of two entries each, the larger ones in their halves; NaN if there is one
+  static __device__ __forceinline__ uint32_t larger(uint32_t x, uint32_t y) {
+    uint32_t a;
+    asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(a) : "r"(x), "r"(y));
+    return a;
+  }
+  static __device__ __forceinline__ float value(uint32_t x) {
+    float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(f.x) : "f"(f.y));
     return f.x;
+  }
+  static __device__ __forceinline__ uint32_t bound(float x) {  // never above x
+    const uint32_t h = __half_as_ushort(__float2half_rd(x));
+    return h | h << 16;
+  }
+  static __device__ __forceinline__ bool reaches(uint32_t x, uint32_t b) {
+    uint32_t r;
+    asm("{\n\t.reg .pred p, q;\n\tsetp.geu.f16x2 p|q, %1, %2;\n\tor.pred p, p, q;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r) : "r"(x), "r"(b));
+    return r != 0;
   }
   static __device__ __forceinline__ void unpack(const uint4& r, float* v) {
     const __half2* h = reinterpret_cast<const __half2*>(&r);
@@ -149,6 +174,12 @@ struct Vec<__half> {
                     : count_masks(__hgtu2_mask(h[0], tt), __hgtu2_mask(h[1], tt), __hgtu2_mask(h[2], tt), __hgtu2_mask(h[3], tt));
   }
 };
+
+// A vector's largest entry, as larger() leaves it.
+template <typename T>
+__device__ __forceinline__ uint32_t largest(const uint4& r) {
+  return Vec<T>::larger(Vec<T>::larger(r.x, r.y), Vec<T>::larger(r.z, r.w));
+}
 
 // ------------------------------------------------------------------- order
 // Whole number whose order is the order of the logits: NaN highest, -0 = +0.
@@ -383,7 +414,7 @@ __device__ __forceinline__ float block_bound(Shared& sh, float m, int k) {
 template <typename T>
 __device__ __noinline__ void collect(Shared& sh, const Part<T>& p, float thr) {
   for (int v = p.v0 + threadIdx.x; v < p.v1; v += kThreads)
-    if (!(Vec<T>::max(p.body[v]) < thr)) note(sh, v);
+    if (!(Vec<T>::value(largest<T>(p.body[v])) < thr)) note(sh, v);
 }
 
 // The entries at or above thr of the first n noted vectors, and of the edges, go to the list.
@@ -588,73 +619,91 @@ __global__ void __launch_bounds__(kThreads, 4)
   const uint64_t L2 = pk2(kLog2e, kLog2e);
   Sums s;
   unsigned ahead = 0;
-  float thr = INFINITY, bound = -INFINITY;  // bound: least entry that needs a second look
+  float thr = INFINITY;  // least entry that may be among the top ones
   const float t_bound = !has ? INFINITY : t != t ? -INFINITY : t;
   uint32_t marks[4] = {0u, 0u, 0u, 0u};  // vectors of this thread that reach thr
-  const auto take = [&](const uint4& raw, float vm, int v) {
-    if (!(vm < bound)) {
-      if (!(vm <= s.lim)) s.move(vm, Vec<T>::kFloor);
-      bound = fminf(s.lim, t_bound);
-      const int i = head + v * N;
-      if (v < v1) {
-        if (has && !(vm < t)) {
-          // a vector before the token counts its ties, one after it does not
-          if (t == t && i + N <= tok)
-            ahead += Vec<T>::template above<true>(raw, t);
-          else if (t == t && i > tok)
-            ahead += Vec<T>::template above<false>(raw, t);
-          else
-            ahead += ahead_one_by_one<T>(x + i, i, t, tok);
-        }
+  uint32_t thr_bits = Vec<T>::bound(thr), bound_bits = Vec<T>::bound(-INFINITY);  // bound: least that look() does something for
+  // four vectors whose largest entries are vm, before their sums: the reference and the rank
+  const auto look = [&](const uint4 (&raw)[4], const uint32_t (&vm)[4], int first, int apart) {
+    if (!Vec<T>::reaches(Vec<T>::larger(Vec<T>::larger(vm[0], vm[1]), Vec<T>::larger(vm[2], vm[3])), bound_bits)) return;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float m = Vec<T>::value(vm[u]);
+      const int v = first + u * apart, i = head + v * N;
+      if (!(m <= s.lim)) s.move(m, Vec<T>::kFloor);
+      if (has && !(m < t) && v < v1) {
+        // a vector before the token counts its ties, one after it does not
+        if (t == t && i + N <= tok)
+          ahead += Vec<T>::template above<true>(raw[u], t);
+        else if (t == t && i > tok)
+          ahead += Vec<T>::template above<false>(raw[u], t);
+        else
+          ahead += ahead_one_by_one<T>(x + i, i, t, tok);
       }
     }
+    bound_bits = Vec<T>::bound(fminf(s.lim, t_bound));
+  };
+  const auto sum = [&](const uint4& raw) {
     float f[N];
     unpack_floored<T>(raw, f);
     s.template add<N>(f, L2);
   };
-  const auto max_nan = [](float a, float b) {
-    float m;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
-    return m;
+  const auto first_bound = [&](const uint32_t (&vm)[4]) {
+    thr = block_bound(sh, Vec<T>::value(Vec<T>::larger(Vec<T>::larger(vm[0], vm[1]), Vec<T>::larger(vm[2], vm[3]))), top);
+    thr_bits = Vec<T>::bound(thr);  // exact: an entry
   };
-  for (int step = 0; step < quarter; ++step) {
-    uint4 raw[4];
-    float vm[4];
-    const int vs = v0 + step * kThreads + threadIdx.x;
+  uint4 raw[4];
+  uint32_t vm[4];
+  if (quarter > 0) {
+    // a vector's registers take the next step's as soon as it is summed, so four
+    // loads a thread are nearly always in flight
+    const uint4* at[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) raw[u] = __ldcs(body + vs + u * quarter * kThreads);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) vm[u] = Vec<T>::max(raw[u]);
-    if (top > 0) {
-      if (step == 0) thr = block_bound(sh, max_nan(max_nan(vm[0], vm[1]), max_nan(vm[2], vm[3])), top);
-      const int b = step % 32;
-      if (b == 0 && step > 0) note_marks(sh, marks, vs - 32 * kThreads, quarter * kThreads);
-#pragma unroll
-      for (int u = 0; u < 4; ++u) marks[u] |= vm[u] < thr ? 0u : 1u << b;
+    for (int u = 0; u < 4; ++u) {
+      at[u] = body + v0 + u * quarter * kThreads + threadIdx.x;
+      raw[u] = __ldcs(at[u]);
     }
+    for (int step = 0; step < quarter; ++step) {
+      const int vs = v0 + step * kThreads + threadIdx.x, b = step % 32;
+      const bool more = step + 1 < quarter;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) take(raw[u], vm[u], vs + u * quarter * kThreads);
+      for (int u = 0; u < 4; ++u) vm[u] = largest<T>(raw[u]);
+      if (top > 0) {
+        if (step == 0)
+          first_bound(vm);
+        else if (b == 0)
+          note_marks(sh, marks, vs - 32 * kThreads, quarter * kThreads);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (Vec<T>::reaches(vm[u], thr_bits)) marks[u] |= 1u << b;
+      }
+      look(raw, vm, vs, quarter * kThreads);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        sum(raw[u]);
+        at[u] += kThreads;
+        if (more) raw[u] = __ldcs(at[u]);
+      }
+    }
+    if (top > 0) note_marks(sh, marks, v0 + (quarter - 1) / 32 * 32 * kThreads + threadIdx.x, quarter * kThreads);
   }
-  if (top > 0 && quarter > 0)
-    note_marks(sh, marks, v0 + (quarter - 1) / 32 * 32 * kThreads + threadIdx.x, quarter * kThreads);
   {
-    uint4 raw[4];
-    float vm[4];
     const int vs = v0 + quarter * 4 * kThreads + threadIdx.x;
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < 4; ++u) {
       raw[u] = vs + u * kThreads < v1 ? __ldcs(body + vs + u * kThreads)
                                       : make_uint4(Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf, Vec<T>::kNegInf);
-#pragma unroll
-    for (int u = 0; u < 4; ++u) vm[u] = Vec<T>::max(raw[u]);
+      vm[u] = largest<T>(raw[u]);
+    }
     if (top > 0) {
-      if (quarter == 0) thr = block_bound(sh, max_nan(max_nan(vm[0], vm[1]), max_nan(vm[2], vm[3])), top);
+      if (quarter == 0) first_bound(vm);
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (!(vm[u] < thr) && vs + u * kThreads < v1) note(sh, vs + u * kThreads);
+        if (Vec<T>::reaches(vm[u], thr_bits) && vs + u * kThreads < v1) note(sh, vs + u * kThreads);
     }
+    look(raw, vm, vs, kThreads);
 #pragma unroll
-    for (int u = 0; u < 4; ++u) take(raw[u], vm[u], vs + u * kThreads);
+    for (int u = 0; u < 4; ++u) sum(raw[u]);
   }
   const Part<T> p = {x, body, head, v0, v1, vocab, edges};
   if (threadIdx.x < edges) {
