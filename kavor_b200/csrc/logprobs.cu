@@ -236,7 +236,7 @@ struct Shared {
   Stats warp[kWarps];
   Stats cta;
   unsigned count, noted;
-  uint32_t four[32];
+  uint32_t four[32], maxes[kWarps];
 };
 
 // The 32 largest keys of the block, each warp holding one descending run;
@@ -425,9 +425,16 @@ __device__ __noinline__ void expand(Shared& sh, const Part<T>& p, unsigned n, fl
     const int v = sh.vecs[a];
     float f[N];
     Vec<T>::unpack(p.body[v], f);
+    unsigned hits = 0;
+#pragma unroll
+    for (int j = 0; j < N; ++j) hits |= f[j] < thr ? 0u : 1u << j;
+    unsigned at = atomicAdd(&sh.count, (unsigned)__popc(hits));
 #pragma unroll
     for (int j = 0; j < N; ++j)
-      if (!(f[j] < thr)) push(sh, f[j], p.head + v * N + j);
+      if (hits >> j & 1u) {
+        if (at < kCap) sh.list[at] = key_of(f[j], p.head + v * N + j);
+        ++at;
+      }
   }
   if (threadIdx.x < p.edges) {
     const int i = p.edge_index(threadIdx.x);
@@ -542,24 +549,38 @@ __device__ __forceinline__ Stats stats_of(const Sums& s, unsigned ahead) {
                (unsigned)s.bad};
 }
 
-// The block's statistics, in every thread; a fixed order of joins.
-__device__ __forceinline__ Stats block_join(Shared& sh, Stats st) {
+// The block's statistics, in every thread: each thread's sums are taken to the
+// block's reference, then added in a fixed order.
+__device__ __forceinline__ Stats block_join(Shared& sh, const Stats& st) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  uint32_t o = __reduce_max_sync(0xffffffffu, order_of(st.m));
+  if (lane == 0) sh.maxes[warp] = o;
+  __syncthreads();
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    Stats w;
-    w.m = __shfl_xor_sync(0xffffffffu, st.m, o);
-    w.s = __shfl_xor_sync(0xffffffffu, st.s, o);
-    w.t = __shfl_xor_sync(0xffffffffu, st.t, o);
-    w.rank = __shfl_xor_sync(0xffffffffu, st.rank, o);
-    w.bad = __shfl_xor_sync(0xffffffffu, st.bad, o);
-    st = join(st, w);
+  for (int w = 0; w < kWarps; ++w) o = max(o, sh.maxes[w]);
+  Stats a;
+  a.m = value_of(o);
+  const float d = st.m == -INFINITY ? -200.f : fmaxf(st.m - a.m, -200.f), f = ex2(d * kLog2e);
+  a.s = st.s * f;
+  a.t = (st.t + d * st.s) * f;
+#pragma unroll
+  for (int k = 16; k > 0; k >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, k);
+    a.t += __shfl_xor_sync(0xffffffffu, a.t, k);
   }
+  a.rank = __reduce_add_sync(0xffffffffu, st.rank);
+  a.bad = __any_sync(0xffffffffu, st.bad);
+  if (lane == 0) sh.warp[warp] = a;
   __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh.warp[threadIdx.x >> 5] = st;
-  __syncthreads();
-  st = sh.warp[0];
-  for (int w = 1; w < kWarps; ++w) st = join(st, sh.warp[w]);
-  return st;
+  a = sh.warp[0];
+#pragma unroll
+  for (int w = 1; w < kWarps; ++w) {
+    a.s += sh.warp[w].s;
+    a.t += sh.warp[w].t;
+    a.rank += sh.warp[w].rank;
+    a.bad |= sh.warp[w].bad;
+  }
+  return a;
 }
 
 // The part's sums again, entry by entry, for parts that hold nothing above the
