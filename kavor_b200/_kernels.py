@@ -8,6 +8,7 @@ the CPU: every op is a launch of a kernel in ``libkavor_b200.so``.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -412,6 +413,19 @@ def tree_workspace_bytes(batch: int, num_q_heads: int, num_kv_heads: int, max_se
     return int(n.value)
 
 
+@functools.lru_cache(maxsize=4096)
+def _tree_workspace_on(index: int, *sizes: int) -> int:
+    """``tree_workspace_bytes`` for the device ``index`` (it depends on its SM count)."""
+    prev = _current()
+    if prev == index:
+        return tree_workspace_bytes(*sizes)
+    torch.cuda.set_device(index)
+    try:
+        return tree_workspace_bytes(*sizes)
+    finally:
+        torch.cuda.set_device(prev)
+
+
 def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                    context_lens: torch.Tensor, cu_seqlens_q: torch.Tensor, max_seqlen_q: int, scale: float,
                    tree_mask: torch.Tensor | None = None, k_scale: torch.Tensor | None = None,
@@ -457,7 +471,7 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         _req(out.shape == q.shape and out.stride(2) == 1, "out must have q's shape and contiguous rows")
     # scratch of this call alone (torch's allocator orders its reuse on the stream), so calls on
     # different streams and captured graphs never share it
-    need = tree_workspace_bytes(batch, hq, hkv, max_seqlen_q)
+    need = _tree_workspace_on(index, batch, hq, hkv, max_seqlen_q)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     ost = out.stride()
     _launch(index, "kvb_tree_attn", q.data_ptr(), qst[0], qst[1], total, k_cache.data_ptr(), v_cache.data_ptr(),
