@@ -1,11 +1,11 @@
 // Work partition shared by the tree-attention kernels and their merge.
 //
 // A unit is one (sequence, group of kv heads, block of query rows of each): it
-// walks the sequence's context in tiles of tokens. The tiles of all units, in the
-// order sequence > head group > row block, form one line that is cut into ranges of
-// equal length, one per CTA (at most `parts`): every CTA streams the same number
-// of K/V bytes whatever the lengths of the sequences are, and the host needs
-// none of the device's lengths. A unit cut between CTAs leaves fp32
+// walks the sequence's context in tiles of tokens. The tiles of all units, each unit's
+// after kLead more for its fixed cost, in the order sequence > head group > row
+// block, form one line that is cut into ranges of equal length, one per CTA (at most
+// `parts`): every CTA has about the same work whatever the lengths of the sequences
+// are, and the host needs none of the device's lengths. A unit cut between CTAs leaves fp32
 // partials (unnormalised rows, running maximum and sum) that the merge joins
 // in order, so results do not depend on timing. Included by tree_attn.cu after
 // its error word.
@@ -17,6 +17,12 @@ namespace kvb {
 namespace tree {
 
 constexpr int kHD = 128;
+// What a unit costs besides its tiles (queries, first loads, output), in tiles: it
+// lies on the line before its first tile. With 0, 2, 4 and 6, us: 64 trees of 9 to 32
+// nodes over 200 to 2300 tokens of bf16 118, 96, 89, 90; decode of 256 over 50 to 2000
+// tokens of bf16 227, 188 (3), 176, 177; of e4m3 106, 103 (2), 104, 105; 16 x 64 nodes
+// over e4m3 434, 427, 423, 421.
+constexpr int kLead = 4;
 
 struct Args {
   const bf16* q;
@@ -84,7 +90,9 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int b, bool report) {
   s.blocks = (int)(((int64_t)s.nodes * a.group + a.rows - 1) / a.rows);
   return s;
 }
-__device__ __forceinline__ int64_t cost_of(const Args& a, const Seq& s) { return (int64_t)s.tiles * s.blocks * (a.hkv / a.heads); }
+__device__ __forceinline__ int64_t cost_of(const Args& a, const Seq& s) {
+  return s.tiles ? (int64_t)(s.tiles + kLead) * s.blocks * (a.hkv / a.heads) : 0;
+}
 
 // Exclusive prefix of each thread's sum over the block, and the total.
 template <int kThreads>
@@ -109,7 +117,7 @@ __device__ __forceinline__ int64_t block_prefix(int64_t mine, int64_t* total) {
   return before + incl - mine;
 }
 
-// Tiles of a range; part p holds [p * range, (p + 1) * range) of the line.
+// Length of a range; part p holds [p * range, (p + 1) * range) of the line.
 __device__ __forceinline__ int64_t range_of(int64_t total, int parts) { return (total + parts - 1) / parts; }
 
 // Where this CTA's range starts: the sequence, the offset in its tiles, and
@@ -147,41 +155,48 @@ struct Walk {
   int64_t off, left, range;
   Seq s;
   int h, rb, t0, n;  // first kv head, row block, first tile, tiles
+  int rest;          // tiles of the unit after these
 
   __device__ __forceinline__ Walk(const Args& a, const Start& st) : b(st.b), off(st.off), left(st.left), range(st.left), t0(1) {
     if (left > 0) s = seq_of(a, b, false);
   }
   __device__ __forceinline__ bool next(const Args& a) {
     if (left <= 0) return false;
-    while (off >= cost_of(a, s)) {
-      off = 0;
-      if (++b >= a.batch) return false;
-      s = seq_of(a, b, false);
+    for (;;) {
+      while (off >= cost_of(a, s)) {
+        off = 0;
+        if (++b >= a.batch) return false;
+        s = seq_of(a, b, false);
+      }
+      const int len = s.tiles + kLead;
+      int64_t u;
+      int hg;
+      if (off <= UINT32_MAX) {  // nearly always: a 64-bit division takes ten times as long
+        u = (uint32_t)off / (uint32_t)len;
+        hg = (int)((uint32_t)u / (uint32_t)s.blocks);
+      } else {
+        u = off / len;
+        hg = (int)(u / s.blocks);
+      }
+      const int pos = (int)(off - u * len), room = len - pos, take = (int)(left < room ? left : room);
+      off += take;
+      left -= take;
+      rest = room - take;
+      h = hg * a.heads;
+      rb = (int)(u - (int64_t)hg * s.blocks);
+      t0 = max(pos - kLead, 0);
+      n = max(pos + take - kLead, 0) - t0;
+      if (n > 0) return true;
+      t0 = 1;  // the range ends before the unit's first tile
+      if (left <= 0) return false;
     }
-    int64_t u;
-    int hg;
-    if (off <= UINT32_MAX) {  // nearly always: a 64-bit division takes ten times as long
-      u = (uint32_t)off / (uint32_t)s.tiles;
-      hg = (int)((uint32_t)u / (uint32_t)s.blocks);
-    } else {
-      u = off / s.tiles;
-      hg = (int)(u / s.blocks);
-    }
-    t0 = (int)(off - u * s.tiles);
-    h = hg * a.heads;
-    rb = (int)(u - (int64_t)hg * s.blocks);
-    const int64_t room = s.tiles - t0;
-    n = (int)(left < room ? left : room);
-    off += n;
-    left -= n;
-    return true;
   }
   __device__ __forceinline__ bool whole() const { return t0 == 0 && n == s.tiles; }
   // After the last segment, by one thread of the part.
   __device__ __forceinline__ void leave(const Args& a) const {
     Cut c = {};
     if (t0 == 0 && n < s.tiles) {  // a range that ends inside a unit is a full one
-      c.n = 1 + (int)((s.tiles - n + range - 1) / range);
+      c.n = 1 + (int)((rest + range - 1) / range);
       c.row0 = rb * a.rows;
       c.rows = min(a.rows, s.nodes * a.group - c.row0);
       c.q0 = s.q0;
