@@ -11,9 +11,11 @@
 // bits) is a bf16 value again. Infinities are held as the row's largest value
 // +-448 * 2^e, NaN as NaN; neither counts for the scale.
 //
-// Both kernels are bound by HBM (and, at a decode batch, by one launch):
-// 16 lanes own one row, 16 bytes of bf16 a lane, so a warp moves whole rows
-// with full-width accesses and the row maximum takes four shuffles.
+// Both kernels are bound by HBM (and, at a decode batch, by one launch): 8 lanes
+// (write) or 16 (read) own one row, so a warp moves whole rows with full-width
+// accesses and the row maximum takes three shuffles. Measured: 16384 tokens of 8
+// heads written in 18.5 us (5.5 TB/s of rows, cache bytes and scales), 64 sequences of
+// 100 to 4000 tokens read back in 152 us (5.7 TB/s).
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 

@@ -18,7 +18,13 @@
 // k-th largest entry, so each thread marks those of its vectors that reach it
 // (a few hundred of 19 thousand), one bit each, and only they are looked at again
 // at the end, when warps sort and merge their entries in 32-entry runs. The rank is counted
-// only in vectors whose maximum reaches the token's logit.
+// only in steps where a vector's maximum reaches the token's logit.
+//
+// Measured at 151936 bf16 entries: 2000 rows with 5 alternatives 138 us (4.4 TB/s),
+// without 118 us; bound by instructions (8 to 10 an entry, of which one exponential)
+// and a row's fixed end (join, expansion and sort: a fifth of a CTA's time), not
+// by HBM. 256 rows with 20 alternatives 34 us, 16 rows 12 us: one wave, its fixed ends
+// not hidden behind another row's stream.
 #include <cuda_fp16.h>
 
 #include "common.cuh"

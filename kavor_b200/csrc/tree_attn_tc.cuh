@@ -6,12 +6,14 @@
 // softmax warpgroups take the tiles in turn (one thread per query row, so no
 // reduction crosses threads), walk S twice in loops of 64 columns (straight-line
 // code for a row missed the instruction cache) and put the weights P in TMEM, from
-// where a second chain adds P V to the output rows, also in TMEM. One group's exponentials overlap the
-// other group's and the MMAs. Both groups weigh a row against the same reference,
-// settled tile by tile (a barrier hands it from group to group); it moves only when
-// a tile's maximum passes it by 2^15: weights of up to 2^15 cost nothing in bf16 or
-// half, and the output rows are rescaled once or twice in a context instead of at
-// every tile. One warp issues the TMA loads, one thread the MMAs.
+// where a second chain adds P V to the output rows, also in TMEM. One group's
+// exponentials overlap the other group's and the MMAs. Both groups weigh a row
+// against the same reference, settled tile by tile (a barrier hands it from group to
+// group); it moves only when a tile's maximum passes it by 2^15: weights of up to
+// 2^15 cost nothing in bf16 or half, and the output rows are rescaled once or twice
+// in a context instead of at every tile (a rescale waits for the P V before it: with
+// 2^8, 16 x 64 nodes over e4m3 took 564 us instead of 465). Loads, MMAs and the
+// conversion of V have warps of their own, each waiting for nothing it does not need.
 //
 // Over an e4m3 cache K stays e4m3: Q is split in two e4m3 parts, x = hi + lo, hi =
 // e4m3(x), lo = e4m3(x - hi), which hold a bf16 value (8 bits, two signed 4-bit
@@ -19,8 +21,16 @@
 // and to 2^-18 of that maximum below it. Two e4m3 chains take as long as one
 // 16-bit chain and K is never converted. The weights need more range than e4m3
 // has (2^-18 of the largest would be lost, and 10^5 tokens can hold a fifth of
-// the sum below that), so they are halves, and two more warps turn V into
-// halves, exactly.
+// the sum below that), so they are halves, and four warps turn V into halves,
+// exactly.
+//
+// Measured, 64 query heads over 8 kv heads, 16 trees of 64 nodes, 3900 to 8100
+// tokens: 288 us over bf16 (700 TFLOP/s), 425 over e4m3. A tile takes 2400 clocks
+// over bf16, of which the two MMA chains issue for 1170 and the exponentials (16 a
+// clock) take 1024; over e4m3 3000 to 3500: each score takes both scales, a softmax
+// thread's two walks and the handing over take 5000 of the 6500 between its tiles.
+// 64 trees of 9 to 32 nodes, 32 heads over 8, 200 to 2300 tokens of bf16: 89 us, the
+// fixed 10,000 clocks of each of the 512 units beside their 18 tiles at most.
 #pragma once
 
 namespace kvb {
