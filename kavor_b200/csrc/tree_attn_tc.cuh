@@ -25,7 +25,7 @@
 // exactly.
 //
 // Measured, 64 query heads over 8 kv heads, 16 trees of 64 nodes, 3900 to 8100
-// tokens: 288 us over bf16 (700 TFLOP/s), 425 over e4m3. A tile takes 2400 clocks
+// tokens: 288 us over bf16 (700 TFLOP/s), 396 over e4m3 (508). A tile takes 2400 clocks
 // over bf16, of which the two MMA chains issue for 1170 and the exponentials (16 a
 // clock) take 1024; over e4m3 3000 to 3500: each score takes both scales, a softmax
 // thread's two walks and the handing over take 5000 of the 6500 between its tiles.
@@ -251,8 +251,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t q_full, q_empty, kfull[C::kStages], vfull[C::kStages], k_empty[C::kStages], v_empty[C::kStages],
       v16_full[2], v16_empty[2], s_full[2], s_empty[2], p_full[2], pv_full[2], o_empty;
   __shared__ __align__(16) uint8_t scales[kFp8 ? C::kStages : 1][2][kTile];
-  // scales 2^a (K) and 2^b (V) of a tile: 2^a, b and 2^-b, exact in bf16; two tiles of each group
-  __shared__ __align__(16) bf16 tok_k[kFp8 ? 4 : 1][kTile], tok_b[kFp8 ? 4 : 1][kTile], tok_i[kFp8 ? 4 : 1][kTile];
+  // scales 2^a (K) and 2^b (V) of a tile: 2^a, b and 2^-b; two tiles of each group. (As bf16
+  // they took half the shared memory loads and two instructions more a pair: 428 us, not 396.)
+  __shared__ __align__(16) float tok_k[kFp8 ? 4 : 1][kTile], tok_b[kFp8 ? 4 : 1][kTile], tok_i[kFp8 ? 4 : 1][kTile];
   __shared__ float ref_s[kRows], l_s[2][kRows];
   __shared__ float qs_s[kFp8 ? 4 : 1][kRows];  // scale of a query row's e4m3 parts, of four segments
   __shared__ uint32_t o_started;  // the output rows hold something before a segment's first P V
@@ -574,9 +575,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const uint32_t kc = scales[st][0][r], vc = scales[st][1][r];
           float inv = __uint_as_float((254u - vc) << 23);
           if (tail && !(inv >= 0.f && inv < INFINITY)) inv = 0.f;  // stale scale bytes
-          tok_k[tb][r] = __ushort_as_bfloat16((unsigned short)(kc << 7));
-          tok_b[tb][r] = __float2bfloat16_rn((float)((int)vc - 127));
-          tok_i[tb][r] = __float2bfloat16_rn(inv);
+          tok_k[tb][r] = __uint_as_float(kc << 23);
+          tok_b[tb][r] = (float)((int)vc - 127);
+          tok_i[tb][r] = inv;
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&k_empty[st]));
           named_bar_sync(bar, 128);
@@ -592,7 +593,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         // scale in the second walk), back to S where that saves the second walk
         // something, and their maximum
         const uint64_t rs2 = pk2(rscale, rscale);
-        const auto pair_of = [](uint32_t two) { return pk2(__uint_as_float(two << 16), __uint_as_float(two & 0xffff0000u)); };
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll 1
         for (int c = 0; c < 128; c += 64) {
@@ -601,13 +601,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           if constexpr (kFp8) {
 #pragma unroll
             for (int i = 0; i < 64; i += 8) {
-              const uint4 k = *reinterpret_cast<const uint4*>(&tok_k[tb][c + i]);
-              const uint4 b = *reinterpret_cast<const uint4*>(&tok_b[tb][c + i]);
-              const uint32_t kw[4] = {k.x, k.y, k.z, k.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const uint64_t x = mul2(pk2(v[i + 2 * y], v[i + 2 * y + 1]), rs2);
-                un2(fma2(x, pair_of(kw[y]), pair_of(bw[y])), v[i + 2 * y], v[i + 2 * y + 1]);
+              for (int y = 0; y < 4; y += 2) {
+                const float4 k = *reinterpret_cast<const float4*>(&tok_k[tb][c + i + 2 * y]);
+                const float4 b = *reinterpret_cast<const float4*>(&tok_b[tb][c + i + 2 * y]);
+                const uint64_t x0 = mul2(pk2(v[i + 2 * y], v[i + 2 * y + 1]), rs2);
+                const uint64_t x1 = mul2(pk2(v[i + 2 * y + 2], v[i + 2 * y + 3]), rs2);
+                un2(fma2(x0, pk2(k.x, k.y), pk2(b.x, b.y)), v[i + 2 * y], v[i + 2 * y + 1]);
+                un2(fma2(x1, pk2(k.z, k.w), pk2(b.z, b.w)), v[i + 2 * y + 2], v[i + 2 * y + 3]);
               }
             }
           }
@@ -687,11 +688,12 @@ __global__ void __launch_bounds__(kThreads, 1)
                 e[y] = pk2(x0, x1);
               }
               if constexpr (kFp8) {
-                const uint4 n = *reinterpret_cast<const uint4*>(&tok_i[tb][c + i]);
-                sum[0] = fma2(e[0], pair_of(n.x), sum[0]);
-                sum[1] = fma2(e[1], pair_of(n.y), sum[1]);
-                sum[2] = fma2(e[2], pair_of(n.z), sum[2]);
-                sum[3] = fma2(e[3], pair_of(n.w), sum[3]);
+                const float4 n0 = *reinterpret_cast<const float4*>(&tok_i[tb][c + i]);
+                const float4 n1 = *reinterpret_cast<const float4*>(&tok_i[tb][c + i + 4]);
+                sum[0] = fma2(e[0], pk2(n0.x, n0.y), sum[0]);
+                sum[1] = fma2(e[1], pk2(n0.z, n0.w), sum[1]);
+                sum[2] = fma2(e[2], pk2(n1.x, n1.y), sum[2]);
+                sum[3] = fma2(e[3], pk2(n1.z, n1.w), sum[3]);
               } else {
 #pragma unroll
                 for (int y = 0; y < 4; ++y) sum[y] = add2(sum[y], e[y]);
