@@ -647,12 +647,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float corr = m_new == m_ref ? 1.f : ex2(m_ref - m_new);
             wait_pv_other(other + ((j + 1) >> 1) - 1);  // the tile before: P V run in order
 #pragma unroll 1
-            for (int c = 0; c < 8; ++c) {
-              float y[16];
-              tc::tmem_ld16(orow + c * 16, y);
+            for (int c = 0; c < 128; c += 64) {
+              float y[64];
+              tmem_row64(orow + c, y);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) y[i] *= corr;
-              tc::tmem_st16(orow + c * 16, y);
+              for (int i = 0; i < 64; ++i) y[i] *= corr;
+              tc::tmem_st32(orow + c, y);
+              tc::tmem_st32(orow + c + 32, y + 32);
             }
             l_run *= corr;
           }

@@ -652,3 +652,40 @@ def test_a_verification_step_of_drafted_trees_over_the_8bit_cache():
     logits = torch.nn.functional.linear(got.flatten(1), w)
     check_logprobs(logits, torch.randint(0, vocab, (nodes,), generator=gen(47)), 5)
     assert token_logprobs(logits, logits.argmax(1)).ranks.max() >= 0
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_a_step_as_programmatic_dependents_equals_plain_launches(fp8):
+    """Every kernel reads what the one before left only after waiting for it, whichever way it is launched."""
+    from kavor_b200 import _kernels as K
+    from kavor_b200.layers.sampler import token_logprobs
+
+    drafts = [Draft([700, 90, 2500], [1, 1, 1], 16, 8, fp8, seed=40), Draft([700, 90, 2500], [9, 30, 4], 32, 4, fp8, seed=41)]
+    logits = torch.randn(40, 5000, generator=gen(42)).to(DEV, torch.bfloat16)
+    tokens = torch.arange(40, device=DEV) * 7
+
+    def step():
+        out = []
+        for _ in range(3):
+            for d in drafts:
+                out.append(d.run())
+            out.extend(token_logprobs(logits, tokens, top_k=8))
+        torch.cuda.synchronize()
+        return out
+
+    want = step()
+    K.set_pdl(True)
+    try:
+        got = step()
+    finally:
+        K.set_pdl(False)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_tree_attention_of_units_much_smaller_than_a_part_and_of_few_tiles():
+    """More CTAs than tiles, and units of one tile beside one of thousands."""
+    for lens, sizes, hq, hkv in (([1] * 300, [1] * 300, 8, 1), ([64], [1], 8, 8), ([130] * 3 + [9000], [20, 1, 2, 5], 8, 2),
+                                 ([3] * 40 + [0, 5000], [2] * 40 + [0, 40], 16, 2)):
+        for fp8 in (False, True):
+            d = Draft(lens, sizes, hq, hkv, fp8, seed=len(lens))
+            d.check(d.run())
