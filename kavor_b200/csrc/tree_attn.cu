@@ -787,12 +787,18 @@ void fill(Variant* v) {
   v->parts = C::kCtas * device_sm_count();  // what the SMs hold: one wave
 }
 
+// More than 16 query rows a kv head over bf16, or 32 over e4m3 (two units of the
+// warp-MMA kernel), take tcgen05. Warp MMAs against tcgen05, us: bf16, 256 x 1024
+// tokens, 4 rows 167 / 218, 12 rows 186 / 220; 16 x 3900..8100 tokens, 8 rows 72 / 73,
+// 16 rows 78 / 73, 32 rows 121 / 75; one of 1531 tokens, 16 rows 19.5 / 17.5. e4m3, 256
+// x 1024 tokens, 16 rows 141 / 335, 32 rows 253 / 345; 16 x 3900..8100, 16 rows 57 / 101,
+// 32 rows 92 / 103, 48 rows 129 / 106; 130001 tokens, 32 rows 41 / 46, 48 rows 51 / 48.
 Variant variant_for(bool fp8, int hq, int hkv, int max_nodes, int block_size) {
   Variant v;
   const int64_t rows = (int64_t)(hq / hkv) * max_nodes;
   const bool few = rows <= 8;
   const int hp = !fp8 ? 1 : hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;
-  if (rows > 16) {
+  if (rows > (fp8 ? 32 : 16)) {
     v.nt = 0;
     v.rows = tcore::kRows;
     v.heads = 1;

@@ -1,5 +1,5 @@
-// The tensor-core form of the tree attention, for units of more than 16 query
-// rows: included by tree_attn.cu.
+// The tcgen05 form of the tree attention, for units of many query rows: included
+// by tree_attn.cu.
 //
 // A CTA owns 128 query rows (nodes x query heads of one kv head) and walks the
 // context in 128-token tiles: S = Q K^T is a tcgen05.mma chain into TMEM, two
@@ -25,10 +25,12 @@
 // exactly.
 //
 // Measured, 64 query heads over 8 kv heads, 16 trees of 64 nodes, 3900 to 8100
-// tokens: 288 us over bf16 (700 TFLOP/s), 396 over e4m3 (508). A tile takes 2400 clocks
+// tokens: 278 us over bf16 (724 TFLOP/s; K and V come 3.9 times from HBM, once for each
+// of a sequence's row blocks: 5.4 TB/s), 387 over e4m3 (520). A tile takes 2400 clocks
 // over bf16, of which the two MMA chains issue for 1170 and the exponentials (16 a
-// clock) take 1024; over e4m3 3000 to 3500: each score takes both scales, a softmax
-// thread's two walks and the handing over take 5000 of the 6500 between its tiles.
+// clock) take 1024; over e4m3 4500: each score takes both scales (a softmax
+// thread's two walks and the handing over take 5000 of the 6500 between its tiles),
+// and with these inputs' wide scores a tile in five rescales some of its rows.
 // 64 trees of 9 to 32 nodes, 32 heads over 8, 200 to 2300 tokens of bf16: 89 us, the
 // fixed 10,000 clocks of each of the 512 units beside their 18 tiles at most.
 #pragma once
