@@ -299,7 +299,8 @@ _current = torch.cuda.current_device
 
 
 def _stream_on(index: int) -> int:
-    return torch.cuda.current_stream(index).cuda_stream
+    # the stream's handle alone: torch.cuda.current_stream builds an object around it, 1 us of a decode step's call
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _launch(index: int, name: str, *args) -> None:
@@ -436,9 +437,9 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     _on(index, block_tables, "block_tables", torch.int32)
     _on(index, context_lens, "context_lens", torch.int32)
     _on(index, cu_seqlens_q, "cu_seqlens_q", torch.int32)
-    _req(q.dim() == 3, "q must be [total_q, heads, head_dim]")
-    total, hq, hd = q.shape
-    qst = q.stride()
+    shape, qst = q.shape, q.stride()
+    _req(len(shape) == 3, "q must be [total_q, heads, head_dim]")
+    total, hq, hd = shape
     _req(qst[2] == 1, "q must have contiguous rows")
     _req((k_scale is None) == (v_scale is None), "k_scale and v_scale come together")
     if k_scale is not None:
@@ -450,33 +451,33 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
         nblk, bs, hkv, chd = _cache_shape(k_cache, v_cache)
         ks_ptr, vs_ptr, sstride = None, None, 0
     _req(chd == hd, "q and the cache must share head_dim")
-    batch = context_lens.numel()
-    _req(context_lens.dim() == 1 and context_lens.is_contiguous(), "context_lens must be [batch]")
+    lens_shape, tab_shape, tab_st = context_lens.shape, block_tables.shape, block_tables.stride()
+    _req(len(lens_shape) == 1 and context_lens.is_contiguous(), "context_lens must be [batch]")
+    batch = lens_shape[0]
     _req(cu_seqlens_q.shape == (batch + 1,) and cu_seqlens_q.is_contiguous(), "cu_seqlens_q must be [batch + 1]")
-    _req(block_tables.dim() == 2 and block_tables.stride(1) == 1 and block_tables.shape[0] == batch,
-         "block_tables must be [batch, max_blocks]")
+    _req(len(tab_shape) == 2 and tab_st[1] == 1 and tab_shape[0] == batch, "block_tables must be [batch, max_blocks]")
     max_seqlen_q = int(max_seqlen_q)
     mask_ptr, mask_stride, words = None, 0, 0
     if tree_mask is not None:
         _on(index, tree_mask, "tree_mask", torch.int32)
-        _req(tree_mask.dim() == 2 and tree_mask.shape[0] == total and tree_mask.stride(1) == 1,
-             "tree_mask must be [total_q, words]")
-        words = tree_mask.shape[1]
+        m_shape, m_st = tree_mask.shape, tree_mask.stride()
+        _req(len(m_shape) == 2 and m_shape[0] == total and m_st[1] == 1, "tree_mask must be [total_q, words]")
+        words = m_shape[1]
         _req(words * 32 >= max_seqlen_q, "tree_mask rows must hold max_seqlen_q bits")
-        mask_ptr, mask_stride = tree_mask.data_ptr(), tree_mask.stride(0)
+        mask_ptr, mask_stride = tree_mask.data_ptr(), m_st[0]
     if out is None:
-        out = torch.empty(total, hq, hd, dtype=_BF16, device=q.device)
+        out = torch.empty(shape, dtype=_BF16, device=q.device)
     else:
         _on(index, out, "out", _BF16)
-        _req(out.shape == q.shape and out.stride(2) == 1, "out must have q's shape and contiguous rows")
+        _req(out.shape == shape and out.stride(2) == 1, "out must have q's shape and contiguous rows")
     # scratch of this call alone (torch's allocator orders its reuse on the stream), so calls on
     # different streams and captured graphs never share it
     need = _tree_workspace_on(index, batch, hq, hkv, max_seqlen_q)
     ws = torch.empty(need, dtype=torch.uint8, device=q.device)
     ost = out.stride()
     _launch(index, "kvb_tree_attn", q.data_ptr(), qst[0], qst[1], total, k_cache.data_ptr(), v_cache.data_ptr(),
-            ks_ptr, vs_ptr, nblk, k_cache.stride(0), sstride, bs, block_tables.data_ptr(), block_tables.stride(0),
-            block_tables.shape[1], context_lens.data_ptr(), cu_seqlens_q.data_ptr(), max_seqlen_q, mask_ptr,
+            ks_ptr, vs_ptr, nblk, k_cache.stride(0), sstride, bs, block_tables.data_ptr(), tab_st[0],
+            tab_shape[1], context_lens.data_ptr(), cu_seqlens_q.data_ptr(), max_seqlen_q, mask_ptr,
             mask_stride, words, out.data_ptr(), ost[0], ost[1], batch, hq, hkv, hd, float(scale), ws.data_ptr(), need)
     return out
 
@@ -682,19 +683,22 @@ def token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, top_k: int = 0
     """(logprobs [N], ranks [N], entropy [N], top_ids [N, k], top_logprobs [N, k]) of logits [N, vocab]."""
     index = _device_index(logits, "logits")
     kind = _LOGIT_TYPES.get(logits.dtype)
-    _req(kind is not None, f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
-    _req(logits.dim() == 2 and logits.stride(1) == 1, "logits must be [rows, vocab] with contiguous rows")
+    if kind is None:
+        _req(False, f"logits must be bf16, fp16 or fp32, got {logits.dtype}")
+    shape, stride = logits.shape, logits.stride()
+    _req(len(shape) == 2 and stride[1] == 1, "logits must be [rows, vocab] with contiguous rows")
     _on(index, token_ids, "token_ids", torch.int64)
-    rows, vocab = logits.shape
+    rows, vocab = shape
     _req(token_ids.shape == (rows,) and token_ids.is_contiguous(), "token_ids must be [rows]")
     top_k = int(top_k)
     _req(0 <= top_k <= 32 and top_k <= vocab, "top_k must be at most 32 and at most the vocabulary")
     dev = logits.device
-    # two allocations: the whole numbers and the 32-bit values
-    whole = torch.empty(rows * (1 + top_k), dtype=torch.int64, device=dev)
-    real = torch.empty(rows * (2 + top_k), dtype=torch.float32, device=dev)
-    at, rt = whole.data_ptr(), real.data_ptr()
-    _launch(index, "kvb_token_logprobs", logits.data_ptr(), kind, logits.stride(0) if rows > 1 else vocab,
-            token_ids.data_ptr(), rows, vocab, top_k, rt, at, rt + 4 * rows, at + 8 * rows, rt + 8 * rows)
-    return (real[:rows], whole[:rows], real[rows:2 * rows], whole[rows:].view(rows, top_k),
-            real[2 * rows:].view(rows, top_k))
+    lp = torch.empty(rows, dtype=torch.float32, device=dev)
+    rank = torch.empty(rows, dtype=torch.int64, device=dev)
+    entropy = torch.empty(rows, dtype=torch.float32, device=dev)
+    top_ids = torch.empty(rows, top_k, dtype=torch.int64, device=dev)
+    top_lp = torch.empty(rows, top_k, dtype=torch.float32, device=dev)
+    _launch(index, "kvb_token_logprobs", logits.data_ptr(), kind, stride[0] if rows > 1 else vocab,
+            token_ids.data_ptr(), rows, vocab, top_k, lp.data_ptr(), rank.data_ptr(), entropy.data_ptr(),
+            top_ids.data_ptr(), top_lp.data_ptr())
+    return lp, rank, entropy, top_ids, top_lp
