@@ -907,6 +907,9 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   a.rows = v.rows;
   a.by_dims = v.nt == 0;
   a.heads = v.heads;
+  a.head_groups = num_kv_heads / v.heads;
+  while ((1 << a.row_shift) < v.rows) ++a.row_shift;
+  while ((1 << a.tile_shift) < v.tile) ++a.tile_shift;
   a.tile = v.tile;
   a.box = v.box;
   a.parts = v.parts;

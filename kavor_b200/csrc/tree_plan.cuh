@@ -44,6 +44,8 @@ struct Args {
   int batch, hq, hkv, group;
   int num_blocks, block_size;
   int heads;              // kv heads of a unit
+  int head_groups;        // groups of that many
+  int row_shift, tile_shift;  // rows and tile are powers of two
   int parts, rows, tile;  // CTAs of the attention grid, query rows of a unit and head, tokens of a tile
   int box;                // tokens of a TMA box: a tile's, or a page's when that is smaller
   int by_dims;            // partials by dims: [parts][2][32][rows][4] (heads = 1)
@@ -86,12 +88,12 @@ __device__ __forceinline__ Seq seq_of(const Args& a, int b, bool report) {
     if (report) atomicOr(&g_err_tree, (unsigned)kErrBlockTable);
     s.len = (int)room;
   }
-  s.tiles = (s.len + a.tile - 1) / a.tile;
-  s.blocks = (int)(((int64_t)s.nodes * a.group + a.rows - 1) / a.rows);
+  s.tiles = (s.len + a.tile - 1) >> a.tile_shift;
+  s.blocks = (int)(((int64_t)s.nodes * a.group + a.rows - 1) >> a.row_shift);
   return s;
 }
 __device__ __forceinline__ int64_t cost_of(const Args& a, const Seq& s) {
-  return s.tiles ? (int64_t)(s.tiles + kLead) * s.blocks * (a.hkv / a.heads) : 0;
+  return s.tiles ? (int64_t)(s.tiles + kLead) * s.blocks * a.head_groups : 0;
 }
 
 // Exclusive prefix of each thread's sum over the block, and the total.
@@ -118,7 +120,10 @@ __device__ __forceinline__ int64_t block_prefix(int64_t mine, int64_t* total) {
 }
 
 // Length of a range; part p holds [p * range, (p + 1) * range) of the line.
-__device__ __forceinline__ int64_t range_of(int64_t total, int parts) { return (total + parts - 1) / parts; }
+__device__ __forceinline__ int64_t range_of(int64_t total, int parts) {
+  // 32 bits are nearly always enough: a 64-bit division takes ten times as long
+  return total <= INT32_MAX ? ((uint32_t)total + parts - 1) / (uint32_t)parts : (total + parts - 1) / parts;
+}
 
 // Where this CTA's range starts: the sequence, the offset in its tiles, and
 // how many tiles the range has. Every thread of the block calls it.
