@@ -362,13 +362,15 @@ struct Part {
   }
 };
 
-// Entries of the vector at x (first index i) that come before the token, for the
-// one vector that holds it and for a NaN token.
+// Entries of a vector (first index i) that come before the token, for the one
+// vector that holds it and for a NaN token.
 template <typename T>
-__device__ __noinline__ unsigned ahead_one_by_one(const T* x, int i, float t, int tok) {
+__device__ __noinline__ unsigned ahead_one_by_one(uint4 raw, int i, float t, int tok) {
+  float f[Vec<T>::kN];
+  Vec<T>::unpack(raw, f);
   unsigned n = 0;
-#pragma unroll 1
-  for (int j = 0; j < Vec<T>::kN; ++j) n += is_ahead(Vec<T>::one(x + j), i + j, t, tok);
+#pragma unroll
+  for (int j = 0; j < Vec<T>::kN; ++j) n += is_ahead(f[j], i + j, t, tok);
   return n;
 }
 
@@ -665,7 +667,7 @@ __global__ void __launch_bounds__(kThreads, 4)
         else if (t == t && i > tok)
           ahead += Vec<T>::template above<false>(raw[u], t);
         else
-          ahead += ahead_one_by_one<T>(x + i, i, t, tok);
+          ahead += ahead_one_by_one<T>(raw[u], i, t, tok);
       }
     }
     bound_bits = Vec<T>::bound(fminf(s.lim, t_bound));
