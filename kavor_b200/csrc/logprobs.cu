@@ -20,10 +20,10 @@
 // at the end, when warps sort and merge their entries in 32-entry runs. The rank is counted
 // only in steps where a vector's maximum reaches the token's logit.
 //
-// Measured at 151936 bf16 entries: 2000 rows with 5 alternatives 138 us (4.4 TB/s),
+// Measured at 151936 bf16 entries: 2000 rows with 5 alternatives 132 us (4.6 TB/s),
 // without 118 us; bound by instructions (8 to 10 an entry, of which one exponential)
 // and a row's fixed end (join, expansion and sort: a fifth of a CTA's time), not
-// by HBM. 256 rows with 20 alternatives 34 us, 16 rows 12 us: one wave, its fixed ends
+// by HBM. 256 rows with 20 alternatives 33 us, 16 rows 12 us: one wave, its fixed ends
 // not hidden behind another row's stream.
 #include <cuda_fp16.h>
 
@@ -69,15 +69,14 @@ struct Vec<float> {
     v[0] = __uint_as_float(r.x), v[1] = __uint_as_float(r.y), v[2] = __uint_as_float(r.z), v[3] = __uint_as_float(r.w);
   }
   static __device__ __forceinline__ float one(const float* p) { return *p; }
-  // entries above t (kOrEqual: or equal to it), NaN among them
-  template <bool kOrEqual>
-  static __device__ __forceinline__ unsigned above(const uint4& r, float t) {
-    float v[4];
-    unpack(r, v);
-    unsigned n = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) n += kOrEqual ? !(v[j] < t) : !(v[j] <= t);
-    return n;
+  // entries that reach a bound, NaN among them
+  static __device__ __forceinline__ unsigned count(const uint4& r, uint32_t b) {
+    return (unsigned)reaches(r.x, b) + reaches(r.y, b) + reaches(r.z, b) + reaches(r.w, b);
+  }
+  // the bound that only entries above b's value reach (not for NaN or +inf)
+  static __device__ __forceinline__ uint32_t above(uint32_t b) {
+    const uint32_t u = b == 0x80000000u ? 0u : b;
+    return u & 0x80000000u ? u - 1 : u + 1;
   }
 };
 
@@ -124,12 +123,14 @@ struct Vec<bf16> {
     }
   }
   static __device__ __forceinline__ float one(const bf16* p) { return __bfloat162float(*p); }
-  template <bool kOrEqual>
-  static __device__ __forceinline__ unsigned above(const uint4& r, float t) {
-    const __nv_bfloat162 tt = __float2bfloat162_rn(t);  // exact: t is one of the entries
+  static __device__ __forceinline__ unsigned count(const uint4& r, uint32_t b) {
+    const __nv_bfloat162 t = *reinterpret_cast<const __nv_bfloat162*>(&b);
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
-    return kOrEqual ? count_masks(__hgeu2_mask(h[0], tt), __hgeu2_mask(h[1], tt), __hgeu2_mask(h[2], tt), __hgeu2_mask(h[3], tt))
-                    : count_masks(__hgtu2_mask(h[0], tt), __hgtu2_mask(h[1], tt), __hgtu2_mask(h[2], tt), __hgtu2_mask(h[3], tt));
+    return count_masks(__hgeu2_mask(h[0], t), __hgeu2_mask(h[1], t), __hgeu2_mask(h[2], t), __hgeu2_mask(h[3], t));
+  }
+  static __device__ __forceinline__ uint32_t above(uint32_t b) {  // both halves alike
+    const uint32_t u = (b & 0xffffu) == 0x8000u ? 0u : b & 0xffffu, h = u & 0x8000u ? u - 1 : u + 1;
+    return h | h << 16;
   }
 };
 template <>
@@ -172,12 +173,14 @@ struct Vec<__half> {
     }
   }
   static __device__ __forceinline__ float one(const __half* p) { return __half2float(*p); }
-  template <bool kOrEqual>
-  static __device__ __forceinline__ unsigned above(const uint4& r, float t) {
-    const __half2 tt = __float2half2_rn(t);  // exact: t is one of the entries
+  static __device__ __forceinline__ unsigned count(const uint4& r, uint32_t b) {
+    const __half2 t = *reinterpret_cast<const __half2*>(&b);
     const __half2* h = reinterpret_cast<const __half2*>(&r);
-    return kOrEqual ? count_masks(__hgeu2_mask(h[0], tt), __hgeu2_mask(h[1], tt), __hgeu2_mask(h[2], tt), __hgeu2_mask(h[3], tt))
-                    : count_masks(__hgtu2_mask(h[0], tt), __hgtu2_mask(h[1], tt), __hgtu2_mask(h[2], tt), __hgtu2_mask(h[3], tt));
+    return count_masks(__hgeu2_mask(h[0], t), __hgeu2_mask(h[1], t), __hgeu2_mask(h[2], t), __hgeu2_mask(h[3], t));
+  }
+  static __device__ __forceinline__ uint32_t above(uint32_t b) {  // both halves alike
+    const uint32_t u = (b & 0xffffu) == 0x8000u ? 0u : b & 0xffffu, h = u & 0x8000u ? u - 1 : u + 1;
+    return h | h << 16;
   }
 };
 
@@ -362,8 +365,7 @@ struct Part {
   }
 };
 
-// Entries of a vector (first index i) that come before the token, for the one
-// vector that holds it and for a NaN token.
+// Entries of a vector (first index i) that come before a NaN or infinite token.
 template <typename T>
 __device__ __noinline__ unsigned ahead_one_by_one(uint4 raw, int i, float t, int tok) {
   float f[Vec<T>::kN];
@@ -649,28 +651,37 @@ __global__ void __launch_bounds__(kThreads, 4)
   Sums s;
   unsigned ahead = 0;
   float thr = INFINITY;  // least entry that may be among the top ones
-  const float t_bound = !has ? INFINITY : t != t ? -INFINITY : t;
+  const bool plain = has && t < INFINITY;  // not a NaN or +inf
+  const uint32_t t_bits = Vec<T>::bound(t != t ? -INFINITY : t);
+  // the ties before the token in its own vector
+  if (plain && threadIdx.x < N && tok >= head + v0 * N && tok < head + v1 * N) {
+    const int i = tok - (tok - head) % N + threadIdx.x;
+    ahead = i < tok && Vec<T>::one(x + i) == t;
+  }
   uint32_t marks[4] = {0u, 0u, 0u, 0u};  // vectors of this thread that reach thr
-  uint32_t thr_bits = Vec<T>::bound(thr), bound_bits = Vec<T>::bound(-INFINITY);  // bound: least that look() does something for
+  uint32_t thr_bits = Vec<T>::bound(thr), lim_bits = Vec<T>::bound(-INFINITY);
   // four vectors whose largest entries are vm, before their sums: the reference and the rank
   const auto look = [&](const uint4 (&raw)[4], const uint32_t (&vm)[4], int first, int apart) {
-    if (!Vec<T>::reaches(Vec<T>::larger(Vec<T>::larger(vm[0], vm[1]), Vec<T>::larger(vm[2], vm[3])), bound_bits)) return;
+    const uint32_t most = Vec<T>::larger(Vec<T>::larger(vm[0], vm[1]), Vec<T>::larger(vm[2], vm[3]));
+    if (Vec<T>::reaches(most, lim_bits)) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const float m = Vec<T>::value(vm[u]);
+        if (!(m <= s.lim)) s.move(m, Vec<T>::kFloor);
+      }
+      lim_bits = Vec<T>::bound(s.lim);
+    }
+    if (!has || !Vec<T>::reaches(most, t_bits)) return;
+    const uint32_t after = Vec<T>::above(t_bits);
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const float m = Vec<T>::value(vm[u]);
       const int v = first + u * apart, i = head + v * N;
-      if (!(m <= s.lim)) s.move(m, Vec<T>::kFloor);
-      if (has && !(m < t) && v < v1) {
-        // a vector before the token counts its ties, one after it does not
-        if (t == t && i + N <= tok)
-          ahead += Vec<T>::template above<true>(raw[u], t);
-        else if (t == t && i > tok)
-          ahead += Vec<T>::template above<false>(raw[u], t);
-        else
-          ahead += ahead_one_by_one<T>(raw[u], i, t, tok);
-      }
+      if (v >= v1) continue;
+      if (plain)  // before the token ties count too, from its own vector on they do not
+        ahead += Vec<T>::count(raw[u], i + N <= tok ? t_bits : after);
+      else
+        ahead += ahead_one_by_one<T>(raw[u], i, t, tok);
     }
-    bound_bits = Vec<T>::bound(fminf(s.lim, t_bound));
   };
   const auto sum = [&](const uint4& raw) {
     float f[N];
