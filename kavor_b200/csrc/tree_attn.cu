@@ -787,18 +787,22 @@ void fill(Variant* v) {
   v->parts = C::kCtas * device_sm_count();  // what the SMs hold: one wave
 }
 
-// More than 16 query rows a kv head over bf16, or 32 over e4m3 (two units of the
-// warp-MMA kernel), take tcgen05. Warp MMAs against tcgen05, us: bf16, 256 x 1024
-// tokens, 4 rows 167 / 218, 12 rows 186 / 220; 16 x 3900..8100 tokens, 8 rows 72 / 73,
-// 16 rows 78 / 73, 32 rows 121 / 75; one of 1531 tokens, 16 rows 19.5 / 17.5. e4m3, 256
-// x 1024 tokens, 16 rows 141 / 335, 32 rows 253 / 345; 16 x 3900..8100, 16 rows 57 / 101,
-// 32 rows 92 / 103, 48 rows 129 / 106; 130001 tokens, 32 rows 41 / 46, 48 rows 51 / 48.
-Variant variant_for(bool fp8, int hq, int hkv, int max_nodes, int block_size) {
+// More than 16 query rows a kv head over bf16 (8, while every sequence and kv head
+// can have an SM), or 32 over e4m3 (two units of the warp-MMA kernel), take tcgen05.
+// Warp MMAs against tcgen05, us:
+// bf16, 256 sequences of 1024 tokens: 4 rows 167 / 218, 12 rows 186 / 220; 16 of
+// 3900..8100: 8 rows 72 / 73, 16 rows 78 / 73, 32 rows 121 / 75; 16 rows over 8 heads: one
+// of 100 16.4 / 13.4, 1531 18.7 / 16.4, 8000 20.5 / 21.6, 100000 81 / 78, 18 of 100..9000
+// 83 / 64, 32 of 500..1500 42 / 43.
+// e4m3, 256 of 1024: 16 rows 141 / 335, 32 rows 253 / 345; 16 of 3900..8100: 16 rows 57 /
+// 101, 32 rows 92 / 103, 48 rows 129 / 106; 130001 tokens: 32 rows 41 / 46, 48 rows 51 / 48.
+Variant variant_for(bool fp8, int batch, int hq, int hkv, int max_nodes, int block_size) {
   Variant v;
   const int64_t rows = (int64_t)(hq / hkv) * max_nodes;
   const bool few = rows <= 8;
   const int hp = !fp8 ? 1 : hkv % 4 == 0 ? 4 : hkv % 2 == 0 ? 2 : 1;
-  if (rows > (fp8 ? 32 : 16)) {
+  const int most = fp8 ? 32 : (int64_t)batch * hkv <= device_sm_count() ? 8 : 16;  // rows for warp MMAs
+  if (rows > most) {
     v.nt = 0;
     v.rows = tcore::kRows;
     v.heads = 1;
@@ -860,8 +864,8 @@ extern "C" int kvb_tree_attn_workspace_size(int batch, int num_q_heads, int num_
   if (batch < 0 || num_q_heads <= 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_seqlen_q < 0)
     return set_error(kInvalid, "kvb_tree_attn_workspace_size: bad sizes");
   // the larger of the two cache types' needs (the block size does not matter)
-  const size_t a = variant_for(false, num_q_heads, num_kv_heads, max_seqlen_q, 256).workspace;
-  const size_t b = variant_for(true, num_q_heads, num_kv_heads, max_seqlen_q, 256).workspace;
+  const size_t a = variant_for(false, batch, num_q_heads, num_kv_heads, max_seqlen_q, 256).workspace;
+  const size_t b = variant_for(true, batch, num_q_heads, num_kv_heads, max_seqlen_q, 256).workspace;
   *bytes = a > b ? a : b;
   return kOk;
 }
@@ -903,7 +907,7 @@ extern "C" int kvb_tree_attn(const void* q, int64_t q_stride_t, int64_t q_stride
   if (!(scale > 0.f) || scale > 1e30f) return set_error(kInvalid, "kvb_tree_attn: scale must be positive and finite");
 
   Args a = {};
-  const Variant v = variant_for(fp8, num_q_heads, num_kv_heads, max_seqlen_q, block_size);
+  const Variant v = variant_for(fp8, batch, num_q_heads, num_kv_heads, max_seqlen_q, block_size);
   a.rows = v.rows;
   a.by_dims = v.nt == 0;
   a.heads = v.heads;
