@@ -689,3 +689,41 @@ def test_tree_attention_of_units_much_smaller_than_a_part_and_of_few_tiles():
         for fp8 in (False, True):
             d = Draft(lens, sizes, hq, hkv, fp8, seed=len(lens))
             d.check(d.run())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("hq,hkv,size", [(8, 8, 8), (6, 2, 3), (9, 3, 3), (8, 4, 8), (4, 1, 4), (17, 1, 1), (16, 4, 8), (8, 2, 8),
+                                         (11, 1, 3), (12, 3, 8), (33, 1, 1)])
+def test_tree_attention_at_the_row_limits_of_its_kernels(hq, hkv, size, many, fp8):
+    """8, 9, 12, 16, 17, 32 and 33 query rows a kv head, for few sequences and for more than the GPU has SMs."""
+    n = 150 // hkv + 2 if many else 3
+    rng = random.Random(hq * 100 + size)
+    lens = [rng.randint(size, 700 if not many else 200) for _ in range(n)]
+    sizes = [rng.randint(1, size) for _ in range(n - 1)] + [size]
+    d = Draft(lens, sizes, hq, hkv, fp8, seed=hq + size)
+    d.mask[0] = 0
+    d.check(d.run())
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hq,hkv,size,n", [(8, 4, 8, 40), (4, 2, 4, 80), (8, 2, 8, 3)])
+def test_tree_attention_ignores_unseen_nodes_in_every_sequence(hq, hkv, size, n, fp8):
+    """16, 8 and 32 query rows a kv head: node 2 of every tree holds NaN, the others hang under node 0 and do not see it."""
+    lens = [size + 13 * b % 190 for b in range(n)]
+    d = Draft(lens, [size] * n, hq, hkv, fp8, seed=70)
+    d.mask = A().build_tree_mask([[-1] + [0] * (size - 1)] * n)
+    want = d.expected()
+    for b in range(n):
+        pos = lens[b] - size + 2
+        blk, off = int(d.table[b, pos // d.bs]), pos % d.bs
+        for c in (d.k, d.v):
+            if fp8:
+                c.view(torch.uint8)[blk, off] = 0x7F
+            else:
+                c[blk, off] = math.nan
+    got = d.run().cpu()
+    hit = torch.arange(n * size) % size == 2
+    assert torch.isnan(got[hit].float()).all() and torch.isfinite(got[~hit].float()).all()
+    err = (got.double() - want)[~hit]
+    assert float(err.norm() / want[~hit].norm()) < 2.0 ** -8
