@@ -727,3 +727,43 @@ def test_tree_attention_ignores_unseen_nodes_in_every_sequence(hq, hkv, size, n,
     assert torch.isnan(got[hit].float()).all() and torch.isfinite(got[~hit].float()).all()
     err = (got.double() - want)[~hit]
     assert float(err.norm() / want[~hit].norm()) < 2.0 ** -8
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+def test_blocks_whose_offsets_pass_32_bits(fp8):
+    """The same pages at the end of a pool of more than 2^32 bytes and values give the same bytes."""
+    d = Draft([600, 90, 1300], [5, 40, 1], 16, 8, fp8, seed=80)
+    page = d.k.stride(0) * d.k.element_size()
+    pages = 2 ** 32 * d.k.element_size() // page + 2 * d.k.shape[0]
+    big = torch.empty(pages * page, dtype=torch.uint8, device=DEV)
+    shift = pages - d.k.shape[0]
+    big.view(pages, page)[shift:].copy_(torch.as_strided(d.k.view(torch.uint8), (d.k.shape[0], page), (page, 1)))
+
+    def moved(t):
+        flat = big.view(t.dtype)
+        return flat.as_strided((pages, *t.shape[1:]), t.stride(), t.storage_offset())
+
+    want = d.run()
+    parts = [d.k, d.v, d.ks, d.vs] if fp8 else [d.k, d.v]
+    new = [moved(t) for t in parts]
+    table = torch.where(d.table >= 0, d.table + shift, d.table)
+    d.k, d.v = new[:2]
+    if fp8:
+        d.ks, d.vs = new[2:]
+    d.table = table
+    assert torch.equal(d.run(), want)
+    if fp8:
+        cu = torch.tensor([0, 600], dtype=torch.int32, device=DEV)
+        k, v = A().load_kvcache_fp8(*new, table[:1].to(DEV), cu, 600)
+        for got, cache, scale in ((k, new[0], new[2]), (v, new[1], new[3])):
+            assert torch.equal(got.cpu().double(), held_rows(cache, scale, table[0], 600, d.bs))
+        rows = torch.randn(3, 8, D, generator=gen(81)).to(DEV, torch.bfloat16)
+        slots = torch.tensor([pages * d.bs - 1, 5, pages * d.bs - d.bs], dtype=torch.int32, device=DEV)
+        A().store_kvcache_fp8(rows, rows, *new, slots)
+        low = [torch.zeros_like(t[:1]).contiguous() for t in new]
+        A().store_kvcache_fp8(rows, rows, *low, torch.tensor([d.bs - 1, 5, 0], dtype=torch.int32, device=DEV))
+        for at, block in ((d.bs - 1, pages - 1), (5, 0), (0, pages - 1)):
+            for t, s in zip(new[:2], low[:2]):
+                assert torch.equal(t[block, at].view(torch.uint8), s[0, at].view(torch.uint8))
+            for t, s in zip(new[2:], low[2:]):
+                assert torch.equal(t[block, :, at].view(torch.uint8), s[0, :, at].view(torch.uint8))
