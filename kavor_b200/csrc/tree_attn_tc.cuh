@@ -741,39 +741,39 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint32_t bits = __ballot_sync(0xffffffffu, odd);
             if (lane == 0) odd_bits[gr][qd] = bits;
             named_bar_sync(bar, 128);
-            float v[128];
-#pragma unroll
-            for (int i = 0; i < kHD; ++i) v[i] = 0.f;
+            if (j > 0) wait_pv_other(other + ((j + 1) >> 1) - 1);
 #pragma unroll 1
-            for (int t = 0; t < kTile; ++t) {
-              if (!((odd_bits[gr][t >> 5] >> (t & 31)) & 1u)) continue;  // the same for the whole group
-              const uint32_t bits = t < 64 ? t < 32 ? seen[0] : seen[1] : t < 96 ? seen[2] : seen[3];
-              const uint32_t two = tmem_ld1(prow + (t >> 1)) >> (t & 1 ? 16 : 0);
-              if ((bits >> (t & 31)) & 1u) {
-                const float p = kFp8 ? __half2float(__ushort_as_half((unsigned short)two)) : __uint_as_float(two << 16);
+            for (int d = 0; d < 4; ++d) {  // 32 dims at a time: few registers beside the main path's
+              float v[32];
 #pragma unroll
-                for (int c = 0; c < 16; ++c) {
-                  const uint4 y = lds128(vt + t * 128 + (c >> 3) * kHalf + (((c & 7) ^ (t & 7)) << 4));
-                  const uint32_t wd[4] = {y.x, y.y, y.z, y.w};
+              for (int i = 0; i < 32; ++i) v[i] = 0.f;
+#pragma unroll 1
+              for (int t = 0; t < kTile; ++t) {
+                if (!((odd_bits[gr][t >> 5] >> (t & 31)) & 1u)) continue;  // the same for the whole group
+                const uint32_t bits = t < 64 ? t < 32 ? seen[0] : seen[1] : t < 96 ? seen[2] : seen[3];
+                const uint32_t two = tmem_ld1(prow + (t >> 1)) >> (t & 1 ? 16 : 0);
+                if ((bits >> (t & 31)) & 1u) {
+                  const float p = kFp8 ? __half2float(__ushort_as_half((unsigned short)two)) : __uint_as_float(two << 16);
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) {
-                    const float2 f = kFp8 ? __half22float2(*reinterpret_cast<const __half2*>(&wd[i]))
-                                          : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wd[i]));
-                    v[c * 8 + i * 2] += p * f.x;
-                    v[c * 8 + i * 2 + 1] += p * f.y;
+                  for (int c = 0; c < 4; ++c) {
+                    const uint4 y = lds128(vt + t * 128 + (d >> 1) * kHalf + ((((d & 1) * 4 + c) ^ (t & 7)) << 4));
+                    const uint32_t wd[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                      const float2 f = kFp8 ? __half22float2(*reinterpret_cast<const __half2*>(&wd[i]))
+                                            : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wd[i]));
+                      v[c * 8 + i * 2] += p * f.x;
+                      v[c * 8 + i * 2 + 1] += p * f.y;
+                    }
                   }
                 }
+                __syncwarp();
               }
-              __syncwarp();
-            }
-            if (j > 0) wait_pv_other(other + ((j + 1) >> 1) - 1);
+              float y[32];
+              if (j > 0) tc::tmem_ld32(orow + d * 32, y);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-              float y[16];
-              if (j > 0) tc::tmem_ld16(orow + c * 16, y);
-#pragma unroll
-              for (int i = 0; i < 16; ++i) y[i] = (j > 0 ? y[i] : 0.f) + v[c * 16 + i];
-              tc::tmem_st16(orow + c * 16, y);
+              for (int i = 0; i < 32; ++i) v[i] += j > 0 ? y[i] : 0.f;
+              tc::tmem_st32(orow + d * 32, v);
             }
             if (j == 0 && r == 0) o_started = 1;
             named_bar_sync(bar, 128);
