@@ -43,6 +43,11 @@ constexpr int kMaxTop = 32;
 constexpr int kCap = 2048;      // entries of the candidate list
 constexpr float kSlack = 10.f;  // how far an entry may pass a thread's reference
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// The largest magnitude a reference r may have. Powers are taken against c = r log2(e)
+// rounded to 32 bits; c's residue, half a unit of its last place, is up to 4 at 2^26,
+// so the powers lie in 2^+-(4 + 10 log2(e)). (At 1e10 it is 512: 2^y is infinite or 0.)
+// Parts whose largest entry is beyond it are summed again entry by entry.
+constexpr float kFar = 67108864.f;
 
 // ------------------------------------------------------------ element types
 template <typename T>
@@ -293,17 +298,18 @@ __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 // per entry. c is rounded; its residue is put right in the end. S and T hold two
 // partial sums each.
 struct Sums {
-  float r = 0.f, lim = -INFINITY;  // entries above lim move r; lim = -inf: nothing above the floor seen yet
+  float r = 0.f, lim = -INFINITY;  // entries above lim move r; lim = -inf: no entry has made a reference yet
   uint64_t c = 0, S = 0, T = 0;
   bool bad = false;
 
-  // called before a group whose largest entry is vm > lim, or NaN
-  __device__ __forceinline__ void move(float vm, float floor) {
+  // Called before a group whose largest entry is vm > lim, or NaN. low: up to there an
+  // entry (a finite mask, say) makes no reference; it weighs nothing beside ordinary entries.
+  __device__ __forceinline__ void move(float vm, float low) {
     if (!(vm < INFINITY)) {  // NaN or +inf
       bad = true;
       return;
     }
-    if (vm <= floor) return;  // weighs nothing beside an ordinary entry (and its c could overflow)
+    if (vm <= low) return;
     const float nc = -vm * kLog2e;
     if (lim != -INFINITY) {
       float old, unused;
@@ -332,9 +338,14 @@ struct Sums {
   }
 };
 
-// A vector's entries, those below the type's floor raised to it: the weight is
-// 0 beside any ordinary entry, and 0 * y stays 0. (Parts where nothing is above
-// the floor, or where y could overflow, are summed again entry by entry.)
+// The largest entry that makes no reference.
+template <typename T>
+__device__ __forceinline__ constexpr float low_of() {
+  return Vec<T>::kFloor > -kFar ? Vec<T>::kFloor : -kFar;
+}
+
+// A vector's entries, those below the type's floor raised to it, so that their y
+// stays finite: the weight is 0 beside any ordinary entry, and 0 * y stays 0.
 template <typename T>
 __device__ __forceinline__ void unpack_floored(const uint4& raw, float* f) {
   Vec<T>::unpack(make_uint4(Vec<T>::floor_word(raw.x), Vec<T>::floor_word(raw.y), Vec<T>::floor_word(raw.z),
@@ -593,9 +604,9 @@ __device__ __forceinline__ Stats block_join(Shared& sh, const Stats& st) {
   return a;
 }
 
-// The part's sums again, entry by entry, for parts that hold nothing above the
-// type's floor (-inf must not count beside it) or entries so large that the
-// powers' arguments overflow.
+// The part's sums again, entry by entry, each less the maximum before it is
+// scaled: for parts whose largest entry is not well above low_of() (entries up to
+// there have not been counted) or is beyond kFar.
 template <typename T>
 __device__ __noinline__ Stats sum_one_by_one(Shared& sh, const Part<T>& p, unsigned ahead) {
   float m = -INFINITY, S = 0.f, E = 0.f;
@@ -667,7 +678,7 @@ __global__ void __launch_bounds__(kThreads, 4)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const float m = Vec<T>::value(vm[u]);
-        if (!(m <= s.lim)) s.move(m, Vec<T>::kFloor);
+        if (!(m <= s.lim)) s.move(m, low_of<T>());
       }
       lim_bits = Vec<T>::bound(s.lim);
     }
@@ -749,7 +760,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   if (threadIdx.x < edges) {
     const int i = p.edge_index(threadIdx.x);
     const float v = Vec<T>::one(x + i);
-    if (!(v <= s.lim)) s.move(v, Vec<T>::kFloor);
+    if (!(v <= s.lim)) s.move(v, low_of<T>());
     const float f[2] = {fmaxf(v, Vec<T>::kFloor), Vec<T>::kFloor};
     if (s.lim != -INFINITY) s.add<2>(f, L2);
     if (has) ahead += is_ahead(v, i, t, tok);
@@ -758,8 +769,8 @@ __global__ void __launch_bounds__(kThreads, 4)
   // ------------------------------------------------------ join the sums
   Stats st = stats_of(s, ahead);
   st = block_join(sh, st);
-  if (!st.bad && (st.m == -INFINITY || st.m > 1e30f))
-    st = sum_one_by_one(sh, p, ahead);
+  // 256 above low_of(), what has not been counted weighs under e^-256
+  if (!st.bad && !(st.m >= low_of<T>() + 256.f && st.m <= kFar)) st = sum_one_by_one(sh, p, ahead);
   if (threadIdx.x == 0) sh.cta = st;
 
   // ------------------------------------------------- the part's top entries
