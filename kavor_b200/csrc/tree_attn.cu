@@ -39,6 +39,19 @@ using tree::Walk;
 // instructions and K and V are converted once for all rows. e4m3 bytes become
 // halves in registers (exact); two 8x8 register transposes turn the weights from
 // S^T's layout to P^T's.
+//
+// Over e4m3 the weights are halves and carry V's scale: with s_j = scale log2(e) 2^a_j
+// (q . kq_j) and a row's running reference m = max(s_j + b_j), vq_j is multiplied by
+// 2^(s_j + b_j - m + 8). That is the row's share of the output, so what a half loses
+// (steps of 2^-24) is 2^-33 of the largest share at most. The softmax's own sum is of
+// 2^(s_j - m + 8) in 32 bits: taken from the weight, times 2^-b_j, it lost tokens whose
+// share is small only because their V is. The weight is that term times 2^b_j or, for 8
+// query rows, a second exponential (us, times 2^b_j / exponential: decode of 256 x 1024
+// tokens 100.5 / 98.6, 32 rows over 130001 tokens 44.1 / 46.4). A row of V that
+// holds nothing has the scale 2^0 and no share: it counts with kNothing for b_j, or one
+// that draws the attention would push every other weight out of a half's range.
+constexpr float kTop = 8.f;         // log2 of the largest weight over e4m3
+constexpr float kNothing = -100.f;  // the least exponent a written row can have
 constexpr int kWarps = 4;
 constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kScratchStride = kHD + 4;  // fp32 row of the warp merge, padded against bank conflicts
@@ -128,6 +141,24 @@ __device__ __forceinline__ uint32_t lds16(uint32_t addr) {
   return v;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+
+// Bit i: row i of a warp's 16 KT rows of V, from row tok0 of the e4m3 tile at vb, holds a value that is not zero.
+template <int KT>
+__device__ __forceinline__ uint32_t rows_that_hold(uint32_t vb, int tok0, int lane) {
+  uint32_t holds = 0;
+#pragma unroll 1
+  for (int i = 0; i < 4 * KT; ++i) {  // four rows at a time, eight lanes a row
+    uint32_t x[4];
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3])
+                 : "r"(swz<true>(vb, tok0 + i * 4 + (lane >> 3), lane & 7)));
+    const uint32_t lanes = __ballot_sync(0xffffffffu, ((x[0] | x[1] | x[2] | x[3]) & 0x7f7f7f7fu) != 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) holds |= (uint32_t)((lanes >> (8 * r) & 0xffu) != 0) << (i * 4 + r);
+  }
+  return holds;
+}
+
 template <bool kFp8, int NT, int HP>
 __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
     tree_warp_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap,
@@ -360,7 +391,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
         }
       }
 
-      float inv_v[KT][2];  // 2^-exponent of the V rows of this lane's tokens
+      float ev[KT][2], vs[KT][2];  // exponents b and scales 2^b of the V rows of this lane's tokens
+      bool unit = false;           // an exponent is 0
 #pragma unroll
       for (int k = 0; k < KT; ++k)
 #pragma unroll
@@ -369,12 +401,13 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
             const int tk = hw * kTile + tok0 + k * 16 + g + 8 * h;
             const uint32_t kc = scales[s][0][tk], vc = scales[s][1][tk];
             const float ksc = __uint_as_float(kc << 23);
-            const float ev = __uint_as_float(0x4b000000u | vc) - (8388608.f + 127.f);  // vc - 127
-            inv_v[k][h] = __uint_as_float((254u - vc) << 23);
+            ev[k][h] = __uint_as_float(0x4b000000u | vc) - (8388608.f + 127.f);  // vc - 127
+            vs[k][h] = __uint_as_float(vc << 23);
+            unit |= vc == 127u;
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
-              for (int i = 0; i < 2; ++i) sc[k][t][2 * h + i] = fmaf(sc[k][t][2 * h + i], rscale[t][i] * ksc, ev);
+              for (int i = 0; i < 2; ++i) sc[k][t][2 * h + i] *= rscale[t][i] * ksc;
           } else {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -382,6 +415,14 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
               for (int i = 0; i < 2; ++i) sc[k][t][2 * h + i] *= rscale[t][i];
           }
         }
+      if (kFp8 && __any_sync(0xffffffffu, unit)) {  // rare: rows of nothing, or with values between 224 and 448
+        const uint32_t holds = rows_that_hold<KT>(vb, tok0, lane);
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (ev[k][h] == 0.f && !((holds >> (k * 16 + g + 8 * h)) & 1u)) ev[k][h] = kNothing, vs[k][h] = 0.f;
+      }
       uint32_t hidden[KT];  // bit 4 t + 2 h + i: that score is masked
       if (tail) {
 #pragma unroll
@@ -390,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int pos = p0 + k * 16 + g + 8 * h;
-            if (kFp8 && !(inv_v[k][h] >= 0.f && inv_v[k][h] < INFINITY)) inv_v[k][h] = 0.f;  // stale scale bytes
+            if (kFp8 && vs[k][h] == INFINITY) vs[k][h] = 0.f;  // stale scale bytes
 #pragma unroll
             for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -412,24 +453,25 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
       for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float mx = fmaxf(sc[0][t][i], sc[0][t][2 + i]);
+          float mx = -INFINITY;
 #pragma unroll
-          for (int k = 1; k < KT; ++k) mx = fmaxf(mx, fmaxf(sc[k][t][i], sc[k][t][2 + i]));
+          for (int k = 0; k < KT; ++k)
+            mx = fmaxf(mx, kFp8 ? fmaxf(sc[k][t][i] + ev[k][0], sc[k][t][2 + i] + ev[k][1]) : fmaxf(sc[k][t][i], sc[k][t][2 + i]));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
           mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
           const float m_new = fmaxf(m_run[t][i], mx);
-          const float ref = m_new == -INFINITY ? 0.f : m_new;
+          const float top = m_new == -INFINITY ? 0.f : m_new, ref = kFp8 ? top - kTop : top;
           moved |= mx > m_run[t][i];
-          corr[t][i] = ex2(m_run[t][i] - ref);
+          corr[t][i] = ex2(m_run[t][i] - top);
           float sum = 0.f;
 #pragma unroll
           for (int k = 0; k < KT; ++k)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const float x = ex2(sc[k][t][2 * h + i] - ref);
-              sc[k][t][2 * h + i] = x;
-              sum = kFp8 ? fmaf(x, inv_v[k][h], sum) : sum + x;
+              const float y = sc[k][t][2 * h + i] - ref, x = ex2(y);
+              sc[k][t][2 * h + i] = !kFp8 ? x : NT == 1 ? ex2(y + ev[k][h]) : x * vs[k][h];
+              sum += x;
             }
           l_run[t][i] = fmaf(l_run[t][i], corr[t][i], sum);
           m_run[t][i] = m_new;
@@ -443,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
             for (int i = 0; i < 4; ++i) o[t][c][i] *= corr[t][i & 1];
       }
       if (!odd_v) {
-        // the weights are rounded to the type of the V operand: bf16, or half (2^-12) for e4m3
+        // the weights are rounded to the type of the V operand: bf16 (2^-8 of each), or half (2^-11) for e4m3
         uint32_t pb[KT][NT][2];
 #pragma unroll
         for (int k = 0; k < KT; ++k)
