@@ -6,10 +6,9 @@
 // name (with no mask: nodes 0..i, a chain). One node that sees itself is
 // ordinary decode. For query head h of kv head h / G:
 //   out_i = sum_j softmax_j(scale * q_i . k_j) v_j,  0 when nothing is seen.
-// The e4m3 cache holds k_j = 2^a_j kq_j and v_j = 2^b_j vq_j; with
-// x_j = scale * log2(e) * 2^a_j (q_i . kq_j) + b_j the weights 2^(x_j - max x)
-// are at most 1 and multiply vq_j directly, and the softmax's own sum is
-// sum_j 2^(x_j - max x) 2^(-b_j): both scales cost one FMA each.
+// The e4m3 cache holds k_j = 2^a_j kq_j and v_j = 2^b_j vq_j. K's scale multiplies
+// the score; V's goes into the weight where few query rows share a V (first kernel)
+// and into V where many do (tree_attn_tc.cuh).
 #include <cuda_fp16.h>
 #include <cudaTypedefs.h>
 

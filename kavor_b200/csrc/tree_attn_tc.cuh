@@ -10,7 +10,7 @@
 // exponentials overlap the other group's and the MMAs. Both groups weigh a row
 // against the same reference, settled tile by tile (a barrier hands it from group to
 // group); it moves only when a tile's maximum passes it by 2^15: weights of up to
-// 2^15 cost nothing in bf16 or half, and the output rows are rescaled once or twice
+// 2^15 cost nothing in bf16, and the output rows are rescaled once or twice
 // in a context instead of at every tile (a rescale waits for the P V before it: with
 // 2^8, 16 x 64 nodes over e4m3 took 564 us instead of 465). Loads, MMAs and the
 // conversion of V have warps of their own, each waiting for nothing it does not need.
@@ -19,18 +19,19 @@
 // e4m3(x), lo = e4m3(x - hi), which hold a bf16 value (8 bits, two signed 4-bit
 // significands) exactly down to 2^-10 of its row's maximum, scaled to [128, 256),
 // and to 2^-18 of that maximum below it. Two e4m3 chains take as long as one
-// 16-bit chain and K is never converted. The weights need more range than e4m3
-// has (2^-18 of the largest would be lost, and 10^5 tokens can hold a fifth of
-// the sum below that), so they are halves, and four warps turn V into halves,
-// exactly.
+// 16-bit chain and K is never converted. V becomes bf16, times its row's scale: four
+// warps do that, exactly (four significant bits, every scale that is written), so V's
+// scale is in no score and no reference, whatever the rows' sizes are (a zero row is
+// held with the scale 2^0: in the scores it raised the reference by up to 2^14). The
+// weights are bf16 (2^-8 of each), as over the bf16 cache.
 //
 // Measured, 64 query heads over 8 kv heads, 16 trees of 64 nodes, 3900 to 8100
 // tokens: 278 us over bf16 (724 TFLOP/s; K and V come 3.9 times from HBM, once for each
-// of a sequence's row blocks: 5.4 TB/s), 387 over e4m3 (520). A tile takes 2400 clocks
+// of a sequence's row blocks: 5.4 TB/s), 390 over e4m3 (516). A tile takes 2400 clocks
 // over bf16, of which the two MMA chains issue for 1170 and the exponentials (16 a
-// clock) take 1024; over e4m3 4500: each score takes both scales (a softmax
-// thread's two walks and the handing over take 5000 of the 6500 between its tiles),
-// and with these inputs' wide scores a tile in five rescales some of its rows.
+// clock) take 1024. Over e4m3 each score takes K's scale and is stored between the
+// walks, V's scaling takes 27 us (363 without), and with these inputs' wide scores a
+// tile in five rescales some of its rows.
 // 64 trees of 9 to 32 nodes, 32 heads over 8, 200 to 2300 tokens of bf16: 89 us, the
 // fixed 10,000 clocks of each of the 512 units beside their 18 tiles at most.
 #pragma once
@@ -44,7 +45,7 @@ constexpr int kTile = 128;
 constexpr int kGroups = 2;                                // softmax warpgroups
 constexpr uint32_t kCols = 512;                           // S0, S1, O: 128 columns each; P0, P1: 64
 constexpr uint32_t kColO = 256, kColP = 384;
-constexpr float kSlack = 15.f;                            // log2 of the largest weight: below the largest half
+constexpr float kSlack = 15.f;                            // log2 of the largest weight
 constexpr int kHalf = kTile * 128;                        // 128 rows of 128 bytes
 constexpr int kOperand = 2 * kHalf;                       // 16-bit Q or V (two halves of 64 dims), or two e4m3 parts of Q
 // Warps 0 and 2 load K and V, 1 issues Q K^T, 3 issues P V, 4 to 7 load Q and
@@ -253,9 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ __align__(8) uint64_t q_full, q_empty, kfull[C::kStages], vfull[C::kStages], k_empty[C::kStages], v_empty[C::kStages],
       v16_full[2], v16_empty[2], s_full[2], s_empty[2], p_full[2], pv_full[2], o_empty;
   __shared__ __align__(16) uint8_t scales[kFp8 ? C::kStages : 1][2][kTile];
-  // scales 2^a (K) and 2^b (V) of a tile: 2^a, b and 2^-b; two tiles of each group. (As bf16
-  // they took half the shared memory loads and two instructions more a pair: 428 us, not 396.)
-  __shared__ __align__(16) float tok_k[kFp8 ? 4 : 1][kTile], tok_b[kFp8 ? 4 : 1][kTile], tok_i[kFp8 ? 4 : 1][kTile];
+  __shared__ __align__(16) float tok_k[kFp8 ? 4 : 1][kTile];  // scales of a tile's K rows; two tiles of each group
   __shared__ float ref_s[kRows], l_s[2][kRows];
   __shared__ float qs_s[kFp8 ? 4 : 1][kRows];  // scale of a query row's e4m3 parts, of four segments
   __shared__ uint32_t o_started;  // the output rows hold something before a segment's first P V
@@ -271,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < C::kStages; ++i) {
       mbar_init(smem_u32(&kfull[i]), 1);
       mbar_init(smem_u32(&vfull[i]), 1);
-      mbar_init(smem_u32(&k_empty[i]), kFp8 ? 5 : 1);  // the MMAs; the four warps that read the tile's scales
+      mbar_init(smem_u32(&k_empty[i]), kFp8 ? 5 : 1);  // the MMAs; the four warps that read K's scales
       mbar_init(smem_u32(&v_empty[i]), kFp8 ? 4 : 1);  // the converting warps, or the MMAs
     }
     for (int i = 0; i < 2; ++i) {
@@ -338,29 +337,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int x = 0; x < boxes; ++x) {
               const bool none = pg.absent(a, w);
               const int blk = none ? a.num_blocks : pg.blk;  // out of the tensor map: TMA fills zeros
-              if (do_k) {
-                const uint32_t bytes = C::kKV / boxes + (kFp8 && !none ? 2 * a.box : 0);  // the scales come with K
-                if (kFp8 && none) {  // zeros, of scale 1
-                  for (int i = 0; i < 2; ++i)
-                    for (int k = 0; k < a.box / 4; ++k)
-                      reinterpret_cast<uint32_t*>(&scales[st][i][x * a.box])[k] = 0x7f7f7f7fu;
-                  fence_async();  // before a later copy into the same bytes
-                }
-                if (x + 1 < boxes)
-                  mbar_expect_tx(kb, bytes);
-                else
-                  mbar_arrive_expect_tx(kb, bytes);
-                if (kFp8 && !none) {
-                  const int64_t so = blk * a.scale_stride + (int64_t)w.h * a.block_size + pg.off;
-                  bulk_load(smem_u32(&scales[st][0][x * a.box]), a.ks + so, a.box, kb);
-                  bulk_load(smem_u32(&scales[st][1][x * a.box]), a.vs + so, a.box, kb);
-                }
-                load(&kmap, kd + x * a.box * 128, pg.off, blk, kb);
+              const uint32_t bar = do_k ? kb : vb;
+              uint8_t* sc = &scales[kFp8 ? st : 0][do_k ? 0 : 1][kFp8 ? x * a.box : 0];
+              const uint32_t bytes = C::kKV / boxes + (kFp8 && !none ? a.box : 0);  // rows and their scales
+              if (kFp8 && none) {  // zeros, of scale 1
+                for (int k = 0; k < a.box / 4; ++k) reinterpret_cast<uint32_t*>(sc)[k] = 0x7f7f7f7fu;
+                fence_async();  // before a later copy into the same bytes
               }
-              if (do_v) {
-                if (x == 0) mbar_arrive_expect_tx(vb, C::kKV);
-                load(&vmap, vd + x * a.box * 128, pg.off, blk, vb);
+              if (x + 1 < boxes)
+                mbar_expect_tx(bar, bytes);
+              else
+                mbar_arrive_expect_tx(bar, bytes);
+              if (kFp8 && !none) {
+                const int64_t so = blk * a.scale_stride + (int64_t)w.h * a.block_size + pg.off;
+                bulk_load(smem_u32(sc), (do_k ? a.ks : a.vs) + so, a.box, bar);
               }
+              load(do_k ? &kmap : &vmap, (do_k ? kd : vd) + x * a.box * 128, pg.off, blk, bar);
               pg.advance(a, w, a.box);
             }
           }
@@ -374,11 +366,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     } else if (warp == 1 || warp == 3) {
       // ----------------------------------------------------------- MMA issuers
-      // fp32 accumulation, M = N = 128. Q K^T: bf16, or e4m3 parts of Q; P V: bf16
-      // or halves, V read head-dim-major (bit 16). A warp for each, so that neither
-      // waits behind what the other waits for.
+      // fp32 accumulation, M = N = 128. Q K^T: bf16, or e4m3 parts of Q; P V: bf16,
+      // V read head-dim-major (bit 16). A warp for each, so that neither waits behind
+      // what the other waits for.
       constexpr uint32_t kShape = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-      constexpr uint32_t kBf16 = kFp8 ? 0u : (1u << 7) | (1u << 10);
+      constexpr uint32_t kBf16 = (1u << 7) | (1u << 10);
       constexpr int kParts = kFp8 ? 2 : 1, kSteps = kFp8 ? 4 : 8;  // Q K^T: MMAs of 32 or 16 dims
       uint32_t it = 0, seg = 0, done[2] = {0, 0};                  // tiles, segments, tiles of each group so far
       bool ok = true;
@@ -400,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               for (int ks = 0; ks < kSteps; ++ks) {
                 // descriptors count 16 bytes
                 const uint32_t off = ((kFp8 ? 0 : (ks >> 2) * kHalf) + (ks & 3) * 32) >> 4;
-                mma<kFp8>(d, q + (part * kHalf >> 4) + off, k + off, kShape | kBf16, part > 0 || ks > 0);
+                mma<kFp8>(d, q + (part * kHalf >> 4) + off, k + off, kShape | (kFp8 ? 0u : kBf16), part > 0 || ks > 0);
               }
             commit(smem_u32(&k_empty[st]));
             if (j == w.n - 1) commit(smem_u32(&q_empty));
@@ -430,7 +422,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         done[1] += w.n >> 1;
       }
     } else {
-      // ------------------------------------- query rows; V's e4m3 bytes to halves
+      // --------------------------- query rows; V's e4m3 bytes and scales to bf16
       uint32_t it = 0;
       bool ok = true;
       const int t2 = threadIdx.x - 128;
@@ -510,11 +502,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             // 16 dims (chunk c) of token t: two 8-dim chunks of its row's half c / 4
             const int idx = i * 128 + t2, t = idx >> 3, c = idx & 7;
             const uint4 x = lds128(src + t * 128 + ((c ^ (t & 7)) << 4));
+            const float vsc = __uint_as_float((uint32_t)scales[st][1][t] << 23);
+            const uint64_t v2 = pk2(vsc, vsc);
             uint32_t y[8];
             e4m3x4_to_half(x.x, y[0], y[1]);
             e4m3x4_to_half(x.y, y[2], y[3]);
             e4m3x4_to_half(x.z, y[4], y[5]);
             e4m3x4_to_half(x.w, y[6], y[7]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&y[k]));
+              float f0, f1;
+              un2(mul2(pk2(f.x, f.y), v2), f0, f1);
+              y[k] = pack_bf16(f0, f1);
+            }
             const uint32_t row = dst + (c >> 2) * kHalf + t * 128;
             const int first = (c & 3) * 2, odd = c >> 2;  // the halves' lanes start on different banks
 #pragma unroll
@@ -571,15 +572,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int p0 = (w.t0 + j) * kTile;
         const bool tail = p0 + kTile > base;
         if constexpr (kFp8) {
-          // the tile's scales as floats, a token a thread (the buffer's last
+          // K's scales of the tile as floats, a token a thread (the buffer's last
           // readers have passed the barrier of the tile between)
           ok = ok && mbar_wait(smem_u32(&kfull[st]), phase_of(i0), &g_err_tree);
-          const uint32_t kc = scales[st][0][r], vc = scales[st][1][r];
-          float inv = __uint_as_float((254u - vc) << 23);
-          if (tail && !(inv >= 0.f && inv < INFINITY)) inv = 0.f;  // stale scale bytes
-          tok_k[tb][r] = __uint_as_float(kc << 23);
-          tok_b[tb][r] = (float)((int)vc - 127);
-          tok_i[tb][r] = inv;
+          tok_k[tb][r] = __uint_as_float((uint32_t)scales[st][0][r] << 23);
           __syncwarp();
           if (lane == 0) mbar_arrive(smem_u32(&k_empty[st]));
           named_bar_sync(bar, 128);
@@ -602,16 +598,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_row64(srow + c, v);
           if constexpr (kFp8) {
 #pragma unroll
-            for (int i = 0; i < 64; i += 8) {
-#pragma unroll
-              for (int y = 0; y < 4; y += 2) {
-                const float4 k = *reinterpret_cast<const float4*>(&tok_k[tb][c + i + 2 * y]);
-                const float4 b = *reinterpret_cast<const float4*>(&tok_b[tb][c + i + 2 * y]);
-                const uint64_t x0 = mul2(pk2(v[i + 2 * y], v[i + 2 * y + 1]), rs2);
-                const uint64_t x1 = mul2(pk2(v[i + 2 * y + 2], v[i + 2 * y + 3]), rs2);
-                un2(fma2(x0, pk2(k.x, k.y), pk2(b.x, b.y)), v[i + 2 * y], v[i + 2 * y + 1]);
-                un2(fma2(x1, pk2(k.z, k.w), pk2(b.z, b.w)), v[i + 2 * y + 2], v[i + 2 * y + 3]);
-              }
+            for (int i = 0; i < 64; i += 4) {
+              const float4 k = *reinterpret_cast<const float4*>(&tok_k[tb][c + i]);
+              un2(mul2(pk2(v[i], v[i + 1]), mul2(rs2, pk2(k.x, k.y))), v[i], v[i + 1]);
+              un2(mul2(pk2(v[i + 2], v[i + 3]), mul2(rs2, pk2(k.z, k.w))), v[i + 2], v[i + 3]);
             }
           }
           if (tail) {
@@ -687,20 +677,11 @@ __global__ void __launch_bounds__(kThreads, 1)
                 un2(kFp8 ? add2(s2, nref) : fma2(s2, rs2, nref), x0, x1);
                 x0 = ex2(x0);
                 x1 = ex2(x1);
-                p[(i & 31) / 2 + y] = kFp8 ? pack_half(x0, x1) : pack_bf16(x0, x1);
+                p[(i & 31) / 2 + y] = pack_bf16(x0, x1);
                 e[y] = pk2(x0, x1);
               }
-              if constexpr (kFp8) {
-                const float4 n0 = *reinterpret_cast<const float4*>(&tok_i[tb][c + i]);
-                const float4 n1 = *reinterpret_cast<const float4*>(&tok_i[tb][c + i + 4]);
-                sum[0] = fma2(e[0], pk2(n0.x, n0.y), sum[0]);
-                sum[1] = fma2(e[1], pk2(n0.z, n0.w), sum[1]);
-                sum[2] = fma2(e[2], pk2(n1.x, n1.y), sum[2]);
-                sum[3] = fma2(e[3], pk2(n1.z, n1.w), sum[3]);
-              } else {
 #pragma unroll
-                for (int y = 0; y < 4; ++y) sum[y] = add2(sum[y], e[y]);
-              }
+              for (int y = 0; y < 4; ++y) sum[y] = add2(sum[y], e[y]);
             }
             tmem_put16(prow + c / 2 + h * 16, p);
           }
@@ -732,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               // the whole row is looked at, so any order will do: one that starts each lane on other banks
               const int k = (c + r) & 15;
               const uint4 x = lds128(vr + (k >> 3) * kHalf + ((k & 7) << 4));
-              const uint32_t ex = kFp8 ? 0x7c007c00u : 0x7f807f80u;
+              constexpr uint32_t ex = 0x7f807f80u;
               odd |= (__vcmpeq2(x.x & ex, ex) | __vcmpeq2(x.y & ex, ex) | __vcmpeq2(x.z & ex, ex) |
                       __vcmpeq2(x.w & ex, ex)) != 0;
             }
@@ -753,15 +734,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const uint32_t bits = t < 64 ? t < 32 ? seen[0] : seen[1] : t < 96 ? seen[2] : seen[3];
                 const uint32_t two = tmem_ld1(prow + (t >> 1)) >> (t & 1 ? 16 : 0);
                 if ((bits >> (t & 31)) & 1u) {
-                  const float p = kFp8 ? __half2float(__ushort_as_half((unsigned short)two)) : __uint_as_float(two << 16);
+                  const float p = __uint_as_float(two << 16);
 #pragma unroll
                   for (int c = 0; c < 4; ++c) {
                     const uint4 y = lds128(vt + t * 128 + (d >> 1) * kHalf + ((((d & 1) * 4 + c) ^ (t & 7)) << 4));
                     const uint32_t wd[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                      const float2 f = kFp8 ? __half22float2(*reinterpret_cast<const __half2*>(&wd[i]))
-                                            : __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wd[i]));
+                      const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&wd[i]));
                       v[c * 8 + i * 2] += p * f.x;
                       v[c * 8 + i * 2 + 1] += p * f.y;
                     }

@@ -60,8 +60,9 @@ class Held:
 
 
 # query heads, kv heads, nodes of a sequence: 1 to 33 query rows a kv head in the kernel of few rows (heads a
-# unit 4, 2, 1; one and two units)
+# unit 4, 2, 1; one and two units), then more
 FEW = [(32, 8, 1), (8, 4, 6), (8, 2, 4), (8, 2, 8), (12, 2, 1), (4, 1, 4), (9, 3, 4), (8, 1, 4)]
+MANY = [(8, 2, 12), (33, 1, 1), (4, 1, 40), (16, 4, 33)]
 LENS = [300, 2000, 301, 130, 700, 2100, 64, 900]
 
 
@@ -128,4 +129,22 @@ def test_few_rows_with_value_rows_far_apart(hq, hkv, t):
 
 @pytest.mark.parametrize("hq,hkv,t", [(16, 4, 1), (8, 2, 4), (4, 1, 4)])
 def test_few_rows_with_a_zero_value_row_in_a_long_context(hq, hkv, t):
+    long_sink(hq, hkv, t, 0.9).check()
+
+@pytest.mark.parametrize("weight", [0.5, 0.85, 0.99])
+@pytest.mark.parametrize("hq,hkv,t", MANY)
+def test_many_rows_with_a_zero_value_row_that_draws_the_attention(hq, hkv, t, weight):
+    d = sinks(hq, hkv, t, weight)
+    drawn = torch.cat([d.expected(b)[2].flatten() for b in range(len(LENS))])
+    assert abs(float(drawn.mean()) - weight) < 0.15
+    d.check()
+
+
+@pytest.mark.parametrize("hq,hkv,t", MANY)
+def test_many_rows_with_value_rows_far_apart(hq, hkv, t):
+    far_apart(hq, hkv, t).check()
+
+
+@pytest.mark.parametrize("hq,hkv,t", [(16, 1, 4), (8, 2, 12)])
+def test_many_rows_with_a_zero_value_row_in_a_long_context(hq, hkv, t):
     long_sink(hq, hkv, t, 0.9).check()
