@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
                        (int64_t)((w.h + hw) * a.group + (in ? R - node * a.group : 0)) * a.q_sh;
       if constexpr (kFp8) {
         // the row over a power of two as halves: exact to 2^-25 of its largest
-        // finite value, which is brought to [1, 2)
+        // finite value, which is brought to [1, 2); to less than 2^16 where that is
+        // 2^113 or more, and to 2^-14 at least (the scale stays a normal number)
         uint2 raw[8];
         uint32_t mx = 0;
 #pragma unroll
@@ -291,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
         mx = max(mx & 0xffffu, mx >> 16);
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const int e = min(max((int)(mx >> 7) - 127, -100), 100);
+        const int e = min(max((int)(mx >> 7) - 127, -112), 112);
         const float inv = pow2(-e);
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {

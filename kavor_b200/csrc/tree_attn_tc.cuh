@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
               for (int o = 1; o < 16; o <<= 1) mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, o));
               const bool odd = (__ballot_sync(0xffffffffu, inf != 0) >> (lane & 16) & 0xffffu) != 0;
-              const int e = min(max((int)(mx >> 7) - 127 - 7, -100), 100);  // the largest to [128, 256)
+              const int e = max((int)(mx >> 7) - 127 - 7, -126);  // the largest to [128, 256), to 1 at least
               const float inv = pow2(-e);
               float f[8];
 #pragma unroll

@@ -131,6 +131,7 @@ def test_few_rows_with_value_rows_far_apart(hq, hkv, t):
 def test_few_rows_with_a_zero_value_row_in_a_long_context(hq, hkv, t):
     long_sink(hq, hkv, t, 0.9).check()
 
+
 @pytest.mark.parametrize("weight", [0.5, 0.85, 0.99])
 @pytest.mark.parametrize("hq,hkv,t", MANY)
 def test_many_rows_with_a_zero_value_row_that_draws_the_attention(hq, hkv, t, weight):
@@ -148,3 +149,14 @@ def test_many_rows_with_value_rows_far_apart(hq, hkv, t):
 @pytest.mark.parametrize("hq,hkv,t", [(16, 1, 4), (8, 2, 12)])
 def test_many_rows_with_a_zero_value_row_in_a_long_context(hq, hkv, t):
     long_sink(hq, hkv, t, 0.9).check()
+
+
+@pytest.mark.parametrize("hq,hkv,t", [(8, 2, 1), (8, 2, 4), (8, 2, 12)])
+def test_queries_and_keys_at_the_ends_of_the_range(hq, hkv, t):
+    """Queries up to 2^127 over keys of 2^-96, down to 2^-126 over keys of 2^118: scores of ordinary size."""
+    g = gen(11)
+    for q2, k2, scale in ((118, -94, 2.0 ** -29), (-118, 110, 2.0 ** 4), (126, -96, 2.0 ** -35), (-125, 118, 2.0 ** 3)):
+        ks = [(torch.randn(n, hkv, D, generator=g).double() * 2.0 ** k2).to(torch.bfloat16) for n in (200, 333)]
+        vs = [torch.randn(n, hkv, D, generator=g).to(torch.bfloat16) for n in (200, 333)]
+        qs = [(torch.randn(t, hq, D, generator=g).double().clamp(-3, 3) * 2.0 ** q2).to(torch.bfloat16) for _ in range(2)]
+        Held(ks, vs, qs, hkv, scale=scale).check()
