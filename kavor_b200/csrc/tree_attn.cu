@@ -355,6 +355,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
           }
         }
         odd_v = __any_sync(0xffffffffu, odd_v);
+        __syncwarp();  // the zeros are read by other lanes (a vote orders no memory)
       }
 
       // S^T of 16 tokens k: element 2 h + i is token 16 k + g + 8 h, row 8 t + 2 j4 + i

@@ -13,7 +13,7 @@ import math
 import pytest
 import torch
 
-from test_spec_ops_gpu import A, D, DEV, SCALE, _lib, fp8_pool, gen, held_rows, tables_for  # noqa: F401
+from test_spec_ops_gpu import A, D, DEV, SCALE, Draft, _lib, fp8_pool, gen, held_rows, tables_for  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -160,3 +160,14 @@ def test_queries_and_keys_at_the_ends_of_the_range(hq, hkv, t):
         vs = [torch.randn(n, hkv, D, generator=g).to(torch.bfloat16) for n in (200, 333)]
         qs = [(torch.randn(t, hq, D, generator=g).double().clamp(-3, 3) * 2.0 ** q2).to(torch.bfloat16) for _ in range(2)]
         Held(ks, vs, qs, hkv, scale=scale).check()
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("hq,hkv,size", [(4, 1, 1), (8, 4, 2), (16, 2, 2), (20, 1, 2)])
+def test_noise_behind_a_context_of_any_length_has_no_influence(hq, hkv, size, fp8):
+    """Contexts that end at every place of a tile, over pages whose other rows hold NaN and infinities among noise."""
+    lens = list(range(size, 132))
+    d = Draft(lens, [size] * len(lens), hq, hkv, fp8, bs=64, seed=90)
+    a, b = d.run(), d.run()
+    d.check(a)
+    assert torch.equal(a, b)
