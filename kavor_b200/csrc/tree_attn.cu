@@ -44,11 +44,11 @@ using tree::Walk;
 // 2^(s_j + b_j - m + 8). That is the row's share of the output, so what a half loses
 // (steps of 2^-24) is 2^-33 of the largest share at most. The softmax's own sum is of
 // 2^(s_j - m + 8) in 32 bits: taken from the weight, times 2^-b_j, it lost tokens whose
-// share is small only because their V is. The weight is that term times 2^b_j or, for 8
-// query rows, a second exponential (us, times 2^b_j / exponential: decode of 256 x 1024
-// tokens 100.5 / 98.6, 32 rows over 130001 tokens 44.1 / 46.4). A row of V that
-// holds nothing has the scale 2^0 and no share: it counts with kNothing for b_j, or one
-// that draws the attention would push every other weight out of a half's range.
+// share is small only because their V is. The weight is that term times 2^b_j (for 16
+// rows a second exponential was slower: 16 rows over 256 x 1024 tokens 143 us, this 138).
+// A row of V that holds nothing has the scale 2^0 and no share: it counts with kNothing
+// for b_j, or one that draws the attention would push every other weight out of a half's
+// range. Two rows go through each step together (a row at a time: 146 us).
 constexpr float kTop = 8.f;         // log2 of the largest weight over e4m3
 constexpr float kNothing = -100.f;  // the least exponent a written row can have
 constexpr int kWarps = 4;
@@ -138,6 +138,30 @@ __device__ __forceinline__ uint32_t lds16(uint32_t addr) {
   unsigned short v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
   return v;
+}
+// Packed fp32 pairs.
+__device__ __forceinline__ uint64_t pk2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void un2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
@@ -406,9 +430,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
             vs[k][h] = __uint_as_float(vc << 23);
             unit |= vc == 127u;
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-              for (int i = 0; i < 2; ++i) sc[k][t][2 * h + i] *= rscale[t][i] * ksc;
+            for (int t = 0; t < NT; ++t) {
+              float* x = &sc[k][t][2 * h];
+              un2(mul2(pk2(x[0], x[1]), mul2(pk2(rscale[t][0], rscale[t][1]), pk2(ksc, ksc))), x[0], x[1]);
+            }
           } else {
 #pragma unroll
             for (int t = 0; t < NT; ++t)
@@ -451,32 +476,45 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
       float corr[NT][2];
       bool moved = false;  // a maximum of the warp's rows rose
 #pragma unroll
-      for (int t = 0; t < NT; ++t)
+      for (int t = 0; t < NT; ++t) {
+        float mx[2] = {-INFINITY, -INFINITY}, ref[2];
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float x0 = sc[k][t][2 * h], x1 = sc[k][t][2 * h + 1];
+            if constexpr (kFp8) un2(add2(pk2(x0, x1), pk2(ev[k][h], ev[k][h])), x0, x1);
+            mx[0] = fmaxf(mx[0], x0);
+            mx[1] = fmaxf(mx[1], x1);
+          }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          float mx = -INFINITY;
-#pragma unroll
-          for (int k = 0; k < KT; ++k)
-            mx = fmaxf(mx, kFp8 ? fmaxf(sc[k][t][i] + ev[k][0], sc[k][t][2 + i] + ev[k][1]) : fmaxf(sc[k][t][i], sc[k][t][2 + i]));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float m_new = fmaxf(m_run[t][i], mx);
-          const float top = m_new == -INFINITY ? 0.f : m_new, ref = kFp8 ? top - kTop : top;
-          moved |= mx > m_run[t][i];
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 4));
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 8));
+          mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 16));
+          const float m_new = fmaxf(m_run[t][i], mx[i]);
+          const float top = m_new == -INFINITY ? 0.f : m_new;
+          ref[i] = kFp8 ? top - kTop : top;
+          moved |= mx[i] > m_run[t][i];
           corr[t][i] = ex2(m_run[t][i] - top);
-          float sum = 0.f;
-#pragma unroll
-          for (int k = 0; k < KT; ++k)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float y = sc[k][t][2 * h + i] - ref, x = ex2(y);
-              sc[k][t][2 * h + i] = !kFp8 ? x : NT == 1 ? ex2(y + ev[k][h]) : x * vs[k][h];
-              sum += x;
-            }
-          l_run[t][i] = fmaf(l_run[t][i], corr[t][i], sum);
           m_run[t][i] = m_new;
         }
+        const uint64_t nref = pk2(-ref[0], -ref[1]);
+        uint64_t sum = 0;
+#pragma unroll
+        for (int k = 0; k < KT; ++k)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float* x = &sc[k][t][2 * h];
+            un2(add2(pk2(x[0], x[1]), nref), x[0], x[1]);
+            x[0] = ex2(x[0]);
+            x[1] = ex2(x[1]);
+            const uint64_t w = pk2(x[0], x[1]);
+            sum = add2(sum, w);
+            if constexpr (kFp8) un2(mul2(w, pk2(vs[k][h], vs[k][h])), x[0], x[1]);
+          }
+        un2(fma2(pk2(l_run[t][0], l_run[t][1]), pk2(corr[t][0], corr[t][1]), sum), l_run[t][0], l_run[t][1]);
+      }
       if (__any_sync(0xffffffffu, moved)) {  // rarely after a row's first tiles; otherwise every factor is 1
 #pragma unroll
         for (int t = 0; t < NT; ++t)
