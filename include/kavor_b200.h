@@ -213,7 +213,8 @@ int kvb_store_kv_fp8(const void* key, int64_t key_stride_t, int64_t key_stride_h
 
 /* Read back whole sequences: token j of sequence b (cu_seqlens_k[b] + j, an
  * int32 prefix sum [batch + 1]) goes to row cu_seqlens_k[b] + j of k_out and
- * v_out ([total_k, num_kv_heads, 128] bf16, heads packed), exactly. Rows from
+ * v_out ([total_k, num_kv_heads, 128] bf16, heads packed), exactly (a held
+ * 2^128, from values within 1/32 of the largest bf16 value, as infinity). Rows from
  * cu_seqlens_k[batch] on are left as they are. A block id outside the pool
  * raises the device block-table error and gives zeros. */
 int kvb_load_kv_fp8(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
@@ -231,7 +232,9 @@ int kvb_load_kv_fp8(const void* k_cache, const void* v_cache, const void* k_scal
  * tree_mask's row (cu_seqlens_q[b] + i; rows mask_stride words apart,
  * mask_words of each read; one row may serve all, mask_stride 0) is set; with tree_mask NULL it sees nodes 0..i. A row that
  * sees nothing gives zeros; values of unseen nodes have no influence, whatever
- * they are. Output rows past cu_seqlens_q[batch] are left as they are.
+ * they are. fp32 scores and sums, V up to 2^90; weights rounded to bf16 (over
+ * e4m3 with at most 32 query rows a kv head to halves scaled to 2^8 of the row's
+ * largest contribution). Output rows past cu_seqlens_q[batch] are left as they are.
  * The cache is bf16 (k_scale = v_scale = NULL; block_stride in elements, as
  * kvb_paged_decode_attn) or e4m3 with its scales (strides in bytes, as above).
  * max_seqlen_q: at least the largest T_b (0 only if there are no rows); it

@@ -871,12 +871,15 @@ void fill(Variant* v) {
 // More than 16 query rows a kv head over bf16 (8, while every sequence and kv head
 // can have an SM), or 32 over e4m3 (two units of the warp-MMA kernel), take tcgen05.
 // Warp MMAs against tcgen05, us:
-// bf16, 256 sequences of 1024 tokens: 4 rows 167 / 218, 12 rows 186 / 220; 16 of
-// 3900..8100: 8 rows 72 / 73, 16 rows 78 / 73, 32 rows 121 / 75; 16 rows over 8 heads: one
-// of 100 16.4 / 13.4, 1531 18.7 / 16.4, 8000 20.5 / 21.6, 100000 81 / 78, 18 of 100..9000
-// 83 / 64, 32 of 500..1500 42 / 43.
-// e4m3, 256 of 1024: 16 rows 141 / 335, 32 rows 253 / 345; 16 of 3900..8100: 16 rows 57 /
-// 101, 32 rows 92 / 103, 48 rows 129 / 106; 130001 tokens: 32 rows 41 / 46, 48 rows 51 / 48.
+// bf16, 256 sequences of 1024 tokens: 4 rows 169 / 211, 12 rows 186 / 214; 16 of
+// 3900..8100: 8 rows 73 / 74, 16 rows 80 / 75, 32 rows 123 / 77; 16 rows over 8 heads: one
+// of 100 16.4 / 14.4, 1531 19.5 / 18.5, 8000 21.5 / 22.8, 100000 81 / 78, 18 of 100..9000
+// 84 / 66; above the SM count 32 of 500..1500 42 / 44, 128 of those 115 / 140, 32 of
+// 3900..8100 137 / 135, 24 of 9000 152 / 148, but 20 of 100..9000 87 / 72 and 40 of
+// 200..12000 183 / 167: only long and very uneven contexts lose there by the rule, and
+// the host knows no lengths.
+// e4m3, 256 of 1024: 16 rows 139 / 345, 32 rows 252 / 352; 16 of 3900..8100: 16 rows 58 /
+// 97, 32 rows 92 / 99, 48 rows 129 / 103; 130001 tokens: 32 rows 41 / 43, 48 rows 50 / 45.
 Variant variant_for(bool fp8, int batch, int hq, int hkv, int max_nodes, int block_size) {
   Variant v;
   const int64_t rows = (int64_t)(hq / hkv) * max_nodes;

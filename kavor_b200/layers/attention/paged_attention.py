@@ -38,7 +38,8 @@ def load_kvcache_fp8(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torc
                      v_out: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Read whole sequences back from an 8-bit cache: (k, v) bf16 [total_k, Hkv,
     128], sequence b at rows cu_seqlens_k[b]..cu_seqlens_k[b+1], exactly the
-    held values. ``total_k`` is the row count of the outputs; rows from
+    held values (a held 2^128, from values within 1/32 of the largest bf16
+    value, as infinity). ``total_k`` is the row count of the outputs; rows from
     cu_seqlens_k[-1] on are left as they are."""
     return K.load_kvcache_fp8(k_cache, v_cache, k_scale, v_scale, block_tables, cu_seqlens_k, total_k, k_out, v_out)
 
@@ -58,7 +59,10 @@ def tree_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor
     One node per sequence is decode. ``max_seqlen_q`` is at least the largest
     T_b. With ``k_scale``/``v_scale`` the caches are 8-bit
     (``store_kvcache_fp8``). A node that sees nothing gives zeros; what unseen
-    nodes hold has no influence. Returns [total_q, Hq, 128]; rows from
+    nodes hold has no influence. Sums are fp32; the softmax's weights are rounded
+    to bf16 before they meet V, as in the decode attention, or, over an 8-bit cache
+    with at most 32 query rows (nodes x Hq / Hkv) a kv head, to halves scaled to the
+    row's largest contribution. |V| up to 2^90. Returns [total_q, Hq, 128]; rows from
     cu_seqlens_q[-1] on are not written."""
     return K.tree_attention(q, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, max_seqlen_q, scale,
                             tree_mask, k_scale, v_scale, out)

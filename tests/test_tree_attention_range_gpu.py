@@ -171,3 +171,15 @@ def test_noise_behind_a_context_of_any_length_has_no_influence(hq, hkv, size, fp
     a, b = d.run(), d.run()
     d.check(a)
     assert torch.equal(a, b)
+
+
+def test_read_back_of_the_largest_bf16_values():
+    """1.9375 x 2^127 and more round to 2^128, the scale 2^120 times 256: infinity as bf16. The values below stay finite."""
+    x = torch.full((3, 1, D), 1.0, dtype=torch.bfloat16)
+    x[0, 0, 5], x[1, 0, 5], x[2, 0, 5] = torch.finfo(torch.bfloat16).max, -1.9375 * 2.0 ** 127, 1.9296875 * 2.0 ** 127
+    views, _ = fp8_pool(1, 64, 1)
+    A().store_kvcache_fp8(x.to(DEV), x.to(DEV), *views, torch.arange(3, dtype=torch.int32, device=DEV))
+    k, v = A().load_kvcache_fp8(*views, torch.zeros(1, 1, dtype=torch.int32, device=DEV),
+                                torch.tensor([0, 3], dtype=torch.int32, device=DEV), 3)
+    assert k[:, 0, 5].tolist() == [math.inf, -math.inf, 1.875 * 2.0 ** 127] and torch.equal(k, v)
+    assert (k[:, 0, :5] == 0).all()
