@@ -48,7 +48,10 @@ using tree::Walk;
 // rows a second exponential was slower: 16 rows over 256 x 1024 tokens 143 us, this 138).
 // A row of V that holds nothing has the scale 2^0 and no share: it counts with kNothing
 // for b_j, or one that draws the attention would push every other weight out of a half's
-// range. Two rows go through each step together (a row at a time: 146 us).
+// range. Two rows go through each step together (a row at a time: 146 us). A reference
+// can lie 2^220 above the one before it (a block of large rows of V after one of zeros)
+// while the sum so far, up to 2^108 a token, still counts: it is scaled in two steps of
+// half the way.
 constexpr float kTop = 8.f;         // log2 of the largest weight over e4m3
 constexpr float kNothing = -100.f;  // the least exponent a written row can have
 constexpr int kWarps = 4;
@@ -473,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
           }
         }
       }
-      float corr[NT][2];
+      float half[NT][2];   // a row's references before this tile and after it: the root of the factor between them
       bool moved = false;  // a maximum of the warp's rows rose
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
@@ -496,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
           const float top = m_new == -INFINITY ? 0.f : m_new;
           ref[i] = kFp8 ? top - kTop : top;
           moved |= mx[i] > m_run[t][i];
-          corr[t][i] = ex2(m_run[t][i] - top);
+          half[t][i] = ex2(0.5f * (m_run[t][i] - top));
           m_run[t][i] = m_new;
         }
         const uint64_t nref = pk2(-ref[0], -ref[1]);
@@ -513,7 +516,8 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
             sum = add2(sum, w);
             if constexpr (kFp8) un2(mul2(w, pk2(vs[k][h], vs[k][h])), x[0], x[1]);
           }
-        un2(fma2(pk2(l_run[t][0], l_run[t][1]), pk2(corr[t][0], corr[t][1]), sum), l_run[t][0], l_run[t][1]);
+        const uint64_t f = pk2(half[t][0], half[t][1]);
+        un2(fma2(mul2(pk2(l_run[t][0], l_run[t][1]), f), f, sum), l_run[t][0], l_run[t][1]);
       }
       if (__any_sync(0xffffffffu, moved)) {  // rarely after a row's first tiles; otherwise every factor is 1
 #pragma unroll
@@ -521,7 +525,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
 #pragma unroll
           for (int c = 0; c < 8; ++c)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[t][c][i] *= corr[t][i & 1];
+            for (int i = 0; i < 4; ++i) o[t][c][i] *= half[t][i & 1] * half[t][i & 1];
       }
       if (!odd_v) {
         // the weights are rounded to the type of the V operand: bf16 (2^-8 of each), or half (2^-11) for e4m3
@@ -654,7 +658,7 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
 #pragma unroll
           for (int v = 0; v < C::kGroups; ++v) M = fmaxf(M, mw[v * HP + hw][t * 8 + 2 * j4 + i]);
           // a warp whose tokens were all masked contributes nothing (its rows are 0)
-          f[t][i] = m_run[t][i] == -INFINITY ? 0.f : ex2(m_run[t][i] - M);
+          f[t][i] = m_run[t][i] == -INFINITY ? 0.f : ex2(m_run[t][i] - M);  // 0 far below M, as the rows are
         }
 #pragma unroll 1
       for (int turn = 0; turn < C::kGroups; ++turn) {
@@ -688,8 +692,10 @@ __global__ void __launch_bounds__(kThreads, (Cfg<kFp8, NT, HP>::kCtas))
 #pragma unroll
       for (int v = 0; v < C::kGroups; ++v) M = fmaxf(M, mw[v * HP + hh][row]);
 #pragma unroll
-      for (int v = 0; v < C::kGroups; ++v)
-        L += (mw[v * HP + hh][row] == -INFINITY ? 0.f : ex2(mw[v * HP + hh][row] - M)) * lw[v * HP + hh][row];  // keeps NaN
+      for (int v = 0; v < C::kGroups; ++v) {
+        const float e = mw[v * HP + hh][row] == -INFINITY ? 0.f : ex2(0.5f * (mw[v * HP + hh][row] - M));
+        L += lw[v * HP + hh][row] * e * e;  // keeps NaN
+      }
       if (!ok) M = -INFINITY, L = 0.f;
       const float* sp = scratch + hrow * kScratchStride + d0;
       if (nd < w.s.nodes) {
@@ -744,9 +750,11 @@ struct Joined {
 };
 __device__ __forceinline__ void join(Joined& x, float m, float l, const float4& o) {
   const float m_new = fmaxf(x.m, m);
-  // a part in which the row saw nothing (m = -inf) adds 0
-  const float f0 = x.m == -INFINITY ? 0.f : ex2(x.m - m_new), f1 = m == -INFINITY ? 0.f : ex2(m - m_new);
-  x.l = x.l * f0 + l * f1;
+  // A part in which the row saw nothing (m = -inf) adds 0. The sums are scaled in two
+  // steps: they count even where the rows, far below the new reference, do not.
+  const float h0 = x.m == -INFINITY ? 0.f : ex2(0.5f * (x.m - m_new)), h1 = m == -INFINITY ? 0.f : ex2(0.5f * (m - m_new));
+  const float f0 = h0 * h0, f1 = h1 * h1;
+  x.l = x.l * h0 * h0 + l * h1 * h1;
   x.o.x = x.o.x * f0 + o.x * f1;
   x.o.y = x.o.y * f0 + o.y * f1;
   x.o.z = x.o.z * f0 + o.z * f1;

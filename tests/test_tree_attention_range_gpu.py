@@ -151,6 +151,21 @@ def test_many_rows_with_a_zero_value_row_in_a_long_context(hq, hkv, t):
     long_sink(hq, hkv, t, 0.9).check()
 
 
+@pytest.mark.parametrize("apart", [16, 32, 128, 400])
+@pytest.mark.parametrize("hq,hkv,t", [*FEW, *MANY])
+def test_blocks_of_value_rows_far_apart(hq, hkv, t, apart):
+    """Blocks of zero or tiny rows beside blocks of large ones: the reference jumps from tile to tile, warp to warp
+    and part to part, and half of the softmax's sum is under rows that add nothing."""
+    g = gen(13)
+    ks, vs, qs = [], [], []
+    for n, low, high in ((900, 0.0, 1e12), (1300, 1e-25, 1e20), (800, 0.0, 1e25), (700, 1e25, 0.0), (1000, 1e20, 1e-25)):
+        k, v = (torch.randn(n, hkv, D, generator=g) for _ in range(2))
+        v *= torch.where(torch.arange(n) // apart % 2 == 0, low, high).view(n, 1, 1)
+        ks.append(k.to(torch.bfloat16)), vs.append(v.to(torch.bfloat16))
+        qs.append(torch.randn(t, hq, D, generator=g).to(torch.bfloat16))
+    Held(ks, vs, qs, hkv, seed=2).check()
+
+
 @pytest.mark.parametrize("hq,hkv,t", [(8, 2, 1), (8, 2, 4), (8, 2, 12)])
 def test_queries_and_keys_at_the_ends_of_the_range(hq, hkv, t):
     """Queries up to 2^127 over keys of 2^-96, down to 2^-126 over keys of 2^118: scores of ordinary size."""
