@@ -45,7 +45,7 @@ using tree::Walk;
 // (steps of 2^-24) is 2^-33 of the largest share at most. The softmax's own sum is of
 // 2^(s_j - m + 8) in 32 bits: taken from the weight, times 2^-b_j, it lost tokens whose
 // share is small only because their V is. The weight is that term times 2^b_j (for 16
-// rows a second exponential was slower: 16 rows over 256 x 1024 tokens 143 us, this 138).
+// rows a second exponential was slower: 16 rows over 256 x 1024 tokens 143 us, this 139).
 // A row of V that holds nothing has the scale 2^0 and no share: it counts with kNothing
 // for b_j, or one that draws the attention would push every other weight out of a half's
 // range. Two rows go through each step together (a row at a time: 146 us). A reference
@@ -886,7 +886,7 @@ void fill(Variant* v) {
 // 3900..8100 137 / 135, 24 of 9000 152 / 148, but 20 of 100..9000 87 / 72 and 40 of
 // 200..12000 183 / 167: only long and very uneven contexts lose there by the rule, and
 // the host knows no lengths.
-// e4m3, 256 of 1024: 16 rows 139 / 345, 32 rows 252 / 352; 16 of 3900..8100: 16 rows 58 /
+// e4m3, 256 of 1024: 16 rows 139 / 345, 32 rows 253 / 352; 16 of 3900..8100: 16 rows 58 /
 // 97, 32 rows 92 / 99, 48 rows 129 / 103; 130001 tokens: 32 rows 41 / 43, 48 rows 50 / 45.
 Variant variant_for(bool fp8, int batch, int hq, int hkv, int max_nodes, int block_size) {
   Variant v;
